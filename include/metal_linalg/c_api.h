@@ -121,6 +121,124 @@ const char* metal_linalg_svd_backend(uint32_t rows, uint32_t cols, uint32_t batc
 const char* metal_linalg_svdvals_backend(uint32_t rows, uint32_t cols, uint32_t batch);   /* values alone */
 
 /* ---------------------------------------------------------------------------
+ * The gated delta rule: a sequence of decayed reflections (no counterpart in
+ * the reference)
+ * ------------------------------------------------------------------------- */
+
+/* Element types of the operators below. */
+typedef enum metal_linalg_dtype {
+    METAL_LINALG_FLOAT32     = 0,
+    METAL_LINALG_BFLOAT16    = 1,
+    METAL_LINALG_FLOAT16     = 2,
+    METAL_LINALG_FLOAT8_E4M3 = 3,
+    METAL_LINALG_FLOAT8_E5M2 = 4,
+} metal_linalg_dtype;
+
+/* The inputs of one call. For every value head h a state S [key_dim, value_dim]
+ * (float32) runs through the tokens of its sequence,
+ *
+ *     S <- exp(g_t) S;   d_t = beta_t (v_t - S^T k_t);   S <- S + k_t d_t^T;   o_t = scale S^T q_t,
+ *
+ * that is S <- exp(g_t) (I - beta_t k_t k_t^T) S + beta_t k_t v_t^T: products of the
+ * (generalised) reflections this library's QR is made of. Value head h reads q
+ * and k of head h / (value_heads / heads).
+ *
+ * q, k [batch, tokens, heads, key_dim] and v [batch, tokens, value_heads,
+ * value_dim] have element type `dtype` (float32, bfloat16 or float16), g and
+ * beta [batch, tokens, value_heads] are float32. The last dimension of q, k and
+ * v is contiguous; *_stride are the elements between batches, tokens and heads.
+ * key_dim <= 128, value_dim <= 256, value_heads a multiple of heads.
+ *
+ * Sequences: with `sequences` 0 every batch row is one. Otherwise batch is 1 and
+ * sequence i is the tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (index_bytes 4:
+ * int32, 8: int64; sequences + 1 values, the first 0, none falling). Tokens
+ * behind the last sequence give outputs and gradients of zero. A sequence may be empty: its state
+ * passes through.
+ *
+ * All pointers are CUDA device pointers on one GPU; the work is enqueued on the
+ * calling thread's stream (metal_linalg_set_stream). Nothing is allocated: the
+ * caller gives the workspace, so that calls on several streams, or in several
+ * captured graphs, each have their own. */
+typedef struct metal_linalg_delta {
+    uint32_t     batch, tokens, heads, value_heads, key_dim, value_dim;
+    uint32_t     sequences;
+    uint32_t     dtype;                                       /* a metal_linalg_dtype */
+    uint32_t     index_bytes;                                 /* of cu_seqlens and slots: 4 or 8 */
+    float        scale;
+    const void  *q, *k, *v;
+    const float *g, *beta;
+    const float *initial_state;                               /* [sequences or batch, value_heads, key_dim, value_dim], or NULL: zero */
+    const void  *cu_seqlens;
+    int64_t      q_stride[3], k_stride[3], v_stride[3], g_stride[3], beta_stride[3];
+} metal_linalg_delta;
+
+/* o [batch, tokens, value_heads, value_dim] of type `dtype` and final_state (as
+ * initial_state; NULL if not wanted), both contiguous. workspace: at least
+ * metal_linalg_gated_delta_rule_workspace_bytes(p, 0) bytes, on a 256-byte
+ * boundary; the function returns 0 for a problem that the call would refuse. */
+metal_linalg_status metal_linalg_gated_delta_rule(const metal_linalg_delta* p, void* o, float* final_state,
+                                                  void* workspace, uint64_t workspace_bytes);
+uint64_t            metal_linalg_gated_delta_rule_workspace_bytes(const metal_linalg_delta* p, int backward);
+
+/* The gradients from d_o (type `dtype`, strides of batches, tokens and heads, last
+ * dimension contiguous) and d_final_state (contiguous; NULL: zero). The forward is
+ * computed again from the inputs, so nothing of it has to be kept. dq, dk, dv (type
+ * `dtype`), dg, dbeta (float32) and d_initial_state (NULL if not wanted) are
+ * contiguous in the shapes of what they belong to. */
+metal_linalg_status metal_linalg_gated_delta_rule_backward(const metal_linalg_delta* p, const void* d_o,
+                                                           const int64_t* d_o_stride, const float* d_final_state,
+                                                           void* dq, void* dk, void* dv, float* dg, float* dbeta,
+                                                           float* d_initial_state, void* workspace,
+                                                           uint64_t workspace_bytes);
+
+/* A few tokens a sequence, for decoding: batch row b runs its tokens through the
+ * state in slot slots[b] of a pool [pool_size, value_heads, key_dim, value_dim]
+ * (float32, pool_stride elements between slots, the rest contiguous), in place.
+ * slots NULL: row b has slot b. A row whose slot is not in 0 .. pool_size - 1 is padding: its
+ * outputs are zero and no state is touched. Rows that name the same slot are run
+ * one after another in the order of the rows. initial_state, cu_seqlens and
+ * sequences of `p` are not looked at. Needs no workspace. */
+metal_linalg_status metal_linalg_gated_delta_step(const metal_linalg_delta* p, void* o, float* pool, int64_t pool_stride,
+                                                  uint32_t pool_size, const void* slots);
+
+/* ---------------------------------------------------------------------------
+ * Products of matrices in 8-bit floating point with a scale for each block of
+ * 128 (no counterpart in the reference)
+ * ------------------------------------------------------------------------- */
+
+/* x [batch, rows, cols] (float32, bfloat16 or float16; strides in elements between
+ * matrices, rows and columns, one of the last two being 1) to `values` of type
+ * `kind` (METAL_LINALG_FLOAT8_E4M3 or _E5M2; rows `values_stride` bytes apart,
+ * matrices rows * values_stride) and a float32 scale for each block of
+ * block_rows (1 or 128) x 128: scale = max(max|x| / M, 2^-126) with M the type's
+ * largest value (448 or 57344), value = x / scale, a float32 rounded to the nearest, ties to even.
+ * scales [batch, ceil(rows / block_rows), ceil(cols / 128)]. A block with a NaN or an
+ * infinity stands for NaN throughout. (A transposed matrix is given by its strides.) */
+metal_linalg_status metal_linalg_quantize_fp8(const void* x, metal_linalg_dtype dtype, uint32_t batch, uint32_t rows,
+                                              uint32_t cols, int64_t batch_stride, int64_t row_stride, int64_t col_stride,
+                                              uint32_t block_rows, metal_linalg_dtype kind, void* values,
+                                              uint64_t values_stride, float* scales);
+
+/* One operand of metal_linalg_matmul_fp8: `values` with k contiguous, rows
+ * `stride` bytes and matrices `batch_stride` bytes apart (0: one matrix for the
+ * whole batch; else a multiple of `stride`), all multiples of 16 as the address is; scales contiguous, one for each block of
+ * block_rows (1 or 128) x 128, matrices ceil(rows / block_rows) * ceil(k / 128) floats apart (none
+ * where batch_stride is 0). */
+typedef struct metal_linalg_fp8_operand {
+    const void*  values;
+    const float* scales;
+    uint64_t     stride, batch_stride;
+    uint32_t     kind;                                        /* METAL_LINALG_FLOAT8_E4M3 or _E5M2 */
+    uint32_t     block_rows;
+} metal_linalg_fp8_operand;
+
+/* c [batch, m, n] = a [batch, m, k] b [batch, n, k]^T (float32, bfloat16 or float16, contiguous):
+ * products of 128 along k on the tensor cores, times both blocks' scales and summed in float32. */
+metal_linalg_status metal_linalg_matmul_fp8(const metal_linalg_fp8_operand* a, const metal_linalg_fp8_operand* b,
+                                            uint32_t batch, uint32_t m, uint32_t n, uint32_t k, void* c,
+                                            metal_linalg_dtype c_dtype);
+
+/* ---------------------------------------------------------------------------
  * CUDA placement (no counterpart in the reference, whose memory is unified)
  * ------------------------------------------------------------------------- */
 

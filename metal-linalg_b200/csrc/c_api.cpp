@@ -8,6 +8,8 @@
 #include <metal_linalg/c_api.h>
 #include <metal_linalg/core.h>
 
+#include "delta.h"
+#include "fp8.h"
 #include "kernels.h"
 #include "runtime.h"
 
@@ -184,6 +186,60 @@ const char* metal_linalg_svd_backend(uint32_t rows, uint32_t cols, uint32_t batc
 const char* metal_linalg_svdvals_backend(uint32_t rows, uint32_t cols, uint32_t batch) {
     return query<const char*>("unavailable", [&] {
         return ml::svdvals_backend(rows, cols, batch) == ml::SvdBackend::qr_jacobi ? "qr_jacobi" : "unavailable";
+    });
+}
+
+// ---------------------------------------------------------------------------
+// The gated delta rule
+// ---------------------------------------------------------------------------
+
+static const metal_linalg_delta& there(const metal_linalg_delta* p, const char* who) {
+    if (!p) throw std::invalid_argument(std::string(who) + " p is NULL");
+    return *p;
+}
+
+metal_linalg_status metal_linalg_gated_delta_rule(const metal_linalg_delta* p, void* o, float* final_state, void* workspace,
+                                                  uint64_t workspace_bytes) {
+    return run([&] { ml::core::gated_delta_rule(there(p, "[gated_delta_rule]"), o, final_state, workspace, workspace_bytes); });
+}
+
+uint64_t metal_linalg_gated_delta_rule_workspace_bytes(const metal_linalg_delta* p, int backward) {
+    return query<uint64_t>(0, [&] { return ml::core::gated_delta_rule_workspace_bytes(there(p, "[gated_delta_rule]"), backward != 0); });
+}
+
+metal_linalg_status metal_linalg_gated_delta_rule_backward(const metal_linalg_delta* p, const void* d_o, const int64_t* d_o_stride,
+                                                           const float* d_final_state, void* dq, void* dk, void* dv, float* dg,
+                                                           float* dbeta, float* d_initial_state, void* workspace,
+                                                           uint64_t workspace_bytes) {
+    return run([&] {
+        ml::core::gated_delta_rule_backward(there(p, "[gated_delta_rule_backward]"), d_o, d_o_stride, d_final_state, dq, dk, dv, dg,
+                                            dbeta, d_initial_state, workspace, workspace_bytes);
+    });
+}
+
+metal_linalg_status metal_linalg_gated_delta_step(const metal_linalg_delta* p, void* o, float* pool, int64_t pool_stride,
+                                                  uint32_t pool_size, const void* slots) {
+    return run([&] { ml::core::gated_delta_step(there(p, "[gated_delta_step]"), o, pool, pool_stride, pool_size, slots); });
+}
+
+// ---------------------------------------------------------------------------
+// Products in 8-bit floating point
+// ---------------------------------------------------------------------------
+
+metal_linalg_status metal_linalg_quantize_fp8(const void* x, metal_linalg_dtype dtype, uint32_t batch, uint32_t rows, uint32_t cols,
+                                              int64_t batch_stride, int64_t row_stride, int64_t col_stride, uint32_t block_rows,
+                                              metal_linalg_dtype kind, void* values, uint64_t values_stride, float* scales) {
+    return run([&] {
+        ml::core::quantize_fp8(x, (uint32_t)dtype, batch, rows, cols, batch_stride, row_stride, col_stride, block_rows, (uint32_t)kind,
+                               values, values_stride, scales);
+    });
+}
+
+metal_linalg_status metal_linalg_matmul_fp8(const metal_linalg_fp8_operand* a, const metal_linalg_fp8_operand* b, uint32_t batch,
+                                            uint32_t m, uint32_t n, uint32_t k, void* c, metal_linalg_dtype c_dtype) {
+    return run([&] {
+        if (!a || !b) throw std::invalid_argument("[matmul_fp8] an operand is NULL");
+        ml::core::matmul_fp8(*a, *b, batch, m, n, k, c, (uint32_t)c_dtype);
     });
 }
 

@@ -1,0 +1,583 @@
+// The gated delta rule's forward kernels: the table of chunks, T and the decays (a chunk a block), the sequential pass
+// over chunks (16 value columns a chain of products), the outputs (a chunk a block). The formulas stand in delta.h.
+#include "delta.h"
+#include "delta_tiles.cuh"
+#include "runtime.h"
+
+namespace mlb {
+namespace delta {
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// Ragged batches: chunk c's first token, length and sequence; every sequence's first chunk
+// ---------------------------------------------------------------------------
+
+constexpr int kIndexThreads = 256;
+
+__device__ __forceinline__ long long cu_at(const Args& a, uint32_t i) {
+    return a.cu64 ? static_cast<const long long*>(a.cu)[i] : (long long)static_cast<const int*>(a.cu)[i];
+}
+// The bounds of sequence i, whatever cu_seqlens holds: inside the tokens, and not before their start.
+__device__ __forceinline__ void bounds_at(const Args& a, uint32_t i, int& begin, int& end) {
+    const long long total = a.tokens;
+    const long long b = min(max(cu_at(a, i), 0ll), total), e = min(max(cu_at(a, i + 1), b), total);
+    begin = (int)b;
+    end = (int)e;
+}
+
+__global__ void __launch_bounds__(kIndexThreads) delta_index_kernel(const Args a) {
+    __shared__ int sums[kIndexThreads];
+    __shared__ int carry;
+    if (threadIdx.x == 0) carry = 0;
+    __syncthreads();
+    for (uint32_t s0 = 0; s0 < a.sequences; s0 += kIndexThreads) {
+        const uint32_t s = s0 + threadIdx.x;
+        int begin = 0, end = 0;
+        if (s < a.sequences) bounds_at(a, s, begin, end);
+        const int mine = (end - begin + kChunk - 1) / kChunk;
+        sums[threadIdx.x] = mine;
+        __syncthreads();
+        for (int o = 1; o < kIndexThreads; o *= 2) {
+            const int v = threadIdx.x >= o ? sums[threadIdx.x - o] : 0;
+            __syncthreads();
+            sums[threadIdx.x] += v;
+            __syncthreads();
+        }
+        // sequences that overlap (a falling cu_seqlens) could name more chunks than there is room for: none behind it
+        const int first = min(carry + sums[threadIdx.x] - mine, (int)a.chunks);
+        const int last = min(carry + sums[threadIdx.x], (int)a.chunks);
+        if (s < a.sequences) {
+            a.first[s] = first;
+            for (int c = first; c < last; ++c) {
+                const int t = begin + (c - first) * kChunk;
+                reinterpret_cast<int4*>(a.table)[c] = make_int4(t, min(kChunk, end - t), (int)s, 0);
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) carry += sums[kIndexThreads - 1];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        int begin, end;
+        bounds_at(a, a.sequences - 1, begin, end);
+        a.first[a.sequences] = min(carry, (int)a.chunks);
+        a.first[a.sequences + 1] = end;             // tokens from here on belong to no sequence
+    }
+}
+
+// ---------------------------------------------------------------------------
+// T = (I + A)^-1 and the decays
+// ---------------------------------------------------------------------------
+//
+// A block takes a chunk and a q/k head: K K^T once, then for every value head that reads it A, its inverse by blocks of
+// 16 (diagonal blocks by substitution, a column a lane; T_ij = -T_ii sum_m A_im T_mj outward from the diagonal on the
+// tensor cores, whose transposed inner product is the outer one's operand as it stands) and T as fragments for the
+// products that follow.
+constexpr int kPrepThreads = 128;
+constexpr int kLdA = 72;            // row length of A and T in shared memory: 64-bit reads of a fragment meet no bank twice
+
+template <typename T, int DKP>
+struct PrepShared {
+    T      k[kChunk * (DKP + 8)];
+    float  kk[kChunk * kLdA];
+    float  a[kChunk * kLdA];
+    float  t[kChunk * kLdA];
+    Gates  gates;
+};
+
+template <typename T, int DKP>
+__global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const Args p, bool backward) {
+    extern __shared__ __align__(16) char raw[];
+    PrepShared<T, DKP>& sh = *reinterpret_cast<PrepShared<T, DKP>*>(raw);
+    constexpr int LD = DKP + 8;
+    const uint32_t c = blockIdx.x, h = blockIdx.y;
+    const Chunk ch = chunk_at(p, c);
+    if (ch.rows == 0) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    load_rows<T, kPrepThreads>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
+    cp_commit();
+    cp_wait<0>();
+    __syncthreads();
+    {       // K K^T: warp w the rows 16 w .. 16 w + 15, columns up to the diagonal's
+        float acc[8][4] = {};
+#pragma unroll
+        for (int k0 = 0; k0 < DKP; k0 += 16) {
+            if (warp >= 2) mma_rows_rows<T, 8>(acc, sh.k, LD, 16 * warp, sh.k, LD, 0, k0);
+            else           mma_rows_rows<T, 4>(reinterpret_cast<float (&)[4][4]>(acc), sh.k, LD, 16 * warp, sh.k, LD, 0, k0);
+        }
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            *reinterpret_cast<float2*>(&sh.kk[(16 * warp + g) * kLdA + 8 * n + 2 * t]) = make_float2(acc[n][0], acc[n][1]);
+            *reinterpret_cast<float2*>(&sh.kk[(16 * warp + 8 + g) * kLdA + 8 * n + 2 * t]) = make_float2(acc[n][2], acc[n][3]);
+        }
+    }
+    const uint32_t up = p.value_heads / p.heads;
+    for (uint32_t i = 0; i < up; ++i) {
+        const uint32_t hv = h * up + i;
+        const size_t at = (size_t)c * p.value_heads + hv;
+        if (warp == 0) {            // the gates' sums, two tokens a lane
+            double x[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int r = 2 * lane + j;
+                const float gate = r < ch.rows ? p.g[at3(p.g_stride, ch.batch, ch.token + r, hv)] : 0.0f;
+                // e^-256 is zero in float32 with room to spare: a gate that closes for good, or -inf, adds no more than that,
+                // so that the sums behind it keep their last bits
+                x[j] = gate < -256.0f ? -256.0 : (double)gate;
+                sh.gates.beta[r] = r < ch.rows ? p.beta[at3(p.beta_stride, ch.batch, ch.token + r, hv)] : 0.0f;
+            }
+            double sum = x[0] + x[1];
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const double v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += v;
+            }
+            const double end = __shfl_sync(0xffffffffu, sum, 31);
+            sh.gates.sum[2 * lane] = sum - x[1];
+            sh.gates.sum[2 * lane + 1] = sum;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const double s = j ? sum : sum - x[1];
+                sh.gates.e[2 * lane + j] = exp_of(s);
+                sh.gates.left[2 * lane + j] = exp_of(end - s);
+            }
+        }
+        __syncthreads();
+        {
+            const float* src = reinterpret_cast<const float*>(&sh.gates);
+            float* dst = reinterpret_cast<float*>(p.gates + at);
+            for (int j = threadIdx.x; j < (int)(sizeof(Gates) / 4); j += kPrepThreads) dst[j] = src[j];
+        }
+        for (int j = threadIdx.x; j < kChunk * kChunk; j += kPrepThreads) {
+            const int r = j >> 6, q = j & 63;
+            sh.a[r * kLdA + q] = q < r ? sh.gates.beta[r] * exp_of(sh.gates.sum[r] - sh.gates.sum[q]) * sh.kk[r * kLdA + q] : 0.0f;
+            sh.t[r * kLdA + q] = 0.0f;
+        }
+        __syncthreads();
+        if (lane < 16) {            // diagonal blocks: column `lane` of block `warp`
+            const float* a = sh.a + (16 * warp) * kLdA + 16 * warp;
+            float x[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float v = r == lane ? 1.0f : 0.0f;
+#pragma unroll
+                for (int m = 0; m < r; ++m) v = fmaf(-a[r * kLdA + m], x[m], v);
+                x[r] = v;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sh.t[(16 * warp + r) * kLdA + 16 * warp + lane] = x[r];
+        }
+        __syncthreads();
+        for (int dist = 1; dist < 4; ++dist) {
+            if (warp < 4 - dist) {
+                const int bj = warp, bi = warp + dist;
+                float w[2][4] = {};                                     // W^T, W = sum_m A_im T_mj: rows are T's columns
+                for (int m = bj; m < bi; ++m) {
+                    const float* tm = sh.t + (16 * m) * kLdA + 16 * bj;     // T_mj
+                    const float* am = sh.a + (16 * bi) * kLdA + 16 * m;     // A_im
+                    const float x[4] = {tm[2 * t * kLdA + g], tm[(2 * t + 1) * kLdA + g], tm[2 * t * kLdA + g + 8], tm[(2 * t + 1) * kLdA + g + 8]};
+                    const float y[4] = {tm[(2 * t + 8) * kLdA + g], tm[(2 * t + 9) * kLdA + g], tm[(2 * t + 8) * kLdA + g + 8],
+                                        tm[(2 * t + 9) * kLdA + g + 8]};
+                    SplitTf32 s;
+                    s.set(x, y);
+                    mma_tile<float, 2, false>(w, s, am, kLdA, 0, 0);
+                }
+                float out[2][4] = {};
+                const float* ti = sh.t + (16 * bi) * kLdA + 16 * bi;        // T_ii
+#pragma unroll
+                for (int k8 = 0; k8 < 2; ++k8) {
+                    const float2 u = *reinterpret_cast<const float2*>(ti + g * kLdA + 8 * k8 + 2 * t);
+                    const float2 v = *reinterpret_cast<const float2*>(ti + (g + 8) * kLdA + 8 * k8 + 2 * t);
+                    const float x[4] = {-u.x, -u.y, -v.x, -v.y};
+                    SplitTf32x8 s;
+                    s.set(x);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const uint4 b = split_pair(w[k8][2 * n], w[k8][2 * n + 1]);
+#pragma unroll
+                        for (int term = 0; term < 3; ++term) mma_term8(out[n], s, b, term);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    float* o = sh.t + (16 * bi + g) * kLdA + 16 * bj + 8 * n + 2 * t;
+                    *reinterpret_cast<float2*>(o) = make_float2(out[n][0], out[n][1]);
+                    *reinterpret_cast<float2*>(o + 8 * kLdA) = make_float2(out[n][2], out[n][3]);
+                }
+            }
+            __syncthreads();
+        }
+        for (int tile = warp; tile < kTriTiles; tile += kPrepThreads / 32) {
+            int ti = 0;
+            while (tri_tile(ti + 1, 0) <= tile) ++ti;
+            const int tj = tile - tri_tile(ti, 0);
+            const float2 f = *reinterpret_cast<const float2*>(sh.t + (8 * ti + g) * kLdA + 8 * tj + 2 * t);
+            reinterpret_cast<uint4*>(p.tri + at * kTriFloats)[tile * 32 + lane] = split_pair(f.x, f.y);
+            if (backward)
+                reinterpret_cast<uint4*>(p.tri_b + at * kTriFloats)[tile * 32 + lane] =
+                    split_pair(sh.t[(8 * ti + 2 * t) * kLdA + 8 * tj + g], sh.t[(8 * ti + 2 * t + 1) * kLdA + 8 * tj + g]);
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The sequential pass
+// ---------------------------------------------------------------------------
+//
+// A chain is 16 value columns: S^T [16 x dk] lives in accumulators. X^T = S^T K^T; R^T = beta (V^T - e^G X^T);
+// D^T = R^T T^T; S^T = e^{G_63} S^T + (D^T e^{G_63 - G}) K: every product's accumulators are the next one's A operand, and K
+// comes from shared memory as B operands both ways round. KS warps share a chain where there are too few chains to fill the
+// GPU: each holds dk / KS of S's rows, and partial X, R and D cross through shared memory as whole fragments (a lane's 16
+// bytes, no bank met twice).
+constexpr int kStateThreads = 128;
+
+template <typename T, int DKP, int KS>
+struct StateShared {
+    static constexpr int kGroups = 4 / KS;          // chains of a block
+    static constexpr int kLdV = 16 * kGroups + 8;
+    struct Stage {
+        alignas(16) T     k[kChunk * (DKP + 8)];
+        alignas(16) T     v[kChunk * kLdV];
+        alignas(16) float tri[kTriFloats];
+        alignas(16) float gates[3 * kChunk];        // e, left, beta
+    } stage[2];
+    alignas(16) float part[KS > 1 ? 4 * 8 * 32 * 4 : 4];       // [warp][tile][lane][4]: partial X
+    alignas(16) float whole[KS > 1 ? 2 * kGroups * 8 * 32 * 4 : 4];   // R, then D: [which][chain][tile][lane][4]
+};
+
+template <typename T, int DKP, int KS>
+__global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p) {
+    using Sh = StateShared<T, DKP, KS>;
+    using Sp = typename Split<T>::type;
+    extern __shared__ __align__(16) char raw[];
+    Sh& sh = *reinterpret_cast<Sh*>(raw);
+    constexpr int LD = DKP + 8, NT = DKP / 8 / KS;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int chain = warp / KS, part = warp % KS;
+    const uint32_t hv = blockIdx.y, seq = blockIdx.z, h = hv / (p.value_heads / p.heads);
+    const int dv_block = blockIdx.x * 16 * Sh::kGroups, dv0 = dv_block + 16 * chain, k_base = part * NT * 8;
+    const bool live = dv0 < (int)p.dvp;                 // a chain past the last columns computes on zeros and writes nothing
+    uint32_t c0, c1;
+    if (p.sequences) {
+        c0 = p.first[seq];
+        c1 = p.first[seq + 1];
+    } else {
+        c0 = seq * p.row_chunks;
+        c1 = c0 + p.row_chunks;
+    }
+
+    float s[NT][4];
+    const size_t state0 = ((size_t)seq * p.value_heads + hv) * p.dk * p.dv;
+    const auto col = [&](int i) { return dv0 + g + 8 * (i >> 1); };
+    const auto row = [&](int n, int i) { return k_base + 8 * n + 2 * t + (i & 1); };
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            s[n][i] = p.initial_state && row(n, i) < (int)p.dk && col(i) < (int)p.dv
+                          ? p.initial_state[state0 + (size_t)row(n, i) * p.dv + col(i)] : 0.0f;
+
+    const auto fetch = [&](uint32_t c, int which) {
+        typename Sh::Stage& st = sh.stage[which];
+        const Chunk ch = chunk_at(p, c);
+        const size_t at = (size_t)c * p.value_heads + hv;
+        load_rows<T, kStateThreads>(st.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
+        load_rows<T, kStateThreads>(st.v, Sh::kLdV, p.v, at3(p.v_stride, ch.batch, ch.token, hv) + dv_block, p.v_stride[1], ch.rows,
+                                    16 * Sh::kGroups, (int)p.dv - dv_block, p.vec);
+        load_floats<kStateThreads>(st.tri, p.tri + at * kTriFloats, kTriFloats);
+        load_floats<kStateThreads>(st.gates, p.gates[at].e, 3 * kChunk);
+        cp_commit();
+    };
+    if (c0 < c1) fetch(c0, 0);
+    for (uint32_t c = c0; c < c1; ++c) {
+        const typename Sh::Stage& st = sh.stage[(c - c0) & 1];
+        cp_wait<0>();
+        __syncthreads();                                // this chunk is here, and every warp is done with the one before
+        if (c + 1 < c1) fetch(c + 1, (c - c0 + 1) & 1);
+        const size_t at = (size_t)c * p.value_heads + hv;
+        const float *e = st.gates, *left = e + kChunk, *beta = left + kChunk;
+
+        // the state at the chunk's start
+        if (live) {
+            float* out = p.states + at * p.dkp * p.dvp;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[(size_t)row(n, i) * p.dvp + col(i)] = s[n][i];
+        }
+
+        float x[8][4] = {};
+#pragma unroll
+        for (int kk = 0; kk < NT / 2; ++kk) {
+            Sp a;
+            a.set(s[2 * kk], s[2 * kk + 1]);
+            mma_tile<T, 8, false>(x, a, st.k, LD, 0, k_base + 16 * kk);
+        }
+        float4* parts = reinterpret_cast<float4*>(sh.part);
+        float4* whole_r = reinterpret_cast<float4*>(sh.whole) + chain * 8 * 32;
+        float4* whole_d = whole_r + Sh::kGroups * 8 * 32;
+        if constexpr (KS > 1) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                parts[(warp * 8 + n) * 32 + lane] = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
+            asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
+        }
+        // R for this warp's token tiles
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            if (owner_of(n, KS) != part) continue;
+            if constexpr (KS > 1) {
+                x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < KS; ++w) {          // always in the same order
+                    const float4 f = parts[((chain * KS + w) * 8 + n) * 32 + lane];
+                    x[n][0] += f.x; x[n][1] += f.y; x[n][2] += f.z; x[n][3] += f.w;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int tok = 8 * n + 2 * t + (i & 1);
+                const float v = to_f(st.v[tok * Sh::kLdV + 16 * chain + g + 8 * (i >> 1)]);
+                x[n][i] = beta[tok] * fmaf(-e[tok], x[n][i], v);
+            }
+            if constexpr (KS > 1) whole_r[n * 32 + lane] = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
+        }
+        if constexpr (KS > 1) {
+            asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                if (owner_of(n, KS) != part) {
+                    const float4 f = whole_r[n * 32 + lane];
+                    x[n][0] = f.x; x[n][1] = f.y; x[n][2] = f.z; x[n][3] = f.w;
+                }
+        }
+        // D^T = R^T T^T, a k of 8 at a time against the rows of T that reach it
+        float d[8][4] = {};
+        const uint4* tri = reinterpret_cast<const uint4*>(st.tri);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            SplitTf32x8 a;
+            a.set(x[j]);
+#pragma unroll
+            for (int term = 0; term < 3; ++term)
+#pragma unroll
+                for (int n = j; n < 8; ++n)
+                    if (owner_of(n, KS) == part) mma_term8(d[n], a, tri[tri_tile(n, j) * 32 + lane], term);
+        }
+        float* d_out = p.d + at * kChunk * p.dvp;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            if (owner_of(n, KS) != part) continue;
+            if constexpr (KS > 1) whole_d[n * 32 + lane] = make_float4(d[n][0], d[n][1], d[n][2], d[n][3]);
+            if (live)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d_out[(size_t)(8 * n + 2 * t + (i & 1)) * p.dvp + col(i)] = d[n][i];
+        }
+        if constexpr (KS > 1) {
+            asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                if (owner_of(n, KS) != part) {
+                    const float4 f = whole_d[n * 32 + lane];
+                    d[n][0] = f.x; d[n][1] = f.y; d[n][2] = f.z; d[n][3] = f.w;
+                }
+        }
+        // S' = e^{G_63} S + (e^{G_63 - G} K)^T D
+        const float whole = e[kChunk - 1];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] *= whole;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                d[2 * j][i] *= left[16 * j + 2 * t + (i & 1)];
+                d[2 * j + 1][i] *= left[16 * j + 8 + 2 * t + (i & 1)];
+            }
+            Sp a;
+            a.set(d[2 * j], d[2 * j + 1]);
+            mma_tile<T, NT, true>(s, a, st.k, LD, k_base, 16 * j);
+        }
+    }
+    if (p.final_state)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (row(n, i) < (int)p.dk && col(i) < (int)p.dv) p.final_state[state0 + (size_t)row(n, i) * p.dv + col(i)] = s[n][i];
+}
+
+// ---------------------------------------------------------------------------
+// The outputs
+// ---------------------------------------------------------------------------
+//
+// A block takes a chunk and a value head; a warp 16 value columns of all 64 tokens: O^T = S^T (e^G Q)^T + D^T P^T, with S and D
+// read from memory as A operands (each value once, split once), Q from shared memory, and P (20 tiles of 16 x 8 over the
+// warps) kept there as the B fragments that its accumulators are.
+constexpr int kOutThreads = 256;
+
+template <typename T, int DKP>
+struct OutShared {
+    alignas(16) T     q[kChunk * (DKP + 8)];
+    alignas(16) T     k[kChunk * (DKP + 8)];
+    alignas(16) uint4 p[kTriTiles * 32];
+    alignas(16) Gates gates;
+};
+
+template <typename T, int DKP>
+__global__ void __launch_bounds__(kOutThreads) delta_output_kernel(const Args p) {
+    extern __shared__ __align__(16) char raw[];
+    using Sh = OutShared<T, DKP>;
+    using Sp = typename Split<T>::type;
+    Sh& sh = *reinterpret_cast<Sh*>(raw);
+    constexpr int LD = DKP + 8;
+    const uint32_t c = blockIdx.x, hv = blockIdx.y, h = hv / (p.value_heads / p.heads);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    T* o = static_cast<T*>(p.o);
+    const Chunk ch = chunk_at(p, c);
+    if (ch.rows == 0) {             // a ragged batch's blocks behind its chunks: tokens behind the last sequence become zero
+        const uint32_t used = p.first[p.sequences], spare = gridDim.x - used;
+        const int end = p.first[p.sequences + 1];
+        for (long long r0 = end + (long long)(c - used) * kChunk; r0 < (long long)p.tokens; r0 += (long long)spare * kChunk)
+            for (int i = threadIdx.x; i < kChunk * (int)p.dv; i += kOutThreads) {
+                const long long r = r0 + i / (int)p.dv;
+                if (r < (long long)p.tokens) o[(r * p.value_heads + hv) * p.dv + i % (int)p.dv] = from_f<T>(0.0f);
+            }
+        return;
+    }
+    const size_t at = (size_t)c * p.value_heads + hv;
+    load_rows<T, kOutThreads>(sh.q, LD, p.q, at3(p.q_stride, ch.batch, ch.token, h), p.q_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
+    load_rows<T, kOutThreads>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
+    load_floats<kOutThreads>(reinterpret_cast<float*>(&sh.gates), reinterpret_cast<const float*>(p.gates + at), sizeof(Gates) / 4);
+    cp_commit();
+    cp_wait<0>();
+    __syncthreads();
+    // P's tiles of 16 x 8 on and below the diagonal, two neighbours at a time: (0, 0), (1, 0), (1, 1), (2, 0) ...
+    for (int pair = warp; pair < 10; pair += kOutThreads / 32) {
+        int a = 0;
+        while ((a + 1) * (a + 2) / 2 <= pair) ++a;
+        const int j16 = pair - a * (a + 1) / 2;
+        float acc[2][4] = {};
+#pragma unroll
+        for (int k0 = 0; k0 < DKP; k0 += 16) mma_rows_rows<T, 2>(acc, sh.q, LD, 16 * a, sh.k, LD, 16 * j16, k0);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 16 * a + g + 8 * (i >> 1), q = 16 * j16 + 8 * n + 2 * t + (i & 1);
+                f[i] = q <= r ? acc[n][i] * exp_of(sh.gates.sum[r] - sh.gates.sum[q]) : 0.0f;
+            }
+            const int j8 = 2 * j16 + n;
+            if (j8 <= 2 * a) sh.p[tri_tile(2 * a, j8) * 32 + lane] = split_pair(f[0], f[1]);
+            sh.p[tri_tile(2 * a + 1, j8) * 32 + lane] = split_pair(f[2], f[3]);
+        }
+    }
+    __syncthreads();
+    for (int dv0 = 16 * warp; dv0 < (int)p.dvp; dv0 += 16 * (kOutThreads / 32)) {
+        float acc[8][4] = {};
+        const float* s = p.states + at * p.dkp * p.dvp + dv0 + g;
+#pragma unroll 2
+        for (int k0 = 0; k0 < DKP; k0 += 16) {
+            float x[4], y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = s[(size_t)(k0 + 2 * t + (i & 1)) * p.dvp + 8 * (i >> 1)];
+                y[i] = s[(size_t)(k0 + 8 + 2 * t + (i & 1)) * p.dvp + 8 * (i >> 1)];
+            }
+            Sp a;
+            a.set(x, y);
+            mma_tile<T, 8, false>(acc, a, sh.q, LD, 0, k0);
+        }
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[n][i] *= sh.gates.e[8 * n + 2 * t + (i & 1)];
+        const float* d = p.d + at * kChunk * p.dvp + dv0 + g;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = d[(size_t)(8 * j + 2 * t + (i & 1)) * p.dvp + 8 * (i >> 1)];
+            SplitTf32x8 a;
+            a.set(x);
+#pragma unroll
+            for (int term = 0; term < 3; ++term)
+#pragma unroll
+                for (int n = j; n < 8; ++n) mma_term8(acc[n], a, sh.p[tri_tile(n, j) * 32 + lane], term);
+        }
+        // a lane's eight neighbours g write 8 values that lie next to one another: 16 or 32 bytes of every token's row
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int tok = 8 * n + 2 * t + (i & 1), column = dv0 + g + 8 * (i >> 1);
+                if (tok < ch.rows && column < (int)p.dv)
+                    o[(((size_t)ch.batch * p.tokens + ch.token + tok) * p.value_heads + hv) * p.dv + column] =
+                        from_f<T>(p.scale * acc[n][i]);
+            }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------
+
+template <typename T, int DKP>
+void prepare_as(const Args& a, cudaStream_t stream, bool backward) {
+    const size_t bytes = sizeof(PrepShared<T, DKP>);
+    opt_in(delta_prep_kernel<T, DKP>, bytes);
+    delta_prep_kernel<T, DKP><<<dim3(a.chunks, a.heads), kPrepThreads, bytes, stream>>>(a, backward);
+    cuda_check(cudaGetLastError(), "delta rule preparation");
+}
+
+template <typename T, int DKP, int KS>
+void states_as(const Args& a, cudaStream_t stream) {
+    using Sh = StateShared<T, DKP, KS>;
+    opt_in(delta_state_kernel<T, DKP, KS>, sizeof(Sh));
+    const dim3 grid((a.dvp / 16 + Sh::kGroups - 1) / Sh::kGroups, a.value_heads, a.seqs);
+    delta_state_kernel<T, DKP, KS><<<grid, kStateThreads, sizeof(Sh), stream>>>(a);
+    cuda_check(cudaGetLastError(), "delta rule states");
+}
+
+template <typename T, int DKP>
+void states_of(const Args& a, cudaStream_t stream, int sm_count) {
+    // A chain to four warps while the blocks so made fit the multiprocessors, to two while those do, else to one.
+    const uint64_t chains = (uint64_t)(a.dvp / 16) * a.value_heads * a.seqs;
+    if (chains <= (uint64_t)sm_count) states_as<T, DKP, 4>(a, stream);
+    else if (chains <= 2 * (uint64_t)sm_count) states_as<T, DKP, 2>(a, stream);
+    else states_as<T, DKP, 1>(a, stream);
+}
+
+template <typename T, int DKP>
+void output_as(const Args& a, cudaStream_t stream) {
+    const size_t bytes = sizeof(OutShared<T, DKP>);
+    opt_in(delta_output_kernel<T, DKP>, bytes);
+    // one block more than there can be chunks: a ragged batch's tokens behind the last sequence have a block to clear them
+    delta_output_kernel<T, DKP><<<dim3(a.chunks + (a.sequences ? 1 : 0), a.value_heads), kOutThreads, bytes, stream>>>(a);
+    cuda_check(cudaGetLastError(), "delta rule outputs");
+}
+
+} // namespace
+
+void launch_prepare(const Args& a, cudaStream_t stream, bool backward) {
+    if (a.sequences) {
+        delta_index_kernel<<<1, kIndexThreads, 0, stream>>>(a);
+        cuda_check(cudaGetLastError(), "delta rule index");
+    }
+    if (a.chunks) DELTA_DISPATCH(prepare_as, a, stream, backward);
+}
+
+void launch_states(const Args& a, cudaStream_t stream, int sm_count) { DELTA_DISPATCH(states_of, a, stream, sm_count); }
+
+void launch_forward(const Args& a, cudaStream_t stream, int sm_count) {
+    launch_prepare(a, stream, false);
+    launch_states(a, stream, sm_count);
+    if (a.chunks) DELTA_DISPATCH(output_as, a, stream);
+}
+
+} // namespace delta
+} // namespace mlb

@@ -1,0 +1,350 @@
+#pragma once
+// Warp-level tensor-core products of the gated delta rule in float32 accuracy, and the loads that feed them.
+//
+// mma.sync and not tcgen05: the sequential pass is a chain of products of 16 x 64 x 128, each of which needs the one
+// before it, and the accumulators of one (a lane holds columns 2t and 2t + 1 of rows g and g + 8) are, with k's order
+// permuted in pairs, the A fragment of the next. The chain so stays in a warp's registers: no shared or tensor memory
+// and no barrier between its products.
+//
+// Float32 operands go in parts, smallest products first:
+//   bfloat16 inputs   the other operand x = hi + mid + lo in bfloat16 (24 bits): 3 m16n8k16 for a k of 16
+//   float16 inputs    x = hi + lo in tf32 (22 bits), the input exact in tf32: 2 x 2 m16n8k8
+//   float32 inputs    both in two tf32 parts, lo lo dropped (2^-22): 3 x 2 m16n8k8
+// m16n8k16 in 16 bits and m16n8k8 in tf32 both take 8.2 clocks of a multiprocessor's quarter here (measured, eight
+// independent accumulators; 21 clocks one after another), so the first form costs three quarters of the second.
+#include "delta.h"
+#include "runtime.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace mlb {
+namespace delta {
+
+using bf16 = __nv_bfloat16;
+
+template <typename T> struct Is16 { static constexpr bool value = sizeof(T) == 2; };
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16 from_f<bf16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_16(bf16, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_16(__half, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// x to the nearest tf32 (halves away from zero) and what is left, exact in float32; the tensor core cuts the rest's
+// last bits, 2^-22 of x. Infinities and NaN keep the result not finite through the rest.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float low, float high) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+    return r;
+}
+__device__ __forceinline__ float low_f(uint32_t packed) { return __uint_as_float(packed << 16); }
+__device__ __forceinline__ float high_f(uint32_t packed) { return __uint_as_float(packed & 0xFFFF0000u); }
+// two floats as three pairs of bfloat16
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+    hi = pack_bf16(x, y);
+    const float x1 = x - low_f(hi), y1 = y - high_f(hi);
+    mid = pack_bf16(x1, y1);
+    lo = pack_bf16(x1 - low_f(mid), y1 - high_f(mid));
+}
+
+// ---------------------------------------------------------------------------
+// Operands of a k of 16. A pair of accumulator tiles (x: k 0-7, y: k 8-15; element 0 and 1: row g, k 2t and 2t + 1;
+// 2 and 3: row g + 8) is an A operand as it stands.
+// ---------------------------------------------------------------------------
+
+// A float32 operand in tf32 parts.
+struct SplitTf32 {
+    uint32_t hi[8], lo[8];
+    __device__ __forceinline__ void set(const float (&x)[4], const float (&y)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = (i & 1) * 2 + (i >> 1);      // accumulator 0 1 2 3 -> fragment register 0 2 1 3
+            split_tf32(x[i], hi[at], lo[at]);
+            split_tf32(y[i], hi[4 + at], lo[4 + at]);
+        }
+    }
+};
+// The same in bfloat16 parts.
+struct SplitBf16 {
+    uint32_t part[3][4];     // hi, mid, lo
+    __device__ __forceinline__ void set(const float (&x)[4], const float (&y)[4]) {
+        split_bf16(x[0], x[1], part[0][0], part[1][0], part[2][0]);
+        split_bf16(x[2], x[3], part[0][1], part[1][1], part[2][1]);
+        split_bf16(y[0], y[1], part[0][2], part[1][2], part[2][2]);
+        split_bf16(y[2], y[3], part[0][3], part[1][3], part[2][3]);
+    }
+};
+
+// A B operand of a k of 16 and 8 columns read from a tile of T.
+template <typename T> struct FragB;
+template <> struct FragB<bf16> { uint32_t r[2]; };
+template <> struct FragB<__half> { uint32_t r[2]; };
+template <> struct FragB<float> { uint32_t hi[4], lo[4]; };   // k 2t, 2t + 1, 2t + 8, 2t + 9
+
+template <typename T> struct Split;                 // the split of the other operand that goes with inputs of type T
+template <> struct Split<bf16>   { using type = SplitBf16; static constexpr int kTerms = 3; };
+template <> struct Split<__half> { using type = SplitTf32; static constexpr int kTerms = 2; };
+template <> struct Split<float>  { using type = SplitTf32; static constexpr int kTerms = 3; };
+
+// c += one part of the product of a float32 operand with a tile's; term 0 is the smallest.
+__device__ __forceinline__ void mma_term(float (&c)[4], const SplitBf16& a, const FragB<bf16>& b, int term) {
+    mma_16(bf16(), c, a.part[2 - term], b.r[0], b.r[1]);
+}
+__device__ __forceinline__ void mma_term(float (&c)[4], const SplitTf32& a, const FragB<__half>& b, int term) {
+    const uint32_t (&p)[8] = term == 0 ? a.lo : a.hi;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b.r[h]));
+        mma_tf32(c, p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3], __float_as_uint(f.x), __float_as_uint(f.y));
+    }
+}
+__device__ __forceinline__ void mma_term(float (&c)[4], const SplitTf32& a, const FragB<float>& b, int term) {
+    const uint32_t (&p)[8] = term == 0 ? a.lo : a.hi;
+    const uint32_t (&q)[4] = term == 1 ? b.lo : b.hi;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) mma_tf32(c, p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3], q[2 * h], q[2 * h + 1]);
+}
+
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr) : "memory");
+}
+
+// Two B operands (columns n0 .. n0 + 15, k0 .. k0 + 15) of a tile in shared memory, row length `ld` elements.
+// rows: B[k][n] = tile[n][k]; cols: B[k][n] = tile[k][n].
+template <typename T>
+__device__ __forceinline__ void load_b_rows(FragB<T> (&b)[2], const T* tile, int ld, int n0, int k0) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (Is16<T>::value) {
+        const int r = lane & 7, m = lane >> 3;
+        ldmatrix4(smem_at(tile + (n0 + (m >> 1) * 8 + r) * ld + k0 + (m & 1) * 8), b[0].r[0], b[0].r[1], b[1].r[0], b[1].r[1]);
+    } else {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float2 x = *reinterpret_cast<const float2*>(tile + (n0 + 8 * j + g) * ld + k0 + 2 * t);
+            const float2 y = *reinterpret_cast<const float2*>(tile + (n0 + 8 * j + g) * ld + k0 + 8 + 2 * t);
+            split_tf32(x.x, b[j].hi[0], b[j].lo[0]);
+            split_tf32(x.y, b[j].hi[1], b[j].lo[1]);
+            split_tf32(y.x, b[j].hi[2], b[j].lo[2]);
+            split_tf32(y.y, b[j].hi[3], b[j].lo[3]);
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void load_b_cols(FragB<T> (&b)[2], const T* tile, int ld, int n0, int k0) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (Is16<T>::value) {
+        const int r = lane & 7, m = lane >> 3;
+        ldmatrix4t(smem_at(tile + (k0 + (m & 1) * 8 + r) * ld + n0 + (m >> 1) * 8), b[0].r[0], b[0].r[1], b[1].r[0], b[1].r[1]);
+    } else {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const T* at = tile + (k0 + 2 * t) * ld + n0 + 8 * j + g;
+            split_tf32(at[0], b[j].hi[0], b[j].lo[0]);
+            split_tf32(at[ld], b[j].hi[1], b[j].lo[1]);
+            split_tf32(at[8 * ld], b[j].hi[2], b[j].lo[2]);
+            split_tf32(at[9 * ld], b[j].hi[3], b[j].lo[3]);
+        }
+    }
+}
+
+// acc[NT] += the float32 operand `a` times the tile's columns n0 .. n0 + 8 NT - 1, k0 .. k0 + 15. Four columns' parts are
+// issued in turn, so that an accumulator's products lie four apart (21 clocks of latency against 4 x 8.2).
+template <typename T, int NT, bool kCols>
+__device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const typename Split<T>::type& a, const T* tile, int ld, int n0,
+                                         int k0) {
+    constexpr int kGroup = NT % 4 == 0 ? 4 : 2;
+    static_assert(NT % 2 == 0, "columns come in pairs of eight");
+#pragma unroll
+    for (int n = 0; n < NT; n += kGroup) {
+        FragB<T> b[kGroup / 2][2];
+#pragma unroll
+        for (int j = 0; j < kGroup / 2; ++j) {
+            if constexpr (kCols) load_b_cols<T>(b[j], tile, ld, n0 + 8 * (n + 2 * j), k0);
+            else                 load_b_rows<T>(b[j], tile, ld, n0 + 8 * (n + 2 * j), k0);
+        }
+#pragma unroll
+        for (int term = 0; term < Split<T>::kTerms; ++term)
+#pragma unroll
+            for (int j = 0; j < kGroup; ++j) mma_term(acc[n + j], a, b[j / 2][j & 1], term);
+    }
+}
+
+// The exact product of rows m0 .. m0 + 15 of one tile with rows n0 .. n0 + 8 NT - 1 of another over k0 .. k0 + 15 (16-bit
+// inputs: their products are exact in float32, one term; float32 inputs: three).
+template <typename T, int NT>
+__device__ __forceinline__ void mma_rows_rows(float (&acc)[NT][4], const T* a_tile, int lda, int m0, const T* b_tile, int ldb,
+                                              int n0, int k0) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (Is16<T>::value) {
+        const int r = lane & 7, m = lane >> 3;
+        uint32_t a[4];
+        ldmatrix4(smem_at(a_tile + (m0 + (m & 1) * 8 + r) * lda + k0 + (m >> 1) * 8), a[0], a[1], a[2], a[3]);
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+            FragB<T> b[2];
+            load_b_rows<T>(b, b_tile, ldb, n0 + 8 * n, k0);
+            mma_16(T(), acc[n], a, b[0].r[0], b[0].r[1]);
+            mma_16(T(), acc[n + 1], a, b[1].r[0], b[1].r[1]);
+        }
+    } else {
+        const int g = lane >> 2, t = lane & 3;
+        float x[4], y[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float2 f = *reinterpret_cast<const float2*>(a_tile + (m0 + 8 * h + g) * lda + k0 + 2 * t);
+            const float2 e = *reinterpret_cast<const float2*>(a_tile + (m0 + 8 * h + g) * lda + k0 + 8 + 2 * t);
+            x[2 * h] = f.x; x[2 * h + 1] = f.y;
+            y[2 * h] = e.x; y[2 * h + 1] = e.y;
+        }
+        SplitTf32 a;
+        a.set(x, y);
+        mma_tile<T, NT, false>(acc, a, b_tile, ldb, n0, k0);
+    }
+}
+
+// The tiles of a lower triangle, (row tile i, column tile j <= i), one after another.
+__device__ __forceinline__ constexpr int tri_tile(int i, int j) { return i * (i + 1) / 2 + j; }
+
+// c += a float32 A operand of a k of 8 (accumulator layout) times a tile of fragments in tf32 parts (a lane's float4: hi of
+// k 2t, hi of k 2t + 1, lo, lo).
+struct SplitTf32x8 {
+    uint32_t hi[4], lo[4];
+    __device__ __forceinline__ void set(const float (&x)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split_tf32(x[i], hi[(i & 1) * 2 + (i >> 1)], lo[(i & 1) * 2 + (i >> 1)]);
+    }
+};
+__device__ __forceinline__ void mma_term8(float (&c)[4], const SplitTf32x8& a, const uint4& b, int term) {
+    const uint32_t (&p)[4] = term == 0 ? a.lo : a.hi;
+    mma_tf32(c, p[0], p[1], p[2], p[3], term == 1 ? b.z : b.x, term == 1 ? b.w : b.y);
+}
+__device__ __forceinline__ uint4 split_pair(float x, float y) {
+    uint4 r;
+    split_tf32(x, r.x, r.z);
+    split_tf32(y, r.y, r.w);
+    return r;
+}
+
+// ---------------------------------------------------------------------------
+// Chunks and tiles
+// ---------------------------------------------------------------------------
+
+struct Chunk {
+    int batch, token, rows, seq;     // rows 0: no such chunk
+};
+__device__ __forceinline__ Chunk chunk_at(const Args& a, uint32_t c) {
+    Chunk r;
+    if (a.sequences) {
+        if (c >= (uint32_t)a.first[a.sequences]) return {0, 0, 0, 0};
+        const int4 e = reinterpret_cast<const int4*>(a.table)[c];
+        r = {0, e.x, e.y, e.z};
+    } else {
+        const uint32_t b = c / a.row_chunks, i = c - b * a.row_chunks;
+        r = {(int)b, (int)(i * kChunk), (int)min((uint32_t)kChunk, a.tokens - i * kChunk), (int)b};
+    }
+    return r;
+}
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(smem_at(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
+// A tile of kChunk token rows, `width` columns (a multiple of 8) of which `valid` exist, into shared memory; rows from
+// `rows` on and columns from `valid` on become zero. vec: asynchronously, in 16-byte pieces (`valid` columns and all
+// addresses are multiples of 16 bytes then); else value by value, done at the next barrier.
+template <typename T, int kThreads>
+__device__ __forceinline__ void load_rows(T* tile, int ld, const void* base, long long offset, long long stride, int rows, int width,
+                                          int valid, bool vec) {
+    const T* src = static_cast<const T*>(base) + offset;
+    if (vec) {
+        constexpr int kPer = 16 / sizeof(T);
+        const int pieces = width / kPer;
+        for (int i = threadIdx.x; i < kChunk * pieces; i += kThreads) {
+            const int r = i / pieces, c = (i - r * pieces) * kPer;
+            const bool there = r < rows && c < valid;
+            cp_async16(tile + r * ld + c, there ? src + r * stride + c : src, there);
+        }
+    } else {
+        for (int i = threadIdx.x; i < kChunk * width; i += kThreads) {
+            const int r = i / width, c = i - r * width;
+            tile[r * ld + c] = r < rows && c < valid ? src[r * stride + c] : from_f<T>(0.0f);
+        }
+    }
+}
+// `count` floats (a multiple of 4, 16-byte aligned on both sides), asynchronously.
+template <int kThreads>
+__device__ __forceinline__ void load_floats(float* dst, const float* src, int count) {
+    for (int i = threadIdx.x; i < count / 4; i += kThreads) cp_async16(dst + 4 * i, src + 4 * i, true);
+}
+
+__device__ __forceinline__ long long at3(const long long (&stride)[3], long long b, long long t, long long h) {
+    return b * stride[0] + t * stride[1] + h * stride[2];
+}
+
+// exp(x) for x <= 0 given in 64 bits (and a little above), rounded once from about 2^-30: the float exp of the leading part
+// times 1 + the rest.
+__device__ __forceinline__ float exp_of(double x) {
+    const float h = (float)x;
+    if (!(h > -104.0f)) return h != h ? h : 0.0f;      // below the smallest float32
+    if (h > 88.8f) return __int_as_float(0x7F800000);
+    const float e = expf(h);
+    return fmaf(e, (float)(x - (double)h), e);
+}
+
+// Which of a chain's KS warps computes token tile n: 0 and 7 together, 1 and 6 ..., so that the triangle's work is even.
+__device__ __forceinline__ constexpr int owner_of(int n, int ks) { return (n < 4 ? n : 7 - n) % ks; }
+
+// ---------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------
+
+// More than 48 KB of shared memory (recorded per GPU, and cheap, so it is not remembered).
+template <typename K>
+void opt_in(K kernel, size_t bytes) {
+    cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "delta rule shared memory");
+}
+
+// F<T, DKP> for the problem's type and width.
+#define DELTA_DISPATCH(F, a, ...)                                                                        \
+    do {                                                                                                 \
+        const bool wide = (a).dkp == 128;                                                                \
+        switch ((a).dtype) {                                                                             \
+            case METAL_LINALG_BFLOAT16: wide ? F<bf16, 128>(a, __VA_ARGS__) : F<bf16, 64>(a, __VA_ARGS__); break; \
+            case METAL_LINALG_FLOAT16: wide ? F<__half, 128>(a, __VA_ARGS__) : F<__half, 64>(a, __VA_ARGS__); break; \
+            default: wide ? F<float, 128>(a, __VA_ARGS__) : F<float, 64>(a, __VA_ARGS__); break;         \
+        }                                                                                                \
+    } while (0)
+
+} // namespace delta
+} // namespace mlb

@@ -38,6 +38,17 @@ int device_count() {
     return n;
 }
 
+int sm_count(int device) {
+    static std::atomic<int> known[64];
+    std::atomic<int>& slot = known[device & 63];
+    int n = slot.load(std::memory_order_relaxed);
+    if (n == 0) {
+        cuda_check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device), "cudaDeviceGetAttribute");
+        slot.store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
 DeviceGuard::DeviceGuard(int device) {
     cuda_check(cudaGetDevice(&previous_), "cudaGetDevice");
     if (device != previous_) cuda_check(cudaSetDevice(device), "cudaSetDevice");
@@ -164,6 +175,9 @@ void throw_if_a_kernel_gave_up() {
     for (int i = 0; i < n; ++i) {
         const unsigned word = all[i]->take_status();
         if (!word) continue;
+        if (word == kStatusProductWait)
+            throw std::runtime_error("a kernel on GPU " + std::to_string(all[i]->device) + " gave up on a bounded wait (a copy or a "
+                                     "tensor-core product in 8-bit floating point); the tiles of the output concerned are NaN");
         std::string what = "a kernel on GPU " + std::to_string(all[i]->device) + " gave up on a bounded wait (";
         if (word & kStatusTensorWait) what += "a tensor-core product of the blocked QR";
         if ((word & kStatusTensorWait) && (word & kStatusStreamWait)) what += ", ";

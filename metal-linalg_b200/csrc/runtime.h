@@ -29,6 +29,7 @@ struct Workspace {
 enum : unsigned {
     kStatusTensorWait = 2u,   // an mbarrier wait of a tensor-core product (tc_gemm.cu, tc_gemm2.cu) or of a panel's cluster (qr_panel_cols.cuh)
     kStatusStreamWait = 4u,   // an mbarrier wait of the streaming small-matrix kernel (qr_small_stream.cu)
+    kStatusProductWait = 8u,  // an mbarrier wait of a product in 8-bit floating point (fp8_gemm.cu)
 };
 
 struct DeviceContext {
@@ -97,6 +98,7 @@ private:
 };
 
 int            device_count();
+int            sm_count(int device);          // multiprocessors; asked of the driver once per GPU, creates no context
 DeviceContext& context(int device);   // created on first use; throws without a GPU
 
 // Launches `kernel`, whose first statement is dependency_wait() (common.cuh), so that it may be

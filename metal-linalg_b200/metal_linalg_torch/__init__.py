@@ -19,6 +19,8 @@ torch.compile: underneath it is the custom operator torch.ops.metal_linalg.qr.
 Computation is in float32: other real dtypes are converted, results are float32.
 Beside QR this build holds the SVD that calls it (`svd`, `svdvals`: the QR-preconditioned
 Jacobi route, min(M, N) <= 128); the reference's other decompositions do not exist here.
+Beside those it holds the gated delta rule (`gated_delta_rule`, `gated_delta_step`: products of decayed reflections over
+a sequence, _delta.py) and products in 8-bit floating point (`quantize_fp8`, `matmul_fp8`, `linear_fp8`, _fp8.py).
 """
 from collections import namedtuple
 
@@ -26,11 +28,14 @@ import torch
 
 from . import _lib, _ops  # noqa: F401  (_ops registers torch.ops.metal_linalg.qr)
 from ._build import version as __version__
+from ._delta import gated_delta_rule, gated_delta_step
+from ._fp8 import linear_fp8, matmul_fp8, quantize_fp8
 from ._interop import qr_dlpack, qr_into, qr_shapes
 from ._sharded import qr_sharded, shard_batch
 
 __all__ = [
     "qr", "svd", "svdvals", "svd_backend", "svdvals_backend", "qr_sharded", "shard_batch", "qr_into", "qr_dlpack", "qr_shapes",
+    "gated_delta_rule", "gated_delta_step", "quantize_fp8", "matmul_fp8", "linear_fp8",
     "device_name", "gpu_core_count", "device_count", "cpu_threads", "set_cpu_threads",
     "cpu_only", "set_cpu_only", "CpuOnly",
     "qr_backend", "qr_kernel", "qr_policy", "set_qr_policy", "qr_policy_source",

@@ -1,7 +1,7 @@
 """The C ABI through ctypes (reference: python-torch/metal_linalg_torch/_lib.py).
 
-Only the QR, the SVD that calls it, and the device and policy entry points exist
-in this build, and only they are bound. The library is lib/libmetal_linalg.so beside this package, or the
+Only the QR, the SVD that calls it, the sequence and 8-bit operators (_delta.py, _fp8.py) and the device and
+policy entry points exist in this build, and only they are bound. The library is lib/libmetal_linalg.so beside this package, or the
 file METAL_LINALG_TORCH_LIBRARY names. Calls release the GIL (ctypes does); the
 C side keeps the stream and the device per thread, so no lock is needed here.
 """
@@ -14,6 +14,7 @@ OK, INVALID_ARGUMENT, RUNTIME_ERROR, OUT_OF_MEMORY = 0, 1, 2, 3
 MODES = {"reduced": 0, "r": 1, "complete": 2}
 
 _u32 = ctypes.c_uint32
+_u64 = ctypes.c_uint64
 _ptr = ctypes.c_void_p
 
 
@@ -43,6 +44,13 @@ def _load():
         "metal_linalg_svd": (ctypes.c_int, [_ptr, _u32, _u32, _u32, _ptr, _ptr, _ptr, _ptr]),
         "metal_linalg_svd_backend": (ctypes.c_char_p, [_u32, _u32, _u32]),
         "metal_linalg_svdvals_backend": (ctypes.c_char_p, [_u32, _u32, _u32]),
+        "metal_linalg_gated_delta_rule": (ctypes.c_int, [_ptr, _ptr, _ptr, _ptr, _u64]),
+        "metal_linalg_gated_delta_rule_workspace_bytes": (_u64, [_ptr, ctypes.c_int]),
+        "metal_linalg_gated_delta_rule_backward": (ctypes.c_int, [_ptr] * 11 + [_u64]),
+        "metal_linalg_gated_delta_step": (ctypes.c_int, [_ptr, _ptr, _ptr, ctypes.c_int64, _u32, _ptr]),
+        "metal_linalg_quantize_fp8": (ctypes.c_int, [_ptr, ctypes.c_int, _u32, _u32, _u32] + [ctypes.c_int64] * 3 +
+                                      [_u32, ctypes.c_int, _ptr, _u64, _ptr]),
+        "metal_linalg_matmul_fp8": (ctypes.c_int, [_ptr, _ptr, _u32, _u32, _u32, _u32, _ptr, ctypes.c_int]),
         "metal_linalg_set_stream": (None, [_ptr]),
         "metal_linalg_stream": (_ptr, []),
         "metal_linalg_set_device": (ctypes.c_int, [ctypes.c_int]),

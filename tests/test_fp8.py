@@ -1,0 +1,380 @@
+"""Products in 8-bit floating point with block scales, against 64 bits.
+
+The quantiser's results are its definition's bit for bit. The product's tolerance, for every element and relative to
+sum |a| |b| (scales included): the tensor core adds 32 exact products to a float32 at a time, each addition off by at most
+2^-23 of the sums' magnitude (cut, not rounded), K / 32 of them; a block's sum times the scales is added in float32,
+another K / 128 roundings of 2^-24 and two of the scales' products: (K / 32 + K / 128 + 2) * 2^-23. The result's type adds half a
+step, finfo(t).eps / 2 of the value.
+"""
+import math
+
+import pytest
+import torch
+
+import metal_linalg_torch as mlt
+from metal_linalg_torch import _lib
+
+E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+TOP = {E4M3: 448.0, E5M2: 57344.0}
+
+
+def round_fp8(y, dtype):
+    """float64 to the nearest value of an 8-bit type (3 or 2 bits behind the leading one, smallest normal 2^-6 or 2^-14),
+    ties to even, by arithmetic."""
+    bits, low = (3, -6) if dtype == E4M3 else (2, -14)
+    e = torch.floor(torch.log2(y.abs().clamp_min(2.0 ** -60))).clamp_min(low)
+    step = torch.exp2(e - bits)
+    return (torch.round(y / step) * step).clamp(-TOP[dtype], TOP[dtype])
+
+
+def wanted(x, block_rows, dtype):
+    """(values, scales, the scales spread over the values) in float64 on the CPU; the scale and the quotient are
+    float32 numbers by definition."""
+    x = x.detach().cpu().double()
+    m, n = x.shape[-2:]
+    rows, cols = torch.arange(m) // block_rows, torch.arange(n) // 128
+    top = torch.zeros(*x.shape[:-2], -(-m // block_rows), -(-n // 128), dtype=torch.float64)
+    for i in range(top.shape[-2]):
+        for j in range(top.shape[-1]):
+            top[..., i, j] = x[..., i * block_rows:(i + 1) * block_rows, 128 * j:128 * j + 128].abs().amax((-1, -2))
+    scale = (top / TOP[dtype]).float().double().clamp_min(2.0 ** -126)
+    full = scale[..., rows[:, None], cols]
+    return round_fp8((x / full).float().double(), dtype), scale, full
+
+
+def meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+# ---------------------------------------------------------------------------
+# Refusals and shapes (no GPU needed)
+# ---------------------------------------------------------------------------
+
+def test_meta_gives_shapes():
+    v, s = mlt.quantize_fp8(meta(3, 200, 300))
+    assert v.shape == (3, 200, 300) and v.dtype == E4M3 and s.shape == (3, 200, 3) and v.stride(-2) == 304
+    v, s = mlt.quantize_fp8(meta(200, 300), block=(128, 128), transpose=True, dtype=E5M2)
+    assert v.shape == (300, 200) and v.dtype == E5M2 and s.shape == (3, 2)
+    a, sa = mlt.quantize_fp8(meta(2, 5, 256))
+    b, sb = mlt.quantize_fp8(meta(7, 256), block=(128, 128))
+    assert mlt.matmul_fp8(a, sa, b, sb).shape == (2, 5, 7)
+    assert mlt.matmul_fp8(a, sa, b, sb, out_dtype=torch.float32).dtype == torch.float32
+    assert mlt.linear_fp8(meta(2, 5, 64), meta(9, 64)).shape == (2, 5, 9)
+
+
+@pytest.mark.parametrize("args, error", [
+    (dict(x=meta(4)), ValueError), (dict(x=meta(4, 4, dtype=torch.float64)), TypeError), (dict(x=meta(4, 4), block=(1, 64)), ValueError),
+    (dict(x=meta(4, 4), dtype=torch.float16), TypeError), (dict(x=torch.zeros(4, 4)), ValueError), (dict(x=[1.0]), TypeError),
+    (dict(x=meta(4, 4).requires_grad_()), RuntimeError),
+])
+def test_quantize_refuses(args, error):
+    with pytest.raises(error, match="quantize_fp8"):
+        mlt.quantize_fp8(**args)
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(a=meta(5, 256)), TypeError), (dict(b=meta(7, 255, dtype=E4M3)), ValueError), (dict(a_scale=meta(5, 3, dtype=torch.float32)), ValueError),
+    (dict(a_scale=meta(4, 2, dtype=torch.float32)), ValueError), (dict(a_scale=meta(5, 2)), TypeError), (dict(out_dtype=torch.float64), TypeError),
+    (dict(b=meta(3, 7, 256, dtype=E4M3), b_scale=meta(3, 1, 2, dtype=torch.float32)), ValueError),
+    (dict(a=torch.zeros(5, 256).to(E4M3)), ValueError), (dict(b_scale=meta(1, 2, dtype=torch.float32).requires_grad_()), RuntimeError),
+])
+def test_matmul_refuses(change, error):
+    good = dict(a=meta(5, 256, dtype=E4M3), a_scale=meta(5, 2, dtype=torch.float32), b=meta(7, 256, dtype=E5M2),
+                b_scale=meta(1, 2, dtype=torch.float32))
+    mlt.matmul_fp8(**good)
+    with pytest.raises(error, match="matmul_fp8"):
+        mlt.matmul_fp8(**{**good, **change})
+
+
+@pytest.mark.parametrize("x, w, error", [
+    (meta(4, 8), meta(3, 9), ValueError), (meta(4, 8), meta(8), ValueError), (meta(4, 8, dtype=torch.float64), meta(3, 8), TypeError),
+    (torch.zeros(4, 8), torch.zeros(3, 8), ValueError),
+])
+def test_linear_refuses(x, w, error):
+    with pytest.raises(error, match="linear_fp8"):
+        mlt.linear_fp8(x, w)
+
+
+def test_c_entries_refuse_without_a_gpu():
+    import numpy as np
+    from metal_linalg_torch._fp8 import _OPERAND
+    lib = _lib.lib
+    host = np.zeros(4096, np.float32)
+    at = (host.ctypes.data + 15) // 16 * 16
+    quantize = lambda dtype=0, rows=4, cols=8, strides=(32, 8, 1), block=1, kind=3, values=at, stride=16: lib.metal_linalg_quantize_fp8(  # noqa: E731
+        at, dtype, 1, rows, cols, *strides, block, kind, values, stride, at)
+    for bad in (dict(dtype=3), dict(kind=0), dict(block=2), dict(strides=(32, 8, 2)), dict(values=at + 4), dict(stride=24), dict(stride=0),
+                dict(rows=1 << 30), {}):                    # the last: host pointers
+        assert quantize(**bad) == _lib.INVALID_ARGUMENT and "[quantize_fp8]" in _lib.last_error()
+    assert quantize(rows=0) == _lib.OK
+    operand = lambda values=at, scales=at, stride=128, across=0, kind=3, block=1: _OPERAND.pack(values, scales, stride, across, kind, block)  # noqa: E731
+    matmul = lambda a=operand(), b=operand(), m=4, k=128, dtype=0: lib.metal_linalg_matmul_fp8(a, b, 1, m, 4, k, at, dtype)  # noqa: E731
+    for bad in (dict(dtype=3), dict(m=1 << 30), {}):
+        assert matmul(**bad) == _lib.INVALID_ARGUMENT and "[matmul_fp8]" in _lib.last_error()
+    assert lib.metal_linalg_matmul_fp8(None, operand(), 1, 4, 4, 128, at, 0) == _lib.INVALID_ARGUMENT
+    assert matmul(m=0) == _lib.OK
+    with mlt.CpuOnly():
+        assert matmul() == _lib.RUNTIME_ERROR and quantize() == _lib.RUNTIME_ERROR
+
+
+# ---------------------------------------------------------------------------
+# The quantiser
+# ---------------------------------------------------------------------------
+
+def same(got, want, what):
+    got = got.cpu().double()
+    assert torch.equal(got.isnan(), want.isnan()), what
+    there = ~want.isnan()
+    assert torch.equal(got[there], want[there]), f"{what}: {(got[there] != want[there]).sum().item()} differ"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [E4M3, E5M2])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 128), (128, 128), (3, 129), (130, 7), (257, 200), (2, 136, 264), (2, 3, 33, 40)])
+def test_quantize(shape, block, transpose, dtype, kind):
+    torch.manual_seed(sum(shape))
+    x = (torch.randn(shape, device="cuda") * torch.exp(3 * torch.randn(*shape[:-1], 1, device="cuda"))).to(dtype)
+    values, scales = mlt.quantize_fp8(x, block=(block, 128), transpose=transpose, dtype=kind)
+    v, s, _ = wanted(x.mT if transpose else x, block, kind)
+    assert values.dtype == kind and values.stride(-2) % 16 == 0
+    same(scales, s, "scales")
+    same(values.float(), v, "values")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("block", [1, 128])
+def test_quantize_what_is_not_ordinary(block, transpose):
+    x = torch.randn(300, 300, device="cuda")
+    x[0, :128] = 0                          # zeros
+    x[5, 3] = math.nan
+    x[6, 200] = math.inf
+    x[140] *= 1e-42                         # below the smallest normal float32
+    x[141] = 3e38
+    x[142] = -0.0
+    if transpose:
+        x = x.mT.contiguous()
+    values, scales = mlt.quantize_fp8(x, block=(block, 128), transpose=transpose)
+    v, s, full = wanted(x.mT if transpose else x, block, E4M3)
+    same(scales, s, "scales")
+    # a block with an infinity: the scale is infinite and a value 0 or NaN, NaN either way once multiplied
+    assert (values.cpu().double() * full)[6, 128:256].isnan().all() and (values.cpu().double() * full)[5, :128].isnan().all()
+    there = full.isfinite()
+    same(values.float().cpu()[there], v[there], "values")
+
+
+@pytest.mark.gpu
+def test_quantize_strides():
+    base = torch.randn(4, 70, 3, 200, device="cuda", dtype=torch.bfloat16)
+    for x in (base[:, :, 1], base[:, 1:, 0, 3:], base.transpose(1, 3)[1], base[..., ::2], base[:1].expand(5, -1, -1, -1)[:, :, 0],
+              base[0, :, 0, :1], base[0, :1, 0].mT, base[:, :0, 0], base[1, 0].mT):
+        for block in (1, 128):
+            got, want = (mlt.quantize_fp8(y, block=(block, 128)) for y in (x, x.contiguous()))
+            assert torch.equal(got[0].float(), want[0].float()) and torch.equal(got[1], want[1])
+            got, want = mlt.quantize_fp8(x, block=(block, 128), transpose=True), mlt.quantize_fp8(x.mT.contiguous(), block=(block, 128))
+            assert torch.equal(got[0].float(), want[0].float()) and torch.equal(got[1], want[1])
+
+
+# ---------------------------------------------------------------------------
+# The product
+# ---------------------------------------------------------------------------
+
+def operand(rows, k, block, kind, seed, lead=()):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    wide = -(-k // 16) * 16
+    values = (torch.randn(*lead, rows, wide, device="cuda", generator=gen) * TOP[kind] / 5).clamp(-TOP[kind], TOP[kind]).to(kind)[..., :k]
+    scales = torch.exp(torch.randn(*lead, -(-rows // block), -(-k // 128), device="cuda", generator=gen)) / TOP[kind]
+    return values, scales
+
+
+def spread(values, scales):
+    """The operand's values in float64."""
+    m, k = values.shape[-2:]
+    block = 1 if scales.shape[-2] == m else 128
+    rows, cols = torch.arange(m, device="cuda") // block, torch.arange(k, device="cuda") // 128
+    return values.double() * scales.double()[..., rows[:, None], cols]
+
+
+def check_product(c, a, b, k):
+    """a, b: spread operands."""
+    want, size = a @ b.mT, a.abs() @ b.abs().mT
+    short = torch.finfo(c.dtype).eps / 2
+    allowed = short * want.abs() + (k / 32 + k / 128 + 2) * 2.0 ** -23 * size * (1 + short)
+    over = ((c.double() - want).abs() - allowed).max().item()
+    assert over <= 0, f"{over:.3g} over the bound"
+
+
+SIZES = [
+    # m, n, k: every tile width, shares of k, ragged edges, single rows and columns
+    (1, 1, 1), (1, 128, 128), (16, 256, 1024), (3, 1000, 300), (17, 129, 128), (33, 640, 4096), (64, 4096, 512), (65, 65, 65),
+    (128, 128, 128), (100, 200, 2000), (300, 77, 515), (1000, 16, 256), (257, 1, 129), (512, 512, 1024), (1000, 3001, 777), (2111, 2500, 384),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("blocks", [(1, 128), (1, 1), (128, 128), (128, 1)])
+@pytest.mark.parametrize("size", SIZES)
+def test_matmul(size, blocks):
+    m, n, k = size
+    a, sa = operand(m, k, blocks[0], E4M3, 1)
+    b, sb = operand(n, k, blocks[1], E4M3, 2)
+    for dtype in TYPES:
+        check_product(mlt.matmul_fp8(a, sa, b, sb, out_dtype=dtype), spread(a, sa), spread(b, sb), k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kinds", [(E4M3, E5M2), (E5M2, E4M3), (E5M2, E5M2)])
+@pytest.mark.parametrize("size", [(5, 300, 600), (300, 400, 256)])
+def test_matmul_types(size, kinds):
+    m, n, k = size
+    a, sa = operand(m, k, 1, kinds[0], 3)
+    b, sb = operand(n, k, 128, kinds[1], 4)
+    check_product(mlt.matmul_fp8(a, sa, b, sb, out_dtype=torch.float32), spread(a, sa), spread(b, sb), k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("size", [(4, 200, 256), (150, 130, 300), (1, 64, 64)])
+def test_matmul_batches(size, shared):
+    m, n, k = size
+    a, sa = operand(m, k, 1, E4M3, 5, (2, 3))
+    b, sb = operand(n, k, 128, E4M3, 6, () if shared else (2, 3))
+    c = mlt.matmul_fp8(a, sa, b, sb, out_dtype=torch.float32)
+    assert c.shape == (2, 3, m, n)
+    check_product(c, spread(a, sa), spread(b, sb), k)
+    one = mlt.matmul_fp8(a[1, 2], sa[1, 2], b if shared else b[1, 2], sb if shared else sb[1, 2], out_dtype=torch.float32)
+    check_product(one, spread(a, sa)[1, 2], spread(b, sb) if shared else spread(b, sb)[1, 2], k)
+
+
+@pytest.mark.gpu
+def test_matmul_strides_and_nothing():
+    a, sa = operand(50, 200, 1, E4M3, 7)
+    b, sb = operand(60, 200, 1, E4M3, 8)
+    want = mlt.matmul_fp8(a, sa, b, sb)
+    for x in (a.contiguous(), a.mT.contiguous().mT, torch.cat([a.float(), a.float()], 1).to(E4M3)[:, 200:]):
+        assert torch.equal(mlt.matmul_fp8(x, sa.mT.contiguous().mT, b, sb), want)
+    assert mlt.matmul_fp8(a[:0], sa[:0], b, sb).shape == (0, 60)
+    assert not mlt.matmul_fp8(a[:, :0], sa[:, :0], b[:, :0], sb[:, :0]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(7, 300, 1000), (300, 300, 300)])
+def test_matmul_what_is_not_finite_stays_in_its_row(size):
+    m, n, k = size
+    a, sa = operand(m, k, 1, E4M3, 9)
+    b, sb = operand(n, k, 1, E4M3, 10)
+    clean = mlt.matmul_fp8(a, sa, b, sb)
+    a = a.float()
+    a[2, 1] = math.nan
+    sa[4, 0] = math.inf
+    c = mlt.matmul_fp8(a.to(E4M3), sa, b, sb)
+    rest = [i for i in range(m) if i not in (2, 4)]
+    assert c[2].isnan().all() and not c[4].isfinite().any() and torch.equal(c[rest], clean[rest])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(16, 4096, 8192), (700, 700, 700), (2900, 4000, 512)])
+def test_matmul_gives_the_same_bits_twice(size):
+    m, n, k = size
+    a, sa = operand(m, k, 1, E4M3, 11)
+    b, sb = operand(n, k, 128, E4M3, 12)
+    want = mlt.matmul_fp8(a, sa, b, sb)
+    for _ in range(3):
+        assert torch.equal(mlt.matmul_fp8(a, sa, b, sb), want)
+    check_product(want, spread(a, sa), spread(b, sb), k)
+    _lib.synchronize()                      # no wait ran out
+
+
+# ---------------------------------------------------------------------------
+# The linear map
+# ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("shape", [((1, 16), 16), ((130, 100), 60), ((2, 70, 256), 300)])
+def test_linear(shape, types):
+    lead, n = shape
+    torch.manual_seed(n)
+    x = torch.randn(lead, device="cuda").to(types[0]).requires_grad_()
+    w = torch.randn(n, lead[-1], device="cuda").to(types[1]).requires_grad_()
+    y = mlt.linear_fp8(x, w)
+    dy = torch.randn(*lead[:-1], n, device="cuda").to(types[0])
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert y.shape == dy.shape and dx.dtype == types[0] and dw.dtype == types[1]
+    flat, d = x.detach().reshape(-1, lead[-1]), dy.reshape(-1, n)
+
+    def held(t, block):
+        values, _, full = wanted(t, block, E4M3)
+        return (values * full).cuda()
+
+    check_product(y.detach().reshape(-1, n), held(flat, 1), held(w, 128), lead[-1])
+    check_product(dx.reshape(-1, lead[-1]), held(d, 1), held(w.mT, 128), n)
+    check_product(dw, held(d.mT, 1), held(flat.mT, 1), flat.shape[0])
+    with torch.no_grad():
+        assert torch.equal(mlt.linear_fp8(x, w), y)
+
+
+@pytest.mark.gpu
+def test_linear_gradient_by_differences():
+    """The map is piecewise linear in what it multiplies: with operands that 8 bits hold exactly (small whole numbers, each
+    block's largest a power of two times 448) its differences along such steps are the gradient itself."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    whole = lambda *s: torch.randint(-4, 5, s, device="cuda", generator=gen).float() * 4  # noqa: E731
+    x, w, dy = whole(40, 128), whole(24, 128), whole(40, 24)
+    for t in (x, w, dy):
+        t[:, 0] = 448.0                     # the scale is 1 in every block of every direction
+        t[0, :] = 448.0
+    x.requires_grad_()
+    w.requires_grad_()
+    y = mlt.linear_fp8(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    step = 4.0
+    for leaf, grad, where in ((x, dx, (5, 7)), (x, dx, (39, 100)), (w, dw, (3, 9)), (w, dw, (23, 127))):
+        up, down = leaf.detach().clone(), leaf.detach().clone()
+        up[where], down[where] = 4.0, -4.0
+        f = lambda t: (mlt.linear_fp8(*((t, w.detach()) if leaf is x else (x.detach(), t))).double() * dy.double()).sum()  # noqa: E731
+        assert (f(up) - f(down)).item() / (2 * step) == grad[where].item()
+
+
+@pytest.mark.gpu
+def test_streams_and_graphs():
+    x, w = torch.randn(200, 256, device="cuda").bfloat16(), torch.randn(130, 256, device="cuda").bfloat16()
+    want = mlt.linear_fp8(x, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = mlt.linear_fp8(x, w)
+        leaf = x.detach().requires_grad_()
+        graph = torch.cuda.CUDAGraph()
+        torch.autograd.grad(mlt.linear_fp8(leaf, w), leaf, torch.ones_like(want))
+        with torch.cuda.graph(graph, stream=side):
+            y = mlt.linear_fp8(leaf, w)
+            (dx,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    with torch.no_grad():
+        leaf.mul_(2.0)                      # a power of two: scales double, values stay
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, 2 * want)
+    assert torch.equal(dx, torch.autograd.grad(mlt.linear_fp8(leaf, w), leaf, torch.ones_like(want))[0])
+
+
+@pytest.mark.gpu
+def test_compiled():
+    x, w = torch.randn(70, 64, device="cuda"), torch.randn(30, 64, device="cuda")
+    leaves = [t.detach().requires_grad_() for t in (x, w)]
+    y = torch.compile(lambda a, b: mlt.linear_fp8(a, b) * 2, backend="aot_eager", fullgraph=True)(*leaves)
+    assert torch.equal(y, mlt.linear_fp8(x, w) * 2)
+    grads = torch.autograd.grad(y, leaves, torch.ones_like(y))
+    plain = torch.autograd.grad(mlt.linear_fp8(*leaves) * 2, leaves, torch.ones_like(y))
+    assert all(torch.equal(a, b) for a, b in zip(grads, plain))
+
+    def product(a, b):
+        return mlt.matmul_fp8(*mlt.quantize_fp8(a), *mlt.quantize_fp8(b, block=(128, 128)))
+
+    assert torch.equal(torch.compile(product, backend="aot_eager", fullgraph=True)(x, w), product(x, w))
