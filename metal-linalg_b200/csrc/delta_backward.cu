@@ -228,15 +228,9 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
         float d[8][4] = {};
         const uint4* tri = reinterpret_cast<const uint4*>(st.tri);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            SplitTf32x8 a;
-            a.set(x[i]);
-#pragma unroll
-            for (int term = 0; term < 3; ++term)
-#pragma unroll
-                for (int n = 0; n <= i; ++n)
-                    if (owner_of(n, KS) == part) mma_term8(d[n], a, tri[tri_tile(i, n) * 32 + lane], term);
-        }
+        for (int i = 0; i < 8; ++i)
+            mma_triangle(d, x[i], [&](int n) { return n <= i && owner_of(n, KS) == part; },
+                         [&](int n) { return tri[tri_tile(i, n) * 32 + lane]; });
         float* d_out = p.dr + at * kChunk * p.dvp;
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
@@ -447,31 +441,45 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) 
         for (int n = 0; n < NT; n += 2) {
             FragB<float> b[2];
             load_b_rows<float>(b, sl.s, kLdS, n0 + 8 * n, 0);
+            float c[4][4] = {};             // every slice from nothing, then added in float32 (see mma_tile)
 #pragma unroll
             for (int term = 0; term < 3; ++term)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    mma_slice<kExact>(x1[n + j], a_do, b[j], term);
-                    mma_slice<false>(x2[n + j], a_dr, b[j], term);
+                    mma_slice<kExact>(c[j], a_do, b[j], term);
+                    mma_slice<false>(c[2 + j], a_dr, b[j], term);
                 }
             load_b_rows<float>(b, sl.ds, kLdS, n0 + 8 * n, 0);
+            float e[2][4] = {};
 #pragma unroll
             for (int term = 0; term < 3; ++term)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) mma_slice<false>(x3[n + j], a_d, b[j], term);
+                for (int j = 0; j < 2; ++j) mma_slice<false>(e[j], a_d, b[j], term);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                add_to(x1[n + j], c[j]);
+                add_to(x2[n + j], c[2 + j]);
+                add_to(x3[n + j], e[j]);
+            }
         }
 #pragma unroll
         for (int n = 0; n < 4; n += 2) {
             if (j0 + 8 * n > m0 + 15) continue;             // above the diagonal
             FragB<float> b[2];
             load_b_rows<float>(b, sl.d, kLdS, j0 + 8 * n, 0);
+            float c[4][4] = {};
 #pragma unroll
             for (int term = 0; term < 3; ++term)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    mma_slice<kExact>(mo[n + j], a_do, b[j], term);
-                    mma_slice<false>(mr[n + j], a_dr, b[j], term);
+                    mma_slice<kExact>(c[j], a_do, b[j], term);
+                    mma_slice<false>(c[2 + j], a_dr, b[j], term);
                 }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                add_to(mo[n + j], c[j]);
+                add_to(mr[n + j], c[2 + j]);
+            }
         }
         {           // dV = beta dR, dR . V: a token's four columns a thread
             const int r = threadIdx.x >> 2, q = (threadIdx.x & 3) * 4;

@@ -357,15 +357,9 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
         float d[8][4] = {};
         const uint4* tri = reinterpret_cast<const uint4*>(st.tri);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            SplitTf32x8 a;
-            a.set(x[j]);
-#pragma unroll
-            for (int term = 0; term < 3; ++term)
-#pragma unroll
-                for (int n = j; n < 8; ++n)
-                    if (owner_of(n, KS) == part) mma_term8(d[n], a, tri[tri_tile(n, j) * 32 + lane], term);
-        }
+        for (int j = 0; j < 8; ++j)
+            mma_triangle(d, x[j], [&](int n) { return n >= j && owner_of(n, KS) == part; },
+                         [&](int n) { return tri[tri_tile(n, j) * 32 + lane]; });
         float* d_out = p.d + at * kChunk * p.dvp;
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
@@ -502,12 +496,7 @@ __global__ void __launch_bounds__(kOutThreads) delta_output_kernel(const Args p)
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = d[(size_t)(8 * j + 2 * t + (i & 1)) * p.dvp + 8 * (i >> 1)];
-            SplitTf32x8 a;
-            a.set(x);
-#pragma unroll
-            for (int term = 0; term < 3; ++term)
-#pragma unroll
-                for (int n = j; n < 8; ++n) mma_term8(acc[n], a, sh.p[tri_tile(n, j) * 32 + lane], term);
+            mma_triangle(acc, x, [&](int n) { return n >= j; }, [&](int n) { return sh.p[tri_tile(n, j) * 32 + lane]; });
         }
         // a lane's eight neighbours g write 8 values that lie next to one another: 16 or 32 bytes of every token's row
 #pragma unroll

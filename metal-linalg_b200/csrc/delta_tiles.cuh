@@ -68,6 +68,11 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint3
     lo = pack_bf16(x1 - low_f(mid), y1 - high_f(mid));
 }
 
+__device__ __forceinline__ void add_to(float (&acc)[4], const float (&c)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += c[i];
+}
+
 // ---------------------------------------------------------------------------
 // Operands of a k of 16. A pair of accumulator tiles (x: k 0-7, y: k 8-15; element 0 and 1: row g, k 2t and 2t + 1;
 // 2 and 3: row g + 8) is an A operand as it stands.
@@ -176,8 +181,10 @@ __device__ __forceinline__ void load_b_cols(FragB<T> (&b)[2], const T* tile, int
     }
 }
 
-// acc[NT] += the float32 operand `a` times the tile's columns n0 .. n0 + 8 NT - 1, k0 .. k0 + 15. Four columns' parts are
-// issued in turn, so that an accumulator's products lie four apart (21 clocks of latency against 4 x 8.2).
+// acc[NT] += the float32 operand `a` times the tile's columns n0 .. n0 + 8 NT - 1, k0 .. k0 + 15. The tensor core cuts its
+// sums instead of rounding them, always towards zero, so every k of 16 is summed from nothing, smallest parts first, and
+// added in float32: with one accumulator all along the gradients were 2e-6 off, an error that grows with the number of
+// additions. Four columns' parts are issued in turn, so that a column's lie four apart (21 clocks of latency against 4 x 8.2).
 template <typename T, int NT, bool kCols>
 __device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const typename Split<T>::type& a, const T* tile, int ld, int n0,
                                          int k0) {
@@ -191,10 +198,13 @@ __device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const typename Spl
             if constexpr (kCols) load_b_cols<T>(b[j], tile, ld, n0 + 8 * (n + 2 * j), k0);
             else                 load_b_rows<T>(b[j], tile, ld, n0 + 8 * (n + 2 * j), k0);
         }
+        float c[kGroup][4] = {};
 #pragma unroll
         for (int term = 0; term < Split<T>::kTerms; ++term)
 #pragma unroll
-            for (int j = 0; j < kGroup; ++j) mma_term(acc[n + j], a, b[j / 2][j & 1], term);
+            for (int j = 0; j < kGroup; ++j) mma_term(c[j], a, b[j / 2][j & 1], term);
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) add_to(acc[n + j], c[j]);
     }
 }
 
@@ -212,8 +222,11 @@ __device__ __forceinline__ void mma_rows_rows(float (&acc)[NT][4], const T* a_ti
         for (int n = 0; n < NT; n += 2) {
             FragB<T> b[2];
             load_b_rows<T>(b, b_tile, ldb, n0 + 8 * n, k0);
-            mma_16(T(), acc[n], a, b[0].r[0], b[0].r[1]);
-            mma_16(T(), acc[n + 1], a, b[1].r[0], b[1].r[1]);
+            float c[2][4] = {};
+            mma_16(T(), c[0], a, b[0].r[0], b[0].r[1]);
+            mma_16(T(), c[1], a, b[1].r[0], b[1].r[1]);
+            add_to(acc[n], c[0]);
+            add_to(acc[n + 1], c[1]);
         }
     } else {
         const int g = lane >> 2, t = lane & 3;
@@ -252,6 +265,29 @@ __device__ __forceinline__ uint4 split_pair(float x, float y) {
     split_tf32(x, r.x, r.z);
     split_tf32(y, r.y, r.w);
     return r;
+}
+
+// acc[n] += a k of 8 of a float32 operand times fragments, for every tile n that `wanted` names, as mma_tile.
+template <typename Wanted, typename Fragment>
+__device__ __forceinline__ void mma_triangle(float (&acc)[8][4], const float (&x)[4], Wanted wanted, Fragment fragment) {
+    SplitTf32x8 a;
+    a.set(x);
+#pragma unroll
+    for (int n0 = 0; n0 < 8; n0 += 4) {
+        float c[4][4] = {};
+        uint4 b[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            if (wanted(n0 + n)) b[n] = fragment(n0 + n);
+#pragma unroll
+        for (int term = 0; term < 3; ++term)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                if (wanted(n0 + n)) mma_term8(c[n], a, b[n], term);
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            if (wanted(n0 + n)) add_to(acc[n0 + n], c[n]);
+    }
 }
 
 // ---------------------------------------------------------------------------
