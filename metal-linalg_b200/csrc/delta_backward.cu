@@ -47,9 +47,9 @@ __global__ void __launch_bounds__(kDoThreads) delta_do_kernel(const Args p) {
     if (ch.rows == 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const size_t at = (size_t)c * p.value_heads + hv;
-    load_rows<T, kDoThreads>(sh.q, LD, p.q, at3(p.q_stride, ch.batch, ch.token, h), p.q_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
-    load_rows<T, kDoThreads>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
-    load_floats<kDoThreads>(reinterpret_cast<float*>(&sh.gates), reinterpret_cast<const float*>(p.gates + at), sizeof(Gates) / 4);
+    load_rows<T, kDoThreads, DKP>(sh.q, LD, p.q, at3(p.q_stride, ch.batch, ch.token, h), p.q_stride[1], ch.rows, (int)p.dk, p.vec, threadIdx.x);
+    load_rows<T, kDoThreads, DKP>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, threadIdx.x);
+    load_floats<kDoThreads, sizeof(Gates) / 4>(reinterpret_cast<float*>(&sh.gates), reinterpret_cast<const float*>(p.gates + at), threadIdx.x);
     cp_commit();
     cp_wait<0>();
     __syncthreads();
@@ -66,8 +66,8 @@ __global__ void __launch_bounds__(kDoThreads) delta_do_kernel(const Args p) {
         }
     for (int dv0 = 0; dv0 < (int)p.dvp; dv0 += 64) {
         __syncthreads();
-        load_rows<T, kDoThreads>(sh.d_o, LDO, p.d_o, at3(p.do_stride, ch.batch, ch.token, hv) + dv0, p.do_stride[1], ch.rows, 64,
-                                 (int)p.dv - dv0, p.vec);
+        load_rows<T, kDoThreads, 64>(sh.d_o, LDO, p.d_o, at3(p.do_stride, ch.batch, ch.token, hv) + dv0, p.do_stride[1], ch.rows,
+                                     (int)p.dv - dv0, p.vec, threadIdx.x);
         cp_commit();
         cp_wait<0>();
         __syncthreads();
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kDoThreads) delta_do_kernel(const Args p) {
 //
 // The forward's chain with dS'^T in the accumulators: Y^T = dS'^T K^T, dD^T = e^{G_63 - G} Y^T + (scale P^T dO)^T,
 // dR^T = dD^T T, dS^T = e^{G_63} dS'^T + (scale e^G dO)^T Q - (beta e^G dR)^T K.
-constexpr int kReverseThreads = 128;
+constexpr int kReverseThreads = 160;
 
 template <typename T, int DKP, int KS>
 struct ReverseShared {
@@ -112,22 +112,23 @@ struct ReverseShared {
         alignas(16) float tri[kTriFloats];
         alignas(16) float gates[3 * kChunk];
     } stage[kStages];
-    alignas(16) float part[KS > 1 ? 4 * 8 * 32 * 4 : 4];
-    alignas(16) float whole[KS > 1 ? 2 * kGroups * 8 * 32 * 4 : 4];
+    uint4 part[KS > 1 ? 4 * 8 * 32 : 1];
+    uint4 dd[KS > 1 ? kGroups * 8 * kTileWords : 1];        // dD in parts
+    uint4 dr[KS > 1 ? kGroups * 8 * kTileWords : 1];        // -beta e^G dR in parts
+    uint4 d_o[KS > 1 ? kGroups * 8 * kTileWords : 1];       // scale e^G dO in parts
 };
 
 template <typename T, int DKP, int KS>
 __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Args p) {
     using Sh = ReverseShared<T, DKP, KS>;
     using Sp = typename Split<T>::type;
+    using Tile = typename Split<T>::tile;
     extern __shared__ __align__(16) char raw[];
     Sh& sh = *reinterpret_cast<Sh*>(raw);
-    constexpr int LD = DKP + 8, NT = DKP / 8 / KS, LDV = Sh::kLdV;
+    constexpr int LD = DKP + 8, NT = DKP / 8 / KS, LDV = Sh::kLdV, kOwn = 8 / KS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int chain = warp / KS, part = warp % KS;
     const uint32_t hv = blockIdx.y, seq = blockIdx.z, h = hv / (p.value_heads / p.heads);
-    const int dv_block = blockIdx.x * 16 * Sh::kGroups, dv0 = dv_block + 16 * chain, k_base = part * NT * 8;
-    const bool live = dv0 < (int)p.dvp;
+    const int dv_block = blockIdx.x * 16 * Sh::kGroups;
     uint32_t c0, c1;
     if (p.sequences) {
         c0 = p.first[seq];
@@ -136,6 +137,37 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
         c0 = seq * p.row_chunks;
         c1 = c0 + p.row_chunks;
     }
+    if (warp == 4) {
+        const auto fetch = [&](uint32_t c, int which) {
+            typename Sh::Stage& st = sh.stage[which];
+            const Chunk ch = chunk_at(p, c);
+            const size_t at = (size_t)c * p.value_heads + hv;
+            load_rows<T, 32, DKP>(st.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, lane);
+            load_rows<T, 32, DKP>(st.q, LD, p.q, at3(p.q_stride, ch.batch, ch.token, h), p.q_stride[1], ch.rows, (int)p.dk, p.vec, lane);
+            load_rows<T, 32, 16 * Sh::kGroups>(st.d_o, LDV, p.d_o, at3(p.do_stride, ch.batch, ch.token, hv) + dv_block, p.do_stride[1],
+                                               ch.rows, (int)p.dv - dv_block, p.vec, lane);
+            load_rows<float, 32, 16 * Sh::kGroups>(st.dd, LDV, p.dr, (long long)(at * kChunk * p.dvp) + dv_block, p.dvp, kChunk,
+                                                   (int)p.dvp - dv_block, true, lane);
+            load_floats<32, kTriFloats>(st.tri, p.tri_b + at * kTriFloats, lane);
+            load_floats<32, 3 * kChunk>(st.gates, p.gates[at].e, lane);
+            cp_commit();
+        };
+        if (Sh::kStages == 2 && c0 < c1) fetch(c1 - 1, 0);
+        for (uint32_t i0 = 0; i0 < c1 - c0; ++i0) {
+            const uint32_t c = c1 - 1 - i0;
+            if constexpr (Sh::kStages == 1) {
+                __syncthreads();                        // the stage is free
+                fetch(c, 0);
+            }
+            cp_wait<0>();
+            __syncthreads();
+            if (Sh::kStages == 2 && c > c0) fetch(c - 1, (i0 + 1) & 1);
+        }
+        return;
+    }
+    const int chain = warp / KS, part = warp % KS;
+    const int dv0 = dv_block + 16 * chain, k_base = part * NT * 8;
+    const bool live = dv0 < (int)p.dvp;
     float s[NT][4];                     // dS'^T
     const size_t state0 = ((size_t)seq * p.value_heads + hv) * p.dk * p.dv;
     const auto col = [&](int i) { return dv0 + g + 8 * (i >> 1); };
@@ -147,39 +179,26 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
             s[n][i] = p.d_final && row(n, i) < (int)p.dk && col(i) < (int)p.dv
                           ? p.d_final[state0 + (size_t)row(n, i) * p.dv + col(i)] : 0.0f;
 
-    const auto fetch = [&](uint32_t c, int which) {
-        typename Sh::Stage& st = sh.stage[which];
-        const Chunk ch = chunk_at(p, c);
-        const size_t at = (size_t)c * p.value_heads + hv;
-        load_rows<T, kReverseThreads>(st.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
-        load_rows<T, kReverseThreads>(st.q, LD, p.q, at3(p.q_stride, ch.batch, ch.token, h), p.q_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
-        load_rows<T, kReverseThreads>(st.d_o, LDV, p.d_o, at3(p.do_stride, ch.batch, ch.token, hv) + dv_block, p.do_stride[1], ch.rows,
-                                      16 * Sh::kGroups, (int)p.dv - dv_block, p.vec);
-        load_rows<float, kReverseThreads>(st.dd, LDV, p.dr, (long long)(at * kChunk * p.dvp) + dv_block, p.dvp, kChunk,
-                                          16 * Sh::kGroups, (int)p.dvp - dv_block, true);
-        load_floats<kReverseThreads>(st.tri, p.tri_b + at * kTriFloats, kTriFloats);
-        load_floats<kReverseThreads>(st.gates, p.gates[at].e, 3 * kChunk);
-        cp_commit();
-    };
-    if (Sh::kStages == 2 && c0 < c1) fetch(c1 - 1, 0);
+    uint4* dd_parts = sh.dd + (KS > 1 ? chain * 8 * kTileWords : 0);
+    uint4* dr_parts = sh.dr + (KS > 1 ? chain * 8 * kTileWords : 0);
+    uint4* do_parts = sh.d_o + (KS > 1 ? chain * 8 * kTileWords : 0);
     for (uint32_t i0 = 0; i0 < c1 - c0; ++i0) {
         const uint32_t c = c1 - 1 - i0;
         const typename Sh::Stage& st = sh.stage[i0 % Sh::kStages];
-        if constexpr (Sh::kStages == 1) {
-            __syncthreads();
-            fetch(c, 0);
-        }
-        cp_wait<0>();
+        if constexpr (Sh::kStages == 1) __syncthreads();
         __syncthreads();
-        if (Sh::kStages == 2 && c > c0) fetch(c - 1, (i0 + 1) & 1);
         const size_t at = (size_t)c * p.value_heads + hv;
         const float *e = st.gates, *left = e + kChunk, *beta = left + kChunk;
         if (live) {
-            float* out = p.d_states + at * p.dkp * p.dvp;
+            float* out = p.d_states + at * p.dkp * p.dvp + (size_t)(k_base + 2 * t) * p.dvp + dv0 + g;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) out[(size_t)row(n, i) * p.dvp + col(i)] = s[n][i];
+            for (int n = 0; n < NT; ++n) {
+                out[0] = s[n][0];
+                out[8] = s[n][2];
+                out[p.dvp] = s[n][1];
+                out[p.dvp + 8] = s[n][3];
+                out += 8 * p.dvp;
+            }
         }
         float x[8][4] = {};
 #pragma unroll
@@ -188,87 +207,124 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
             a.set(s[2 * kk], s[2 * kk + 1]);
             mma_tile<T, 8, false>(x, a, st.k, LD, 0, k_base + 16 * kk);
         }
-        float4* parts = reinterpret_cast<float4*>(sh.part);
-        float4* whole_d = reinterpret_cast<float4*>(sh.whole) + chain * 8 * 32;
-        float4* whole_r = whole_d + Sh::kGroups * 8 * 32;
         if constexpr (KS > 1) {
 #pragma unroll
             for (int n = 0; n < 8; ++n)
-                parts[(warp * 8 + n) * 32 + lane] = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
+                *reinterpret_cast<float4*>(sh.part + (warp * 8 + n) * 32 + lane) = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
             asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
         }
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            if (owner_of(n, KS) != part) continue;
+        for (int i = 0; i < kOwn; ++i) {
+            const int n = KS > 1 ? own_tile<KS>(part, i) : i;
+            float f[4] = {};
             if constexpr (KS > 1) {
-                x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
 #pragma unroll
                 for (int w = 0; w < KS; ++w) {
-                    const float4 f = parts[((chain * KS + w) * 8 + n) * 32 + lane];
-                    x[n][0] += f.x; x[n][1] += f.y; x[n][2] += f.z; x[n][3] += f.w;
+                    const float4 q = *reinterpret_cast<const float4*>(sh.part + ((chain * KS + w) * 8 + n) * 32 + lane);
+                    const float u[4] = {q.x, q.y, q.z, q.w};
+                    add_to(f, u);
                 }
+            } else {
+                add_to(f, x[i]);
             }
+            const float2 le = *reinterpret_cast<const float2*>(left + 8 * n + 2 * t);
+            const float* dd = st.dd + (8 * n + 2 * t) * LDV + 16 * chain + g;
+            f[0] = fmaf(le.x, f[0], dd[0]);
+            f[1] = fmaf(le.y, f[1], dd[LDV]);
+            f[2] = fmaf(le.x, f[2], dd[8]);
+            f[3] = fmaf(le.y, f[3], dd[LDV + 8]);
+            if constexpr (KS > 1) {
+                TileTf32 a;
+                a.set(f);
+                a.put(dd_parts, n, lane);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int tok = 8 * n + 2 * t + (i & 1);
-                x[n][i] = fmaf(left[tok], x[n][i], st.dd[tok * LDV + 16 * chain + g + 8 * (i >> 1)]);
+                for (int j = 0; j < 4; ++j) x[i][j] = f[j];
             }
-            if constexpr (KS > 1) whole_d[n * 32 + lane] = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
         }
+        const auto out_tile = [&](int n, float (&u)[4]) {          // scale e^G dO of token tile n
+            const float2 ee = *reinterpret_cast<const float2*>(e + 8 * n + 2 * t);
+            const T* d_o = st.d_o + (8 * n + 2 * t) * LDV + 16 * chain + g;
+            u[0] = p.scale * ee.x * to_f(d_o[0]);
+            u[1] = p.scale * ee.y * to_f(d_o[LDV]);
+            u[2] = p.scale * ee.x * to_f(d_o[8]);
+            u[3] = p.scale * ee.y * to_f(d_o[LDV + 8]);
+        };
         if constexpr (KS > 1) {
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                const int n = own_tile<KS>(part, i);
+                float u[4];
+                out_tile(n, u);
+                Tile a;
+                a.set(u);
+                a.put(do_parts, n, lane);
+            }
             asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
-#pragma unroll
-            for (int n = 0; n < 8; ++n)
-                if (owner_of(n, KS) != part) {
-                    const float4 f = whole_d[n * 32 + lane];
-                    x[n][0] = f.x; x[n][1] = f.y; x[n][2] = f.z; x[n][3] = f.w;
-                }
         }
-        // dR^T = dD^T T: tokens i from the column's own on
-        float d[8][4] = {};
-        const uint4* tri = reinterpret_cast<const uint4*>(st.tri);
+        // dR^T = dD^T T: tokens from the column's own on
+        float d[kOwn][4] = {};
+        const uint4* tri = reinterpret_cast<const uint4*>(st.tri) + lane;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            mma_triangle(d, x[i], [&](int n) { return n <= i && owner_of(n, KS) == part; },
-                         [&](int n) { return tri[tri_tile(i, n) * 32 + lane]; });
-        float* d_out = p.dr + at * kChunk * p.dvp;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            if (owner_of(n, KS) != part) continue;
-            if constexpr (KS > 1) whole_r[n * 32 + lane] = make_float4(d[n][0], d[n][1], d[n][2], d[n][3]);
-            if (live)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) d_out[(size_t)(8 * n + 2 * t + (i & 1)) * p.dvp + col(i)] = d[n][i];
+        for (int j = 0; j < 8; ++j) {
+            TileTf32 a;
+            if constexpr (KS > 1) a.get(dd_parts, j, lane);
+            else                  a.set(x[j]);
+            mma_triangle(d, a, [&](int i) { return KS == 1 ? i <= j : i < kOwn / 2 ? j >= 3 || own_tile<KS>(part, i) <= j
+                                                                                   : j >= 4 && own_tile<KS>(part, i) <= j; },
+                         [&](int i) { return tri[tri_tile(j, KS > 1 ? own_tile<KS>(part, i) : i) * 32]; });
         }
-        if constexpr (KS > 1) {
-            asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
+        float* d_out = p.dr + at * kChunk * p.dvp + (size_t)(2 * t) * p.dvp + dv0 + g;
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
-                if (owner_of(n, KS) != part) {
-                    const float4 f = whole_r[n * 32 + lane];
-                    d[n][0] = f.x; d[n][1] = f.y; d[n][2] = f.z; d[n][3] = f.w;
-                }
+        for (int i = 0; i < kOwn; ++i) {
+            const int n = KS > 1 ? own_tile<KS>(part, i) : i;
+            if (live) {
+                float* out = d_out + (size_t)(8 * n) * p.dvp;
+                out[0] = d[i][0];
+                out[8] = d[i][2];
+                out[p.dvp] = d[i][1];
+                out[p.dvp + 8] = d[i][3];
+            }
+            const float2 be = *reinterpret_cast<const float2*>(beta + 8 * n + 2 * t), ee = *reinterpret_cast<const float2*>(e + 8 * n + 2 * t);
+            d[i][0] *= -be.x * ee.x; d[i][1] *= -be.y * ee.y; d[i][2] *= -be.x * ee.x; d[i][3] *= -be.y * ee.y;
+            if constexpr (KS > 1) {
+                Tile a;
+                a.set(d[i]);
+                a.put(dr_parts, n, lane);
+            }
         }
+        // dS = e^{G_63} dS' + scale (e^G Q)^T dO - (beta e^G K)^T dR; the part that needs no dR before the barrier
         const float whole = e[kChunk - 1];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] *= whole;
+        for (int n = 0; n < NT; ++n) scale_by(s[n], whole);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float u[2][4];
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int tok = 16 * j + 8 * half + 2 * t + (i & 1);
-                    u[half][i] = p.scale * e[tok] * to_f(st.d_o[tok * LDV + 16 * chain + g + 8 * (i >> 1)]);
-                    d[2 * j + half][i] *= -beta[tok] * e[tok];
-                }
             Sp a;
-            a.set(u[0], u[1]);
+            if constexpr (KS > 1) {
+                Tile u, v;
+                u.get(do_parts, 2 * j, lane);
+                v.get(do_parts, 2 * j + 1, lane);
+                a.set(u, v);
+            } else {
+                float u[4], v[4];
+                out_tile(2 * j, u);
+                out_tile(2 * j + 1, v);
+                a.set(u, v);
+            }
             mma_tile<T, NT, true>(s, a, st.q, LD, k_base, 16 * j);
-            a.set(d[2 * j], d[2 * j + 1]);
+        }
+        if constexpr (KS > 1) asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            Sp a;
+            if constexpr (KS > 1) {
+                Tile u, v;
+                u.get(dr_parts, 2 * j, lane);
+                v.get(dr_parts, 2 * j + 1, lane);
+                a.set(u, v);
+            } else {
+                a.set(d[2 * j], d[2 * j + 1]);
+            }
             mma_tile<T, NT, true>(s, a, st.k, LD, k_base, 16 * j);
         }
     }
@@ -415,15 +471,15 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) 
             cp_async16(sl.d + r * kLdS + q, d + (size_t)r * p.dvp + q, true);
             cp_async16(sl.dr + r * kLdS + q, dr + (size_t)r * p.dvp + q, true);
         }
-        load_rows<T, kGradThreads>(sl.d_o, kLdS, p.d_o, at3(p.do_stride, ch.batch, ch.token, hv) + dv0, p.do_stride[1], ch.rows, 16,
-                                   (int)p.dv - dv0, p.vec);
-        load_rows<T, kGradThreads>(sl.v, kLdS, p.v, at3(p.v_stride, ch.batch, ch.token, hv) + dv0, p.v_stride[1], ch.rows, 16,
-                                   (int)p.dv - dv0, p.vec);
+        load_rows<T, kGradThreads, 16>(sl.d_o, kLdS, p.d_o, at3(p.do_stride, ch.batch, ch.token, hv) + dv0, p.do_stride[1], ch.rows,
+                                       (int)p.dv - dv0, p.vec, threadIdx.x);
+        load_rows<T, kGradThreads, 16>(sl.v, kLdS, p.v, at3(p.v_stride, ch.batch, ch.token, hv) + dv0, p.v_stride[1], ch.rows,
+                                       (int)p.dv - dv0, p.vec, threadIdx.x);
         cp_commit();
     };
-    load_rows<T, kGradThreads>(sh.q, LD, p.q, at3(p.q_stride, ch.batch, ch.token, h), p.q_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
-    load_rows<T, kGradThreads>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
-    load_floats<kGradThreads>(reinterpret_cast<float*>(&sh.gates), reinterpret_cast<const float*>(p.gates + at), sizeof(Gates) / 4);
+    load_rows<T, kGradThreads, DKP>(sh.q, LD, p.q, at3(p.q_stride, ch.batch, ch.token, h), p.q_stride[1], ch.rows, (int)p.dk, p.vec, threadIdx.x);
+    load_rows<T, kGradThreads, DKP>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, threadIdx.x);
+    load_floats<kGradThreads, sizeof(Gates) / 4>(reinterpret_cast<float*>(&sh.gates), reinterpret_cast<const float*>(p.gates + at), threadIdx.x);
     fetch(0, 0);
 
     float x1[NT][4] = {}, x2[NT][4] = {}, x3[NT][4] = {}, mo[4][4] = {}, mr[4][4] = {};

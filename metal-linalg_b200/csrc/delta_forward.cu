@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const Args p, 
     const Chunk ch = chunk_at(p, c);
     if (ch.rows == 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    load_rows<T, kPrepThreads>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
+    load_rows<T, kPrepThreads, DKP>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, threadIdx.x);
     cp_commit();
     cp_wait<0>();
     __syncthreads();
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const Args p, 
                     const float2 u = *reinterpret_cast<const float2*>(ti + g * kLdA + 8 * k8 + 2 * t);
                     const float2 v = *reinterpret_cast<const float2*>(ti + (g + 8) * kLdA + 8 * k8 + 2 * t);
                     const float x[4] = {-u.x, -u.y, -v.x, -v.y};
-                    SplitTf32x8 s;
+                    TileTf32 s;
                     s.set(x);
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
@@ -229,9 +229,9 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const Args p, 
 // A chain is 16 value columns: S^T [16 x dk] lives in accumulators. X^T = S^T K^T; R^T = beta (V^T - e^G X^T);
 // D^T = R^T T^T; S^T = e^{G_63} S^T + (D^T e^{G_63 - G}) K: every product's accumulators are the next one's A operand, and K
 // comes from shared memory as B operands both ways round. KS warps share a chain where there are too few chains to fill the
-// GPU: each holds dk / KS of S's rows, and partial X, R and D cross through shared memory as whole fragments (a lane's 16
-// bytes, no bank met twice).
-constexpr int kStateThreads = 128;
+// GPU: each holds dk / KS of S's rows; partial X crosses through shared memory as whole fragments (a lane's 16 bytes, no bank
+// met twice), R and D already in their parts. A fifth warp fetches the next chunk meanwhile.
+constexpr int kStateThreads = 160;
 
 template <typename T, int DKP, int KS>
 struct StateShared {
@@ -243,22 +243,22 @@ struct StateShared {
         alignas(16) float tri[kTriFloats];
         alignas(16) float gates[3 * kChunk];        // e, left, beta
     } stage[2];
-    alignas(16) float part[KS > 1 ? 4 * 8 * 32 * 4 : 4];       // [warp][tile][lane][4]: partial X
-    alignas(16) float whole[KS > 1 ? 2 * kGroups * 8 * 32 * 4 : 4];   // R, then D: [which][chain][tile][lane][4]
+    uint4 part[KS > 1 ? 4 * 8 * 32 : 1];            // [warp][tile][lane]: partial X
+    uint4 r[KS > 1 ? kGroups * 8 * kTileWords : 1]; // [chain][tile]: R in parts
+    uint4 d[KS > 1 ? kGroups * 8 * kTileWords : 1]; // e^{G_63 - G} D in parts
 };
 
 template <typename T, int DKP, int KS>
 __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p) {
     using Sh = StateShared<T, DKP, KS>;
     using Sp = typename Split<T>::type;
+    using Tile = typename Split<T>::tile;
     extern __shared__ __align__(16) char raw[];
     Sh& sh = *reinterpret_cast<Sh*>(raw);
-    constexpr int LD = DKP + 8, NT = DKP / 8 / KS;
+    constexpr int LD = DKP + 8, NT = DKP / 8 / KS, kOwn = 8 / KS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int chain = warp / KS, part = warp % KS;
     const uint32_t hv = blockIdx.y, seq = blockIdx.z, h = hv / (p.value_heads / p.heads);
-    const int dv_block = blockIdx.x * 16 * Sh::kGroups, dv0 = dv_block + 16 * chain, k_base = part * NT * 8;
-    const bool live = dv0 < (int)p.dvp;                 // a chain past the last columns computes on zeros and writes nothing
+    const int dv_block = blockIdx.x * 16 * Sh::kGroups;
     uint32_t c0, c1;
     if (p.sequences) {
         c0 = p.first[seq];
@@ -267,6 +267,29 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
         c0 = seq * p.row_chunks;
         c1 = c0 + p.row_chunks;
     }
+    if (warp == 4) {            // the fetching warp: a chunk ahead, complete at the barrier that opens it
+        const auto fetch = [&](uint32_t c, int which) {
+            typename Sh::Stage& st = sh.stage[which];
+            const Chunk ch = chunk_at(p, c);
+            const size_t at = (size_t)c * p.value_heads + hv;
+            load_rows<T, 32, DKP>(st.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, lane);
+            load_rows<T, 32, 16 * Sh::kGroups>(st.v, Sh::kLdV, p.v, at3(p.v_stride, ch.batch, ch.token, hv) + dv_block, p.v_stride[1],
+                                               ch.rows, (int)p.dv - dv_block, p.vec, lane);
+            load_floats<32, kTriFloats>(st.tri, p.tri + at * kTriFloats, lane);
+            load_floats<32, 3 * kChunk>(st.gates, p.gates[at].e, lane);
+            cp_commit();
+        };
+        if (c0 < c1) fetch(c0, 0);
+        for (uint32_t c = c0; c < c1; ++c) {
+            cp_wait<0>();
+            __syncthreads();
+            if (c + 1 < c1) fetch(c + 1, (c - c0 + 1) & 1);
+        }
+        return;
+    }
+    const int chain = warp / KS, part = warp % KS;
+    const int dv0 = dv_block + 16 * chain, k_base = part * NT * 8;
+    const bool live = dv0 < (int)p.dvp;                 // a chain past the last columns computes on zeros and writes nothing
 
     float s[NT][4];
     const size_t state0 = ((size_t)seq * p.value_heads + hv) * p.dk * p.dv;
@@ -279,33 +302,25 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
             s[n][i] = p.initial_state && row(n, i) < (int)p.dk && col(i) < (int)p.dv
                           ? p.initial_state[state0 + (size_t)row(n, i) * p.dv + col(i)] : 0.0f;
 
-    const auto fetch = [&](uint32_t c, int which) {
-        typename Sh::Stage& st = sh.stage[which];
-        const Chunk ch = chunk_at(p, c);
-        const size_t at = (size_t)c * p.value_heads + hv;
-        load_rows<T, kStateThreads>(st.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
-        load_rows<T, kStateThreads>(st.v, Sh::kLdV, p.v, at3(p.v_stride, ch.batch, ch.token, hv) + dv_block, p.v_stride[1], ch.rows,
-                                    16 * Sh::kGroups, (int)p.dv - dv_block, p.vec);
-        load_floats<kStateThreads>(st.tri, p.tri + at * kTriFloats, kTriFloats);
-        load_floats<kStateThreads>(st.gates, p.gates[at].e, 3 * kChunk);
-        cp_commit();
-    };
-    if (c0 < c1) fetch(c0, 0);
+    uint4* r_parts = sh.r + (KS > 1 ? chain * 8 * kTileWords : 0);
+    uint4* d_parts = sh.d + (KS > 1 ? chain * 8 * kTileWords : 0);
     for (uint32_t c = c0; c < c1; ++c) {
         const typename Sh::Stage& st = sh.stage[(c - c0) & 1];
-        cp_wait<0>();
         __syncthreads();                                // this chunk is here, and every warp is done with the one before
-        if (c + 1 < c1) fetch(c + 1, (c - c0 + 1) & 1);
         const size_t at = (size_t)c * p.value_heads + hv;
         const float *e = st.gates, *left = e + kChunk, *beta = left + kChunk;
 
         // the state at the chunk's start
         if (live) {
-            float* out = p.states + at * p.dkp * p.dvp;
+            float* out = p.states + at * p.dkp * p.dvp + (size_t)(k_base + 2 * t) * p.dvp + dv0 + g;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) out[(size_t)row(n, i) * p.dvp + col(i)] = s[n][i];
+            for (int n = 0; n < NT; ++n) {
+                out[0] = s[n][0];
+                out[8] = s[n][2];
+                out[p.dvp] = s[n][1];
+                out[p.dvp + 8] = s[n][3];
+                out += 8 * p.dvp;
+            }
         }
 
         float x[8][4] = {};
@@ -315,84 +330,91 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
             a.set(s[2 * kk], s[2 * kk + 1]);
             mma_tile<T, 8, false>(x, a, st.k, LD, 0, k_base + 16 * kk);
         }
-        float4* parts = reinterpret_cast<float4*>(sh.part);
-        float4* whole_r = reinterpret_cast<float4*>(sh.whole) + chain * 8 * 32;
-        float4* whole_d = whole_r + Sh::kGroups * 8 * 32;
         if constexpr (KS > 1) {
 #pragma unroll
             for (int n = 0; n < 8; ++n)
-                parts[(warp * 8 + n) * 32 + lane] = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
+                *reinterpret_cast<float4*>(sh.part + (warp * 8 + n) * 32 + lane) = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
             asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
         }
         // R for this warp's token tiles
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            if (owner_of(n, KS) != part) continue;
+        for (int i = 0; i < kOwn; ++i) {
+            const int n = KS > 1 ? own_tile<KS>(part, i) : i;
+            float f[4] = {};
             if constexpr (KS > 1) {
-                x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
 #pragma unroll
                 for (int w = 0; w < KS; ++w) {          // always in the same order
-                    const float4 f = parts[((chain * KS + w) * 8 + n) * 32 + lane];
-                    x[n][0] += f.x; x[n][1] += f.y; x[n][2] += f.z; x[n][3] += f.w;
+                    const float4 q = *reinterpret_cast<const float4*>(sh.part + ((chain * KS + w) * 8 + n) * 32 + lane);
+                    const float u[4] = {q.x, q.y, q.z, q.w};
+                    add_to(f, u);
                 }
+            } else {
+                add_to(f, x[i]);
             }
+            const float2 be = *reinterpret_cast<const float2*>(beta + 8 * n + 2 * t), ee = *reinterpret_cast<const float2*>(e + 8 * n + 2 * t);
+            const T* v = st.v + (8 * n + 2 * t) * Sh::kLdV + 16 * chain + g;
+            f[0] = be.x * fmaf(-ee.x, f[0], to_f(v[0]));
+            f[1] = be.y * fmaf(-ee.y, f[1], to_f(v[Sh::kLdV]));
+            f[2] = be.x * fmaf(-ee.x, f[2], to_f(v[8]));
+            f[3] = be.y * fmaf(-ee.y, f[3], to_f(v[Sh::kLdV + 8]));
+            if constexpr (KS > 1) {
+                TileTf32 a;
+                a.set(f);
+                a.put(r_parts, n, lane);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int tok = 8 * n + 2 * t + (i & 1);
-                const float v = to_f(st.v[tok * Sh::kLdV + 16 * chain + g + 8 * (i >> 1)]);
-                x[n][i] = beta[tok] * fmaf(-e[tok], x[n][i], v);
+                for (int j = 0; j < 4; ++j) x[i][j] = f[j];
             }
-            if constexpr (KS > 1) whole_r[n * 32 + lane] = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
         }
-        if constexpr (KS > 1) {
-            asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
-#pragma unroll
-            for (int n = 0; n < 8; ++n)
-                if (owner_of(n, KS) != part) {
-                    const float4 f = whole_r[n * 32 + lane];
-                    x[n][0] = f.x; x[n][1] = f.y; x[n][2] = f.z; x[n][3] = f.w;
-                }
-        }
+        if constexpr (KS > 1) asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
         // D^T = R^T T^T, a k of 8 at a time against the rows of T that reach it
-        float d[8][4] = {};
-        const uint4* tri = reinterpret_cast<const uint4*>(st.tri);
+        float d[kOwn][4] = {};
+        const uint4* tri = reinterpret_cast<const uint4*>(st.tri) + lane;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            mma_triangle(d, x[j], [&](int n) { return n >= j && owner_of(n, KS) == part; },
-                         [&](int n) { return tri[tri_tile(n, j) * 32 + lane]; });
-        float* d_out = p.d + at * kChunk * p.dvp;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            if (owner_of(n, KS) != part) continue;
-            if constexpr (KS > 1) whole_d[n * 32 + lane] = make_float4(d[n][0], d[n][1], d[n][2], d[n][3]);
-            if (live)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) d_out[(size_t)(8 * n + 2 * t + (i & 1)) * p.dvp + col(i)] = d[n][i];
+        for (int j = 0; j < 8; ++j) {
+            TileTf32 a;
+            if constexpr (KS > 1) a.get(r_parts, j, lane);
+            else                  a.set(x[j]);
+            // of a pair of tiles one lies above row 4 and one below: which products there are is mostly known
+            mma_triangle(d, a, [&](int i) { return KS == 1 ? i >= j : i < kOwn / 2 ? j < 4 && own_tile<KS>(part, i) >= j
+                                                                                   : j <= 4 || own_tile<KS>(part, i) >= j; },
+                         [&](int i) { return tri[tri_tile(KS > 1 ? own_tile<KS>(part, i) : i, j) * 32]; });
         }
-        if constexpr (KS > 1) {
-            asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
+        float* d_out = p.d + at * kChunk * p.dvp + (size_t)(2 * t) * p.dvp + dv0 + g;
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
-                if (owner_of(n, KS) != part) {
-                    const float4 f = whole_d[n * 32 + lane];
-                    d[n][0] = f.x; d[n][1] = f.y; d[n][2] = f.z; d[n][3] = f.w;
-                }
+        for (int i = 0; i < kOwn; ++i) {
+            const int n = KS > 1 ? own_tile<KS>(part, i) : i;
+            if (live) {
+                float* out = d_out + (size_t)(8 * n) * p.dvp;
+                out[0] = d[i][0];
+                out[8] = d[i][2];
+                out[p.dvp] = d[i][1];
+                out[p.dvp + 8] = d[i][3];
+            }
+            const float2 le = *reinterpret_cast<const float2*>(left + 8 * n + 2 * t);
+            d[i][0] *= le.x; d[i][1] *= le.y; d[i][2] *= le.x; d[i][3] *= le.y;
+            if constexpr (KS > 1) {
+                Tile a;
+                a.set(d[i]);
+                a.put(d_parts, n, lane);
+            }
         }
+        if constexpr (KS > 1) asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
         // S' = e^{G_63} S + (e^{G_63 - G} K)^T D
         const float whole = e[kChunk - 1];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] *= whole;
+        for (int n = 0; n < NT; ++n) scale_by(s[n], whole);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                d[2 * j][i] *= left[16 * j + 2 * t + (i & 1)];
-                d[2 * j + 1][i] *= left[16 * j + 8 + 2 * t + (i & 1)];
-            }
             Sp a;
-            a.set(d[2 * j], d[2 * j + 1]);
+            if constexpr (KS > 1) {
+                Tile u, v;
+                u.get(d_parts, 2 * j, lane);
+                v.get(d_parts, 2 * j + 1, lane);
+                a.set(u, v);
+            } else {
+                a.set(d[2 * j], d[2 * j + 1]);
+            }
             mma_tile<T, NT, true>(s, a, st.k, LD, k_base, 16 * j);
         }
     }
@@ -443,9 +465,9 @@ __global__ void __launch_bounds__(kOutThreads) delta_output_kernel(const Args p)
         return;
     }
     const size_t at = (size_t)c * p.value_heads + hv;
-    load_rows<T, kOutThreads>(sh.q, LD, p.q, at3(p.q_stride, ch.batch, ch.token, h), p.q_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
-    load_rows<T, kOutThreads>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, DKP, (int)p.dk, p.vec);
-    load_floats<kOutThreads>(reinterpret_cast<float*>(&sh.gates), reinterpret_cast<const float*>(p.gates + at), sizeof(Gates) / 4);
+    load_rows<T, kOutThreads, DKP>(sh.q, LD, p.q, at3(p.q_stride, ch.batch, ch.token, h), p.q_stride[1], ch.rows, (int)p.dk, p.vec, threadIdx.x);
+    load_rows<T, kOutThreads, DKP>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, threadIdx.x);
+    load_floats<kOutThreads, sizeof(Gates) / 4>(reinterpret_cast<float*>(&sh.gates), reinterpret_cast<const float*>(p.gates + at), threadIdx.x);
     cp_commit();
     cp_wait<0>();
     __syncthreads();
@@ -496,7 +518,9 @@ __global__ void __launch_bounds__(kOutThreads) delta_output_kernel(const Args p)
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = d[(size_t)(8 * j + 2 * t + (i & 1)) * p.dvp + 8 * (i >> 1)];
-            mma_triangle(acc, x, [&](int n) { return n >= j; }, [&](int n) { return sh.p[tri_tile(n, j) * 32 + lane]; });
+            TileTf32 a;
+            a.set(x);
+            mma_triangle(acc, a, [&](int n) { return n >= j; }, [&](int n) { return sh.p[tri_tile(n, j) * 32 + lane]; });
         }
         // a lane's eight neighbours g write 8 values that lie next to one another: 16 or 32 bytes of every token's row
 #pragma unroll

@@ -68,9 +68,18 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint3
     lo = pack_bf16(x1 - low_f(mid), y1 - high_f(mid));
 }
 
+// Pairs of float32 in one instruction.
 __device__ __forceinline__ void add_to(float (&acc)[4], const float (&c)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] += c[i];
+    for (int i = 0; i < 4; i += 2)
+        asm("{\n .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %3};\n add.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;\n}"
+            : "+f"(acc[i]), "+f"(acc[i + 1]) : "f"(c[i]), "f"(c[i + 1]));
+}
+__device__ __forceinline__ void scale_by(float (&acc)[4], float f) {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2)
+        asm("{\n .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %2};\n mul.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;\n}"
+            : "+f"(acc[i]), "+f"(acc[i + 1]) : "f"(f));
 }
 
 // ---------------------------------------------------------------------------
@@ -78,26 +87,76 @@ __device__ __forceinline__ void add_to(float (&acc)[4], const float (&c)[4]) {
 // 2 and 3: row g + 8) is an A operand as it stands.
 // ---------------------------------------------------------------------------
 
-// A float32 operand in tf32 parts.
+// One accumulator tile (a k of 8) of a float32 operand, in its parts: what warps that share a chain hand one another.
+struct TileTf32 {
+    uint4 hi, lo;                   // fragment registers 0-3 of m16n8k8
+    __device__ __forceinline__ void set(const float (&x)[4]) {
+        split_tf32(x[0], hi.x, lo.x);
+        split_tf32(x[2], hi.y, lo.y);
+        split_tf32(x[1], hi.z, lo.z);
+        split_tf32(x[3], hi.w, lo.w);
+    }
+    __device__ __forceinline__ void put(uint4* at, int tile, int lane) const {
+        at[(2 * tile) * 32 + lane] = hi;
+        at[(2 * tile + 1) * 32 + lane] = lo;
+    }
+    __device__ __forceinline__ void get(const uint4* at, int tile, int lane) {
+        hi = at[(2 * tile) * 32 + lane];
+        lo = at[(2 * tile + 1) * 32 + lane];
+    }
+};
+struct TileBf16 {
+    uint2 part[3];                  // hi, mid, lo; x: row g, y: row g + 8
+    __device__ __forceinline__ void set(const float (&x)[4]) {
+        split_bf16(x[0], x[1], part[0].x, part[1].x, part[2].x);
+        split_bf16(x[2], x[3], part[0].y, part[1].y, part[2].y);
+    }
+    __device__ __forceinline__ void put(uint4* at, int tile, int lane) const {
+        uint2* to = reinterpret_cast<uint2*>(at) + tile * 96 + lane;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) to[32 * i] = part[i];
+    }
+    __device__ __forceinline__ void get(const uint4* at, int tile, int lane) {
+        const uint2* from = reinterpret_cast<const uint2*>(at) + tile * 96 + lane;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) part[i] = from[32 * i];
+    }
+};
+constexpr int kTileWords = 2 * 32;      // uint4 of shared memory a tile takes (the larger of the two)
+
+// A float32 operand of a k of 16 in tf32 parts.
 struct SplitTf32 {
     uint32_t hi[8], lo[8];
+    __device__ __forceinline__ void set(const TileTf32& x, const TileTf32& y) {
+        hi[0] = x.hi.x; hi[1] = x.hi.y; hi[2] = x.hi.z; hi[3] = x.hi.w;
+        hi[4] = y.hi.x; hi[5] = y.hi.y; hi[6] = y.hi.z; hi[7] = y.hi.w;
+        lo[0] = x.lo.x; lo[1] = x.lo.y; lo[2] = x.lo.z; lo[3] = x.lo.w;
+        lo[4] = y.lo.x; lo[5] = y.lo.y; lo[6] = y.lo.z; lo[7] = y.lo.w;
+    }
     __device__ __forceinline__ void set(const float (&x)[4], const float (&y)[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = (i & 1) * 2 + (i >> 1);      // accumulator 0 1 2 3 -> fragment register 0 2 1 3
-            split_tf32(x[i], hi[at], lo[at]);
-            split_tf32(y[i], hi[4 + at], lo[4 + at]);
-        }
+        TileTf32 a, b;
+        a.set(x);
+        b.set(y);
+        set(a, b);
     }
 };
 // The same in bfloat16 parts.
 struct SplitBf16 {
     uint32_t part[3][4];     // hi, mid, lo
+    __device__ __forceinline__ void set(const TileBf16& x, const TileBf16& y) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            part[i][0] = x.part[i].x;
+            part[i][1] = x.part[i].y;
+            part[i][2] = y.part[i].x;
+            part[i][3] = y.part[i].y;
+        }
+    }
     __device__ __forceinline__ void set(const float (&x)[4], const float (&y)[4]) {
-        split_bf16(x[0], x[1], part[0][0], part[1][0], part[2][0]);
-        split_bf16(x[2], x[3], part[0][1], part[1][1], part[2][1]);
-        split_bf16(y[0], y[1], part[0][2], part[1][2], part[2][2]);
-        split_bf16(y[2], y[3], part[0][3], part[1][3], part[2][3]);
+        TileBf16 a, b;
+        a.set(x);
+        b.set(y);
+        set(a, b);
     }
 };
 
@@ -108,9 +167,9 @@ template <> struct FragB<__half> { uint32_t r[2]; };
 template <> struct FragB<float> { uint32_t hi[4], lo[4]; };   // k 2t, 2t + 1, 2t + 8, 2t + 9
 
 template <typename T> struct Split;                 // the split of the other operand that goes with inputs of type T
-template <> struct Split<bf16>   { using type = SplitBf16; static constexpr int kTerms = 3; };
-template <> struct Split<__half> { using type = SplitTf32; static constexpr int kTerms = 2; };
-template <> struct Split<float>  { using type = SplitTf32; static constexpr int kTerms = 3; };
+template <> struct Split<bf16>   { using type = SplitBf16; using tile = TileBf16; static constexpr int kTerms = 3; };
+template <> struct Split<__half> { using type = SplitTf32; using tile = TileTf32; static constexpr int kTerms = 2; };
+template <> struct Split<float>  { using type = SplitTf32; using tile = TileTf32; static constexpr int kTerms = 3; };
 
 // c += one part of the product of a float32 operand with a tile's; term 0 is the smallest.
 __device__ __forceinline__ void mma_term(float (&c)[4], const SplitBf16& a, const FragB<bf16>& b, int term) {
@@ -247,18 +306,11 @@ __device__ __forceinline__ void mma_rows_rows(float (&acc)[NT][4], const T* a_ti
 // The tiles of a lower triangle, (row tile i, column tile j <= i), one after another.
 __device__ __forceinline__ constexpr int tri_tile(int i, int j) { return i * (i + 1) / 2 + j; }
 
-// c += a float32 A operand of a k of 8 (accumulator layout) times a tile of fragments in tf32 parts (a lane's float4: hi of
-// k 2t, hi of k 2t + 1, lo, lo).
-struct SplitTf32x8 {
-    uint32_t hi[4], lo[4];
-    __device__ __forceinline__ void set(const float (&x)[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) split_tf32(x[i], hi[(i & 1) * 2 + (i >> 1)], lo[(i & 1) * 2 + (i >> 1)]);
-    }
-};
-__device__ __forceinline__ void mma_term8(float (&c)[4], const SplitTf32x8& a, const uint4& b, int term) {
-    const uint32_t (&p)[4] = term == 0 ? a.lo : a.hi;
-    mma_tf32(c, p[0], p[1], p[2], p[3], term == 1 ? b.z : b.x, term == 1 ? b.w : b.y);
+// c += one part of a k of 8 of a float32 operand times a tile of fragments in tf32 parts (a lane's uint4: hi of k 2t, hi of
+// k 2t + 1, lo, lo).
+__device__ __forceinline__ void mma_term8(float (&c)[4], const TileTf32& a, const uint4& b, int term) {
+    const uint4& p = term == 0 ? a.lo : a.hi;
+    mma_tf32(c, p.x, p.y, p.z, p.w, term == 1 ? b.z : b.x, term == 1 ? b.w : b.y);
 }
 __device__ __forceinline__ uint4 split_pair(float x, float y) {
     uint4 r;
@@ -266,26 +318,24 @@ __device__ __forceinline__ uint4 split_pair(float x, float y) {
     split_tf32(y, r.y, r.w);
     return r;
 }
-
-// acc[n] += a k of 8 of a float32 operand times fragments, for every tile n that `wanted` names, as mma_tile.
-template <typename Wanted, typename Fragment>
-__device__ __forceinline__ void mma_triangle(float (&acc)[8][4], const float (&x)[4], Wanted wanted, Fragment fragment) {
-    SplitTf32x8 a;
-    a.set(x);
+// acc[i] += a k of 8 of a float32 operand times fragment(i) for every i that wanted(i) names, as mma_tile.
+template <int N, typename Wanted, typename Fragment>
+__device__ __forceinline__ void mma_triangle(float (&acc)[N][4], const TileTf32& a, Wanted wanted, Fragment fragment) {
+    constexpr int kGroup = N < 4 ? N : 4;
 #pragma unroll
-    for (int n0 = 0; n0 < 8; n0 += 4) {
-        float c[4][4] = {};
-        uint4 b[4];
+    for (int n0 = 0; n0 < N; n0 += kGroup) {
+        float c[kGroup][4] = {};
+        uint4 b[kGroup];
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < kGroup; ++n)
             if (wanted(n0 + n)) b[n] = fragment(n0 + n);
 #pragma unroll
         for (int term = 0; term < 3; ++term)
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int n = 0; n < kGroup; ++n)
                 if (wanted(n0 + n)) mma_term8(c[n], a, b[n], term);
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < kGroup; ++n)
             if (wanted(n0 + n)) add_to(acc[n0 + n], c[n]);
     }
 }
@@ -316,32 +366,47 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool vali
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
 
-// A tile of kChunk token rows, `width` columns (a multiple of 8) of which `valid` exist, into shared memory; rows from
-// `rows` on and columns from `valid` on become zero. vec: asynchronously, in 16-byte pieces (`valid` columns and all
-// addresses are multiples of 16 bytes then); else value by value, done at the next barrier.
-template <typename T, int kThreads>
-__device__ __forceinline__ void load_rows(T* tile, int ld, const void* base, long long offset, long long stride, int rows, int width,
-                                          int valid, bool vec) {
+// A tile of kChunk token rows, kWidth columns (a multiple of 8) of which `valid` exist, into shared memory by the kThreads
+// threads whose number `tid` is; rows from `rows` on and columns from `valid` on become zero. vec: asynchronously, in
+// 16-byte pieces (`valid` columns and all addresses are multiples of 16 bytes then); else value by value, done at the next
+// barrier.
+template <typename T, int kThreads, int kWidth>
+__device__ __forceinline__ void load_rows(T* tile, int ld, const void* base, long long offset, long long stride, int rows, int valid,
+                                          bool vec, int tid) {
     const T* src = static_cast<const T*>(base) + offset;
     if (vec) {
-        constexpr int kPer = 16 / sizeof(T);
-        const int pieces = width / kPer;
-        for (int i = threadIdx.x; i < kChunk * pieces; i += kThreads) {
-            const int r = i / pieces, c = (i - r * pieces) * kPer;
-            const bool there = r < rows && c < valid;
-            cp_async16(tile + r * ld + c, there ? src + r * stride + c : src, there);
+        constexpr int kPer = 16 / sizeof(T), kPieces = kWidth / kPer;
+        constexpr int kStep = kThreads / kPieces > 0 ? kThreads / kPieces : 1;      // rows at a time
+        constexpr int kAcross = kPieces > kThreads ? kPieces / kThreads : 1;
+        static_assert(kThreads % kPieces == 0 || kPieces % kThreads == 0, "pieces of a row and threads go into one another");
+        const int r0 = kPieces > kThreads ? 0 : tid / kPieces, c0 = kPieces > kThreads ? tid * kPer : (tid % kPieces) * kPer;
+#pragma unroll
+        for (int a = 0; a < kAcross; ++a) {
+            const int c = c0 + a * kThreads * kPer;
+            const T* from = src + r0 * stride + c;
+            T* to = tile + r0 * ld + c;
+            const int limit = c < valid ? rows : 0;
+#pragma unroll
+            for (int r = 0; r < kChunk; r += kStep) {
+                const bool there = r + r0 < limit;
+                if (kChunk % kStep == 0 || r + r0 < kChunk) cp_async16(to, there ? from : src, there);
+                from += kStep * stride;
+                to += kStep * ld;
+            }
         }
     } else {
-        for (int i = threadIdx.x; i < kChunk * width; i += kThreads) {
-            const int r = i / width, c = i - r * width;
+        for (int i = tid; i < kChunk * kWidth; i += kThreads) {
+            const int r = i / kWidth, c = i - r * kWidth;
             tile[r * ld + c] = r < rows && c < valid ? src[r * stride + c] : from_f<T>(0.0f);
         }
     }
 }
-// `count` floats (a multiple of 4, 16-byte aligned on both sides), asynchronously.
-template <int kThreads>
-__device__ __forceinline__ void load_floats(float* dst, const float* src, int count) {
-    for (int i = threadIdx.x; i < count / 4; i += kThreads) cp_async16(dst + 4 * i, src + 4 * i, true);
+// kCount floats (a multiple of 4, 16-byte aligned on both sides), asynchronously.
+template <int kThreads, int kCount>
+__device__ __forceinline__ void load_floats(float* dst, const float* src, int tid) {
+#pragma unroll
+    for (int i = 0; i < kCount / 4; i += kThreads)
+        if ((kCount / 4) % kThreads == 0 || i + tid < kCount / 4) cp_async16(dst + 4 * (i + tid), src + 4 * (i + tid), true);
 }
 
 __device__ __forceinline__ long long at3(const long long (&stride)[3], long long b, long long t, long long h) {
@@ -358,8 +423,13 @@ __device__ __forceinline__ float exp_of(double x) {
     return fmaf(e, (float)(x - (double)h), e);
 }
 
-// Which of a chain's KS warps computes token tile n: 0 and 7 together, 1 and 6 ..., so that the triangle's work is even.
-__device__ __forceinline__ constexpr int owner_of(int n, int ks) { return (n < 4 ? n : 7 - n) % ks; }
+// Of a chain's 8 token tiles, the i-th that warp `part` of its KS computes: 0 and 7 together, 1 and 6 ..., so that the
+// triangle's work is even.
+template <int KS>
+__device__ __forceinline__ int own_tile(int part, int i) {
+    constexpr int kOwn = 8 / KS;
+    return i < kOwn / 2 ? part + KS * i : 7 - (part + KS * (kOwn - 1 - i));
+}
 
 // ---------------------------------------------------------------------------
 // Launches
