@@ -16,6 +16,7 @@
 #include "delta.h"
 #include "delta_tiles.cuh"
 #include "runtime.h"
+#include <cstdlib>
 
 namespace mlb {
 namespace delta {
@@ -103,7 +104,7 @@ template <typename T, int DKP, int KS>
 struct ReverseShared {
     static constexpr int kGroups = 4 / KS;
     static constexpr int kLdV = 16 * kGroups + 8;
-    static constexpr int kStages = sizeof(T) == 4 ? 1 : 2;      // two of float32 are more than a multiprocessor holds
+    static constexpr int kStages = sizeof(T) == 4 || KS == 4 ? 1 : 2;      // two of float32 are more than a multiprocessor holds
     struct Stage {
         alignas(16) T     k[kChunk * (DKP + 8)];
         alignas(16) T     q[kChunk * (DKP + 8)];
@@ -112,9 +113,8 @@ struct ReverseShared {
         alignas(16) float tri[kTriFloats];
         alignas(16) float gates[3 * kChunk];
     } stage[kStages];
-    uint4 part[KS > 1 ? 4 * 8 * 32 : 1];
+    uint4 part[KS > 1 ? 4 * 8 * 32 : 1];                    // partial Y; then -beta e^G dR in parts
     uint4 dd[KS > 1 ? kGroups * 8 * kTileWords : 1];        // dD in parts
-    uint4 dr[KS > 1 ? kGroups * 8 * kTileWords : 1];        // -beta e^G dR in parts
     uint4 d_o[KS > 1 ? kGroups * 8 * kTileWords : 1];       // scale e^G dO in parts
 };
 
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
                           ? p.d_final[state0 + (size_t)row(n, i) * p.dv + col(i)] : 0.0f;
 
     uint4* dd_parts = sh.dd + (KS > 1 ? chain * 8 * kTileWords : 0);
-    uint4* dr_parts = sh.dr + (KS > 1 ? chain * 8 * kTileWords : 0);
+    uint4* dr_parts = sh.part + (KS > 1 ? chain * 8 * kTileWords : 0);
     uint4* do_parts = sh.d_o + (KS > 1 ? chain * 8 * kTileWords : 0);
     for (uint32_t i0 = 0; i0 < c1 - c0; ++i0) {
         const uint32_t c = c1 - 1 - i0;
@@ -748,8 +748,10 @@ void backward_as(const Args& a, cudaStream_t stream, int sm_count) {
         cuda_check(cudaGetLastError(), "delta rule P^T dO");
     }
     const uint64_t chains = (uint64_t)(a.dvp / 16) * a.value_heads * a.seqs;        // as the forward's
-    if (chains <= (uint64_t)sm_count) reverse_as<T, DKP, 4>(a, stream);
-    else if (chains <= 2 * (uint64_t)sm_count) reverse_as<T, DKP, 2>(a, stream);
+    const char* ks = getenv("DELTA_KS");
+    const int k = ks ? atoi(ks) : chains <= (uint64_t)sm_count ? 4 : chains <= 2 * (uint64_t)sm_count ? 2 : 1;
+    if (k == 4) reverse_as<T, DKP, 4>(a, stream);
+    else if (k == 2) reverse_as<T, DKP, 2>(a, stream);
     else reverse_as<T, DKP, 1>(a, stream);
     if (a.chunks) {
         opt_in(delta_grad_kernel<T, DKP>, sizeof(GradShared<T, DKP>));

@@ -3,6 +3,7 @@
 #include "delta.h"
 #include "delta_tiles.cuh"
 #include "runtime.h"
+#include <cstdlib>
 
 namespace mlb {
 namespace delta {
@@ -243,9 +244,9 @@ struct StateShared {
         alignas(16) float tri[kTriFloats];
         alignas(16) float gates[3 * kChunk];        // e, left, beta
     } stage[2];
-    uint4 part[KS > 1 ? 4 * 8 * 32 : 1];            // [warp][tile][lane]: partial X
+    // [warp][tile][lane]: partial X; then, when every R is there, [chain][tile]: e^{G_63 - G} D in parts
+    uint4 part[KS > 1 ? 4 * 8 * 32 : 1];
     uint4 r[KS > 1 ? kGroups * 8 * kTileWords : 1]; // [chain][tile]: R in parts
-    uint4 d[KS > 1 ? kGroups * 8 * kTileWords : 1]; // e^{G_63 - G} D in parts
 };
 
 template <typename T, int DKP, int KS>
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
                           ? p.initial_state[state0 + (size_t)row(n, i) * p.dv + col(i)] : 0.0f;
 
     uint4* r_parts = sh.r + (KS > 1 ? chain * 8 * kTileWords : 0);
-    uint4* d_parts = sh.d + (KS > 1 ? chain * 8 * kTileWords : 0);
+    uint4* d_parts = sh.part + (KS > 1 ? chain * 8 * kTileWords : 0);
     for (uint32_t c = c0; c < c1; ++c) {
         const typename Sh::Stage& st = sh.stage[(c - c0) & 1];
         __syncthreads();                                // this chunk is here, and every warp is done with the one before
@@ -560,8 +561,10 @@ template <typename T, int DKP>
 void states_of(const Args& a, cudaStream_t stream, int sm_count) {
     // A chain to four warps while the blocks so made fit the multiprocessors, to two while those do, else to one.
     const uint64_t chains = (uint64_t)(a.dvp / 16) * a.value_heads * a.seqs;
-    if (chains <= (uint64_t)sm_count) states_as<T, DKP, 4>(a, stream);
-    else if (chains <= 2 * (uint64_t)sm_count) states_as<T, DKP, 2>(a, stream);
+    const char* ks = getenv("DELTA_KS");
+    const int k = ks ? atoi(ks) : chains <= (uint64_t)sm_count ? 4 : chains <= 2 * (uint64_t)sm_count ? 2 : 1;
+    if (k == 4) states_as<T, DKP, 4>(a, stream);
+    else if (k == 2) states_as<T, DKP, 2>(a, stream);
     else states_as<T, DKP, 1>(a, stream);
 }
 

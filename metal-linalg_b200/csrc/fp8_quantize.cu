@@ -2,7 +2,7 @@
 //
 //     scale = max(max|x| / M, 2^-126),   value = x / scale, a float32, rounded to the nearest (ties to even)
 //
-// The quotient is a true division, so that the values are the definition's bit for bit. Every kernel reads x once: what
+// The quotient is correctly rounded, so that the values are the definition's bit for bit. Every kernel reads x once: what
 // bounds them is memory.
 //   rows     x contiguous along columns, 1 x 128: 16 lanes a block, eight values a lane
 //   tiles    the same in 128 x 128: 256 threads hold the tile in registers
@@ -44,28 +44,53 @@ __device__ __forceinline__ uint32_t pair_of(float low, float high) {
     else                 asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(high), "f"(low));
     return r;
 }
+// x / scale, correctly rounded, for one scale and many x. With r the correctly rounded reciprocal and q = x r,
+// q + (x - q scale) r in fused operations is the correctly rounded quotient (Markstein, IBM J. Res. Dev. 34, 1990) as long
+// as the remainder is exact: three operations a value instead of a division's ten or so. Outside 2^-100 .. 2^120 the
+// remainder can underflow (or the scale is infinite or NaN): there it is the division itself.
+struct Quotient {
+    float scale, r;
+    bool  plain;
+    __device__ __forceinline__ explicit Quotient(float s) : scale(s), r(1.0f / s), plain(!(s >= 0x1p-100f && s <= 0x1p120f)) {}
+    __device__ __forceinline__ float operator()(float x) const {
+        const float q = x * r;
+        return fmaf(fmaf(-q, scale, x), r, q);
+    }
+};
 template <bool kE5m2>
-__device__ __forceinline__ uint32_t four_of(const float* v, float scale) {
-    return pair_of<kE5m2>(__fdiv_rn(v[0], scale), __fdiv_rn(v[1], scale)) |
-           (pair_of<kE5m2>(__fdiv_rn(v[2], scale), __fdiv_rn(v[3], scale)) << 16);
+__device__ __forceinline__ uint32_t four_of(const float* v, const Quotient& by) {
+    if (by.plain)
+        return pair_of<kE5m2>(__fdiv_rn(v[0], by.scale), __fdiv_rn(v[1], by.scale)) |
+               (pair_of<kE5m2>(__fdiv_rn(v[2], by.scale), __fdiv_rn(v[3], by.scale)) << 16);
+    return pair_of<kE5m2>(by(v[0]), by(v[1])) | (pair_of<kE5m2>(by(v[2]), by(v[3])) << 16);
 }
 
-// Eight neighbouring values from column c on; zero behind the last.
-template <typename T>
-__device__ __forceinline__ void load8(float (&v)[8], const T* row, uint32_t c, uint32_t cols, bool vec) {
-    if (vec && c + 8 <= cols) {
-        constexpr int kWords = sizeof(T) / 2;           // 16-byte words
-        uint4 w[kWords];
+// Eight neighbouring values from column c on as they lie in memory; zero behind the last.
+template <typename T> struct Eight {
+    static constexpr int kWords = sizeof(T) / 2;           // 16-byte words
+    uint4 w[kWords];
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
+        for (int i = 0; i < kWords; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const T* row, uint32_t c, uint32_t cols, bool vec) {
+        if (vec && c + 8 <= cols) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
+        } else {
+            clear();
+            T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < cols) e[i] = row[c + i];
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
         const T* e = reinterpret_cast<const T*>(w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = as_float(e[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? as_float(row[c + i]) : 0.0f;
     }
-}
+};
 
 template <typename T, bool kE5m2>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeArgs a) {
@@ -75,21 +100,21 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeA
     const bool there = unit < units;                    // whole warps take part in the exchange
     const uint32_t row = there ? (uint32_t)(unit / blocks) : 0, block = there ? (uint32_t)(unit - (uint64_t)row * blocks) : 0;
     const uint32_t c = block * kB + (threadIdx.x & 15) * 8;
-    float v[8];
-    if (there) load8<T>(v, static_cast<const T*>(a.x) + z * a.batch_stride + (long long)row * a.row_stride, c, a.cols, a.vec);
-    else
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    float top = 0.0f;
+    Eight<T> x;
+    x.clear();
+    if (there) x.load(static_cast<const T*>(a.x) + z * a.batch_stride + (long long)row * a.row_stride, c, a.cols, a.vec);
+    float v[8], top = 0.0f;
+    x.get(v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(v[i]));
 #pragma unroll
     for (int o = 1; o < 16; o *= 2) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float scale = scale_of<kE5m2>(top);
     if (!there) return;
+    const Quotient by(scale);
     if (c < a.cols)
         *reinterpret_cast<uint2*>(a.values + z * a.values_batch + row * a.values_stride + c) =
-            make_uint2(four_of<kE5m2>(v, scale), four_of<kE5m2>(v + 4, scale));
+            make_uint2(four_of<kE5m2>(v, by), four_of<kE5m2>(v + 4, by));
     if ((threadIdx.x & 15) == 0) a.scales[((uint64_t)z * a.rows + row) * blocks + block] = scale;
 }
 
@@ -105,33 +130,37 @@ __device__ __forceinline__ float block_max(float top, float* shared) {
 }
 
 template <typename T, bool kE5m2>
-__global__ void __launch_bounds__(kThreads) quantize_tiles_kernel(const QuantizeArgs a) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) quantize_tiles_kernel(const QuantizeArgs a) {
     __shared__ float tops[kThreads / 32];
     const uint32_t blocks = (a.cols + kB - 1) / kB, z = blockIdx.y;
     const uint32_t br = blockIdx.x / blocks, bc = blockIdx.x - br * blocks;
     const uint32_t c = bc * kB + (threadIdx.x & 15) * 8, r0 = br * kB + (threadIdx.x >> 4);
     const T* x = static_cast<const T*>(a.x) + z * a.batch_stride;
-    float v[8][8];
+    Eight<T> held[8];
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint32_t r = r0 + 16 * i;
-        if (r < a.rows) load8<T>(v[i], x + (long long)r * a.row_stride, c, a.cols, a.vec);
-        else
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        if (r < a.rows) held[i].load(x + (long long)r * a.row_stride, c, a.cols, a.vec);
+        else            held[i].clear();
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i) {
+        float v[8];
+        held[i].get(v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(v[i][j]));
+        for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(v[j]));
+    }
     const float scale = scale_of<kE5m2>(block_max(top, tops));
+    const Quotient by(scale);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint32_t r = r0 + 16 * i;
+        float v[8];
+        held[i].get(v);
         if (r < a.rows && c < a.cols)
             *reinterpret_cast<uint2*>(a.values + z * a.values_batch + r * a.values_stride + c) =
-                make_uint2(four_of<kE5m2>(v[i], scale), four_of<kE5m2>(v[i] + 4, scale));
+                make_uint2(four_of<kE5m2>(v, by), four_of<kE5m2>(v + 4, by));
     }
     if (threadIdx.x == 0) a.scales[((uint64_t)z * ((a.rows + kB - 1) / kB) + br) * blocks + bc] = scale;
 }
@@ -149,7 +178,7 @@ __global__ void __launch_bounds__(kThreads) quantize_turned_kernel(const Quantiz
     const T* x = static_cast<const T*>(a.x) + z * a.batch_stride + r0;
     if (a.vec && r0 + kB <= a.rows) {
         constexpr int kPer = 16 / sizeof(T), kPieces = kB / kPer;
-#pragma unroll 4
+#pragma unroll
         for (int i = threadIdx.x; i < kB * kPieces; i += kThreads) {
             const uint32_t c = i / kPieces, r = (i - c * kPieces) * kPer;
             const bool there = c0 + c < a.cols;
@@ -158,7 +187,18 @@ __global__ void __launch_bounds__(kThreads) quantize_turned_kernel(const Quantiz
                          :: "r"((uint32_t)__cvta_generic_to_shared(tile + c * kB + r)), "l"(src), "r"(there ? 16 : 0) : "memory");
         }
         asm volatile("cp.async.commit_group;\n cp.async.wait_group 0;" ::: "memory");
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll 16
+        for (int i = threadIdx.x; i < kB * kB; i += kThreads) {
+            const uint32_t c = i / kB, r = i - c * kB;
+            const bool there = c0 + c < a.cols && r0 + r < a.rows;
+            const T* src = there ? x + (long long)(c0 + c) * a.col_stride + r : static_cast<const T*>(a.x);
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
+                         :: "r"((uint32_t)__cvta_generic_to_shared(tile + c * kB + r)), "l"(src), "r"(there ? 4 : 0) : "memory");
+        }
+        asm volatile("cp.async.commit_group;\n cp.async.wait_group 0;" ::: "memory");
     } else {
+#pragma unroll 16
         for (int i = threadIdx.x; i < kB * kB; i += kThreads) {
             const uint32_t c = i / kB, r = i - c * kB;
             tile[c * kB + r] = c0 + c < a.cols && r0 + r < a.rows ? x[(long long)(c0 + c) * a.col_stride + r] : T(0.0f);
@@ -181,13 +221,14 @@ __global__ void __launch_bounds__(kThreads) quantize_turned_kernel(const Quantiz
         top = block_max(top, tops);
     }
     const float scale = scale_of<kE5m2>(top);
+    const Quotient by(scale);
     if (r0 + r < a.rows) {
         uint8_t* out = a.values + z * a.values_batch + (r0 + r) * a.values_stride + c0 + half * (kB / 2);
 #pragma unroll
         for (int i = 0; i < kB / 2; i += 16)
             if (c0 + half * (kB / 2) + i < a.cols)
-                *reinterpret_cast<uint4*>(out + i) = make_uint4(four_of<kE5m2>(v + i, scale), four_of<kE5m2>(v + i + 4, scale),
-                                                               four_of<kE5m2>(v + i + 8, scale), four_of<kE5m2>(v + i + 12, scale));
+                *reinterpret_cast<uint4*>(out + i) = make_uint4(four_of<kE5m2>(v + i, by), four_of<kE5m2>(v + i + 4, by),
+                                                               four_of<kE5m2>(v + i + 8, by), four_of<kE5m2>(v + i + 12, by));
         if (a.block_rows == 1 && half == 0) a.scales[((uint64_t)z * a.rows + r0 + r) * blocks + bc] = scale;
     }
     if (a.block_rows != 1 && threadIdx.x == 0) a.scales[((uint64_t)z * ((a.rows + kB - 1) / kB) + br) * blocks + bc] = scale;

@@ -22,6 +22,8 @@ from . import _lib
 __all__ = ["gated_delta_rule", "gated_delta_step"]
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_FLOATING = frozenset((torch.float32, torch.bfloat16, torch.float16, torch.float64))
+_PLACES = frozenset(("cuda", "meta"))
 _PROBLEM = struct.Struct("=9If7Q15q")
 
 
@@ -30,7 +32,23 @@ def _fail(name, message, kind=ValueError):
 
 
 def _check(name, q, k, v, g, beta):
-    """The inputs as the library takes them (float32 gates, last dimensions contiguous), and the sizes."""
+    """Refuses inputs the library cannot take; returns their sizes."""
+    try:
+        shape, v_shape, dtype, device = q.shape, v.shape, q.dtype, q.device
+        fine = (len(shape) == 4 and len(v_shape) == 4 and k.shape == shape and v_shape[:2] == shape[:2] and dtype in _DTYPES
+                and k.dtype == dtype and v.dtype == dtype and g.shape == v_shape[:3] and beta.shape == v_shape[:3]
+                and g.dtype in _FLOATING and beta.dtype in _FLOATING and v_shape[2] % max(shape[2], 1) == 0 and shape[2] and v_shape[2]
+                and 1 <= shape[3] <= 128 and 1 <= v_shape[3] <= 256 and device.type in _PLACES
+                and k.device == device and v.device == device and g.device == device and beta.device == device)
+    except AttributeError:
+        fine = False
+    if not fine:
+        _explain(name, q, k, v, g, beta)
+    return (*shape, *v_shape[2:])
+
+
+def _explain(name, q, k, v, g, beta):
+    """Says what is wrong with inputs that _check found wanting."""
     for what, x in (("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta)):
         if not isinstance(x, Tensor):
             _fail(name, f"{what} must be a tensor, got {type(x).__name__}", TypeError)
@@ -38,12 +56,12 @@ def _check(name, q, k, v, g, beta):
         _fail(name, f"q, k and v must be float32, bfloat16 or float16, got {q.dtype}", TypeError)
     if k.dtype != q.dtype or v.dtype != q.dtype:
         _fail(name, f"q, k and v must have one dtype, got {q.dtype}, {k.dtype} and {v.dtype}", TypeError)
-    if not (g.is_floating_point() and beta.is_floating_point()):
+    if g.dtype not in _FLOATING or beta.dtype not in _FLOATING:
         _fail(name, f"g and beta must be floating point, got {g.dtype} and {beta.dtype}", TypeError)
     if q.dim() != 4 or v.dim() != 4 or k.shape != q.shape or v.shape[:2] != q.shape[:2]:
         _fail(name, "expected q and k [B, T, H, Dk] and v [B, T, HV, Dv], got "
                     f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
-    b, t, h, dk = q.shape
+    h, dk = q.shape[2:]
     hv, dv = v.shape[2:]
     if g.shape != v.shape[:3] or beta.shape != v.shape[:3]:
         _fail(name, f"expected g and beta [B, T, HV] = {tuple(v.shape[:3])}, got {tuple(g.shape)} and {tuple(beta.shape)}")
@@ -51,13 +69,12 @@ def _check(name, q, k, v, g, beta):
         _fail(name, f"the {hv} heads of v must be a multiple of the {h} of q and k")
     if not 1 <= dk <= 128 or not 1 <= dv <= 256:
         _fail(name, f"Dk must be 1 to 128 and Dv 1 to 256, got {dk} and {dv}")
-    device = q.device
-    if device.type not in ("cuda", "meta"):
-        _fail(name, f"tensors on {device} are not supported; use CUDA (this library has no CPU path)")
+    if q.device.type not in _PLACES:
+        _fail(name, f"tensors on {q.device} are not supported; use CUDA (this library has no CPU path)")
     for what, x in (("k", k), ("v", v), ("g", g), ("beta", beta)):
-        if x.device != device:
-            _fail(name, f"{what} is on {x.device}, q on {device}")
-    return b, t, h, dk, hv, dv
+        if x.device != q.device:
+            _fail(name, f"{what} is on {x.device}, q on {q.device}")
+    _fail(name, "unsupported inputs")
 
 
 def _rows(x):
@@ -75,17 +92,14 @@ def _scale(scale, dk):
 def _problem(q, k, v, g, beta, scale, initial=None, cu=None, index_bytes=4):
     """A metal_linalg_delta as bytes."""
     b, t, h, dk = q.shape
-    hv, dv = v.shape[2:]
+    _, _, hv, dv = v.shape
+    q0, q1, q2, _ = q.stride()
+    k0, k1, k2, _ = k.stride()
+    v0, v1, v2, _ = v.stride()
     return _PROBLEM.pack(b, t, h, hv, dk, dv, 0 if cu is None else cu.numel() - 1, _DTYPES[q.dtype], index_bytes, scale,
                          q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
                          0 if initial is None else initial.data_ptr(), 0 if cu is None else cu.data_ptr(),
-                         *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride())
-
-
-def _on_stream(device):
-    """Sets the library's stream to torch's current one of `device` (kernels run on the pointers' device whatever the
-    current one is)."""
-    _lib.lib.metal_linalg_set_stream(torch.cuda.current_stream(device).cuda_stream)
+                         q0, q1, q2, k0, k1, k2, v0, v1, v2, *g.stride(), *beta.stride())
 
 
 def _workspace(problem, backward, device):
@@ -112,11 +126,11 @@ def _forward(q, k, v, g, beta, scale, initial, cu):
     cu = None if cu is None else cu.contiguous()
     n = q.shape[0] if cu is None else cu.numel() - 1
     hv, dv = v.shape[2:]
-    o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    last = torch.empty((n, hv, q.shape[3], dv), dtype=torch.float32, device=v.device)
+    o = v.new_empty(v.shape)
+    last = g.new_empty((n, hv, q.shape[3], dv))
     p = _problem(q, k, v, g, beta, scale, initial, cu, 4 if cu is None else cu.element_size())
     ws = _workspace(p, False, v.device)
-    _on_stream(v.device)
+    _lib.use_stream_of(v)
     _lib.check(_lib.lib.metal_linalg_gated_delta_rule(p, o.data_ptr(), last.data_ptr(), ws.data_ptr(), ws.numel()))
     return o, last
 
@@ -125,13 +139,13 @@ def _backward(d_o, d_last, q, k, v, g, beta, scale, initial, cu):
     q, k, v, d_o = _rows(q), _rows(k), _rows(v), _rows(d_o)
     d_last = None if d_last is None else d_last.contiguous()
     cu = None if cu is None else cu.contiguous()
-    new = lambda x: torch.empty(x.shape, dtype=x.dtype, device=x.device)  # noqa: E731
+    new = lambda x: x.new_empty(x.shape)  # noqa: E731
     dq, dk, dv, dg, dbeta = new(q), new(k), new(v), new(g), new(beta)
     d_initial = None if initial is None else new(initial)
     p = _problem(q, k, v, g, beta, scale, initial, cu, 4 if cu is None else cu.element_size())
     ws = _workspace(p, True, v.device)
     strides = struct.pack("=3q", *d_o.stride()[:3])
-    _on_stream(v.device)
+    _lib.use_stream_of(v)
     _lib.check(_lib.lib.metal_linalg_gated_delta_rule_backward(
         p, d_o.data_ptr(), strides, None if d_last is None else d_last.data_ptr(), dq.data_ptr(), dk.data_ptr(),
         dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(), None if d_initial is None else d_initial.data_ptr(),
@@ -242,9 +256,9 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, cu_seq
 def _step(q, k, v, g, beta, state, slots, scale):
     q, k, v = _rows(q), _rows(k), _rows(v)
     slots = None if slots is None else slots.contiguous()
-    o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    o = v.new_empty(v.shape)
     p = _problem(q, k, v, g, beta, scale, None, None, 4 if slots is None else slots.element_size())
-    _on_stream(v.device)
+    _lib.use_stream_of(v)
     _lib.check(_lib.lib.metal_linalg_gated_delta_step(p, o.data_ptr(), state.data_ptr(), state.stride(0), state.shape[0],
                                                       None if slots is None else slots.data_ptr()))
     return o
@@ -278,9 +292,10 @@ def gated_delta_step(q, k, v, g, beta, state, *, slots=None, scale=None):
         _fail(name, f"expected state [S, {hv}, {dk}, {dv}], got {tuple(state.shape)}")
     if state.device != q.device:
         _fail(name, f"state is on {state.device}, q on {q.device}")
-    if state.numel() and not state[0].is_contiguous():
+    s0, s1, s2, s3 = state.stride()
+    if state.numel() and (s3 != 1 and dv > 1 or s2 != dv and dk > 1 or s1 != dk * dv and hv > 1):
         _fail(name, f"each slot of state must be contiguous, got strides {tuple(state.stride())}")
-    if state.shape[0] > 1 and state.stride(0) < hv * dk * dv:
+    if state.shape[0] > 1 and s0 < hv * dk * dv:
         _fail(name, "the slots of state overlap")
     if slots is not None:
         if not isinstance(slots, Tensor) or slots.dtype not in (torch.int32, torch.int64):
@@ -289,7 +304,8 @@ def gated_delta_step(q, k, v, g, beta, state, *, slots=None, scale=None):
             _fail(name, f"expected slots [{b}] on {q.device}, got {tuple(slots.shape)} on {slots.device}")
     elif b > state.shape[0]:
         _fail(name, f"{b} rows and {state.shape[0]} slots: name them with slots")
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, g, beta, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
+                                    beta.requires_grad or state.requires_grad):
         _fail(name, "not differentiable; use gated_delta_rule for training, or torch.no_grad()", RuntimeError)
     scale = _scale(scale, dk)
     g, beta = _float(g), _float(beta)

@@ -29,37 +29,45 @@ def _fail(name, message, kind=ValueError):
 def _on_gpu(name, what, x):
     if not isinstance(x, Tensor):
         _fail(name, f"{what} must be a tensor, got {type(x).__name__}", TypeError)
-    if x.device.type not in ("cuda", "meta"):
+    if not x.is_cuda and not x.is_meta:
         _fail(name, f"tensors on {x.device} are not supported; use CUDA (this library has no CPU path)")
 
 
-def _on_stream(device):
-    _lib.lib.metal_linalg_set_stream(torch.cuda.current_stream(device).cuda_stream)
-
-
-def _padded(lead, rows, cols, dtype, device):
-    """An uninitialised [..., rows, cols] whose rows lie a multiple of 16 bytes apart."""
+def _padded(x, lead, rows, cols, dtype):
+    """An uninitialised [..., rows, cols] on x's device whose rows lie a multiple of 16 bytes apart."""
     wide = -(-cols // 16) * 16
-    return torch.empty((*lead, rows, wide), dtype=dtype, device=device)[..., :cols]
+    values = x.new_empty((*lead, rows, wide), dtype=dtype)
+    return values if wide == cols else values[..., :cols]
 
 
 def _quantize(x, block_rows, transpose, dtype):
-    if transpose:
-        x = x.mT
     *lead, m, n = x.shape
-    x3 = x.reshape(-1, m, n) if len(lead) != 1 else x       # copies only what no strides can describe
-    if x3.numel() and x3.stride(1) != 1 and x3.stride(2) != 1:
-        x3 = x3.contiguous()
-    values = _padded(lead, m, n, dtype, x.device)
-    scales = torch.empty((*lead, -(-m // block_rows), -(-n // 128)), dtype=torch.float32, device=x.device)
-    if values.numel():
-        # a dimension of one may carry any stride: it is given one the library can read along
-        rows, cols = x3.stride(1), x3.stride(2)
-        if n == 1:
-            cols = 1
-        _on_stream(x.device)
-        _lib.check(_lib.lib.metal_linalg_quantize_fp8(x3.data_ptr(), _DTYPES[x.dtype], x3.shape[0], m, n, x3.stride(0), rows, cols,
-                                                      block_rows, _KINDS[dtype], values.data_ptr(), -(-n // 16) * 16, scales.data_ptr()))
+    *outer, rows, cols = x.stride()
+    if transpose:
+        m, n, rows, cols = n, m, cols, rows
+    values = _padded(x, lead, m, n, dtype)
+    scales = x.new_empty((*lead, -(-m // block_rows), -(-n // 128)), dtype=torch.float32)
+    if not values.numel():
+        return values, scales
+    # a dimension of one may carry any stride: it is given one the library can read along
+    if n == 1:
+        cols = 1
+    elif m == 1 and cols != 1:
+        rows = 1
+    batch, across = 1, 0
+    if len(lead) == 1:
+        (batch,), (across,) = lead, outer
+    elif lead or (rows != 1 and cols != 1):
+        x = x.reshape(-1, *x.shape[-2:])                # copies only what no strides can describe
+        batch, across = x.shape[0], x.stride(0)
+        rows, cols = (x.stride(2), x.stride(1)) if transpose else (x.stride(1), x.stride(2))
+    if rows != 1 and cols != 1 and n > 1:
+        x = x.contiguous()
+        across = x.stride(0) if x.dim() == 3 else 0
+        rows, cols = (1, m) if transpose else (n, 1)
+    _lib.use_stream_of(x)
+    _lib.check(_lib.lib.metal_linalg_quantize_fp8(x.data_ptr(), _DTYPES[x.dtype], batch, m, n, across, rows, cols, block_rows,
+                                                  _KINDS[dtype], values.data_ptr(), -(-n // 16) * 16, scales.data_ptr()))
     return values, scales
 
 
@@ -114,37 +122,41 @@ def _block_rows(name, what, rows, scales_rows):
 def _operand(x, scale, block_rows, batched):
     """A metal_linalg_fp8_operand as bytes, and the tensors it points to. What the library cannot read in place (rows that
     are not a multiple of 16 bytes apart, say) is copied once."""
-    stride = x.stride(-2) if x.shape[-2] > 1 else -(-x.shape[-1] // 16) * 16
-    across = x.stride(0) if batched else 0
-    if (x.stride(-1) != 1 and x.shape[-1] > 1) or stride < x.shape[-1] or stride % 16 or x.data_ptr() % 16 or \
-            across % stride or (batched and x.shape[0] > 1 and across < stride * x.shape[-2]):
-        copy = _padded(x.shape[:-2], *x.shape[-2:], x.dtype, x.device)
+    *_, m, k = x.shape
+    *outer, stride, one = x.stride()
+    if m == 1:
+        stride = -(-k // 16) * 16                       # any stride will do
+    across = outer[0] if batched else 0
+    at = x.data_ptr()
+    if (one != 1 and k > 1) or stride < k or stride % 16 or at % 16 or (batched and (across % stride or across < stride * m)):
+        copy = _padded(x, x.shape[:-2], m, k, x.dtype)
         copy.copy_(x)
-        x = copy
-        stride = x.stride(-2)
-        across = x.stride(0) if batched else 0
+        x, at, stride = copy, copy.data_ptr(), -(-k // 16) * 16
+        across = stride * m if batched else 0
     scale = scale.contiguous()
-    return _OPERAND.pack(x.data_ptr(), scale.data_ptr(), stride, across, _KINDS[x.dtype], block_rows), (x, scale)
+    return _OPERAND.pack(at, scale.data_ptr(), stride, across, _KINDS[x.dtype], block_rows), (x, scale)
 
 
 def _matmul(a, a_scale, b, b_scale, a_rows, b_rows, out_dtype):
     *lead, m, k = a.shape
     n = b.shape[-2]
-    out = torch.empty((*lead, m, n), dtype=out_dtype, device=a.device)
-    if out.numel() == 0:
+    out = a.new_empty((*lead, m, n), dtype=out_dtype)
+    if not out.numel():
         return out
     if k == 0:
         return out.zero_()
-    batch = out.numel() // (m * n)
-    if len(lead) > 1:
-        a = a.reshape(-1, m, k)
-        if b.dim() > 2:
-            b = b.reshape(-1, n, k)
-    if b.dim() == 2 and a.dim() == 3 and a_rows == 1 and a.stride(0) == m * a.stride(1):
-        a, m, batch = a.flatten(0, 1), batch * m, 1      # one matrix for the whole batch: the rows behind one another
-    pa, keep_a = _operand(a, a_scale, a_rows, a.dim() == 3 and batch > 1)
-    pb, keep_b = _operand(b, b_scale, b_rows, b.dim() == 3 and batch > 1)
-    _on_stream(out.device)
+    batch = 1
+    if lead:
+        batch = out.numel() // (m * n)
+        if len(lead) > 1:
+            a = a.reshape(-1, m, k)
+            if b.dim() > 2:
+                b = b.reshape(-1, n, k)
+        if b.dim() == 2 and a_rows == 1 and a.stride(0) == m * a.stride(1):
+            a, m, batch = a.flatten(0, 1), batch * m, 1      # one matrix for the whole batch: the rows behind one another
+    pa, keep_a = _operand(a, a_scale, a_rows, batch > 1)
+    pb, keep_b = _operand(b, b_scale, b_rows, batch > 1 and b.dim() == 3)
+    _lib.use_stream_of(out)
     _lib.check(_lib.lib.metal_linalg_matmul_fp8(pa, pb, batch, m, n, k, out.data_ptr(), _DTYPES[out_dtype]))
     return out
 
@@ -170,8 +182,9 @@ def matmul_fp8(a, a_scale, b, b_scale, *, out_dtype=torch.bfloat16):
     name = "matmul_fp8"
     for what, x in (("a", a), ("a_scale", a_scale), ("b", b), ("b_scale", b_scale)):
         _on_gpu(name, what, x)
-        if x.device != a.device:
-            _fail(name, f"{what} is on {x.device}, a on {a.device}")
+    device = a.device
+    if a_scale.device != device or b.device != device or b_scale.device != device:
+        _fail(name, f"a, a_scale, b and b_scale must be on one device, got {device}, {a_scale.device}, {b.device} and {b_scale.device}")
     if a.dtype not in _KINDS or b.dtype not in _KINDS:
         _fail(name, f"a and b must be float8_e4m3fn or float8_e5m2, got {a.dtype} and {b.dtype}", TypeError)
     if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
@@ -186,7 +199,7 @@ def matmul_fp8(a, a_scale, b, b_scale, *, out_dtype=torch.bfloat16):
             _fail(name, f"expected {what}_scale [..., rows, {blocks}] for {tuple(x.shape)}, got {tuple(s.shape)}")
     a_rows = _block_rows(name, "a", a.shape[-2], a_scale.shape[-2])
     b_rows = _block_rows(name, "b", b.shape[-2], b_scale.shape[-2])
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (a, a_scale, b, b_scale)):
+    if torch.is_grad_enabled() and (a.requires_grad or a_scale.requires_grad or b.requires_grad or b_scale.requires_grad):
         _fail(name, "not differentiable; use linear_fp8, or detach the operands", RuntimeError)
     if torch.compiler.is_compiling() or a.device.type == "meta":
         return torch.ops.metal_linalg.matmul_fp8(a, a_scale, b, b_scale, a_rows, b_rows, out_dtype)

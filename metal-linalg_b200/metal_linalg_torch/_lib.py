@@ -100,6 +100,21 @@ def check(status):
     raise RuntimeError(message)
 
 
+# The address of torch's current stream of a device, without an object around it (2 us less a call); bound at the first use,
+# since this module does without torch otherwise.
+_raw_stream = None
+
+
+def use_stream_of(x):
+    """Sets this thread's stream to torch's current one on tensor x's device (the kernels run on the pointers' device,
+    whichever is current)."""
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = torch._C._cuda_getCurrentRawStream
+    lib.metal_linalg_set_stream(_raw_stream(x.get_device()))
+
+
 def qr(a, batch, rows, cols, q, r, mode="reduced", stream=None):
     """metal_linalg_qr_with_mode on addresses (ints; None for NULL). `stream` is a
     cudaStream_t as an int for device pointers (None: leave this thread's as set)."""
