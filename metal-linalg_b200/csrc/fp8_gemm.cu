@@ -43,7 +43,7 @@ struct GemmArgs {
     uint32_t p_shift, q_shift;         // log2 of the scale blocks' rows: 0 or 7
     uint32_t p_tiles, q_tiles, tiles;  // tiles = p_tiles * q_tiles * batch
     uint32_t batched_p, batched_q;     // 0: the operand is one matrix for the whole batch
-    uint32_t split;                    // blocks that share a tile
+    uint32_t split, split_log;         // blocks that share a tile, a power of two
     uint32_t idesc;
     void*    c;
     uint64_t c_batch;
@@ -51,6 +51,15 @@ struct GemmArgs {
     uint32_t c_dtype;
     uint32_t wide;                     // C's rows (ldq == 1) can be written in 16-byte pieces
     unsigned* status;
+
+    // Tile t's matrix, first row and first column: tiles of a column of C behind one another.
+    template <int BN> __device__ __forceinline__ void place(uint32_t t, uint32_t& z, uint32_t& p0, uint32_t& q0) const {
+        z = t / (p_tiles * q_tiles);
+        t -= z * p_tiles * q_tiles;
+        q0 = t / p_tiles;
+        p0 = (t - q0 * p_tiles) * kRowsTile;
+        q0 *= BN;
+    }
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -68,14 +77,25 @@ __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
                  : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done != 0;
 }
+// The one lane of a converged warp that issues its copies or products. The compiler knows that elect.sync leaves one lane, and
+// so gives tcgen05 and TMA instructions their uniform operands directly; behind `lane == 0` it asks lane by lane (four
+// products and two commits: 365 clocks, 100 this way).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one) :: "memory");
+    return one != 0;
+}
 // False if the wait ran out, here or (sooner) anywhere else in the block.
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* failed) {
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* failed) {
     for (uint32_t i = 0; i < kWaitLimit; ++i) {
         if (try_wait(bar, parity)) return true;
         if ((i & 15) == 15 && *failed) return false;
     }
     *failed = 1;
     return false;
+}
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* failed) {
+    return try_wait(bar, parity) || wait_on(bar, parity, failed);
 }
 
 template <int N> struct TmemLoad;
@@ -104,19 +124,47 @@ __device__ __forceinline__ void store_one(void* c, uint64_t at, uint32_t dtype, 
     else if (dtype == METAL_LINALG_FLOAT16) static_cast<__half*>(c)[at] = __float2half_rn(v);
     else static_cast<float*>(c)[at] = v;
 }
-__device__ __forceinline__ uint32_t pack_two(uint32_t dtype, float a, float b) {
+__device__ __forceinline__ uint32_t pack_two(uint32_t dtype, float2 v) {
     if (dtype == METAL_LINALG_BFLOAT16) {
-        const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+        const __nv_bfloat162 r = __floats2bfloat162_rn(v.x, v.y);
         return *reinterpret_cast<const uint32_t*>(&r);
     }
-    const __half2 r = __floats2half2_rn(a, b);
+    const __half2 r = __floats2half2_rn(v.x, v.y);
     return *reinterpret_cast<const uint32_t*>(&r);
 }
+
+// Two neighbouring sums in one 64-bit register: sum += (x, y) * by.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair_of(float x, float y) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 both_of(Pair p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ void add_scaled(Pair& sum, uint32_t x, uint32_t y, Pair by) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum) : "l"(pair_of(__uint_as_float(x), __uint_as_float(y))), "l"(by));
+}
+__device__ __forceinline__ Pair times(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+template <int N> constexpr uint32_t kLog = 1 + kLog<N / 2>;
+template <> constexpr uint32_t kLog<1> = 0;
 
 template <int BN>
 struct Shape {
     static constexpr int kEpilogueWarps = BN >= 128 ? 8 : 4;
-    static constexpr int kThreads = 32 * (kEpilogueWarps + 2);
+    // 256 columns: 128 sums and two loads of 32 a thread are more registers than twelve warps' even share (168), so the four
+    // warps behind the epilogue's (two of them idle: registers change hands by fours) give theirs up: 256 x 224 + 128 x 56
+    // of the launch's 384 x 168
+    static constexpr bool kUneven = BN == 256;
+    static constexpr int kThreads = 32 * (kEpilogueWarps + (kUneven ? 4 : 2));
     static constexpr int kCols = BN / (kEpilogueWarps / 4);        // columns an epilogue thread sums
     static constexpr int kAcc = BN == 256 ? 2 : 4;                 // accumulators in tensor memory
     static constexpr int kTmem = kAcc * BN < 32 ? 32 : kAcc * BN;
@@ -173,86 +221,48 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     }
 
-    if (warp == S::kEpilogueWarps) {            // loads
-        if (lane == 0) {
-            uint32_t i = 0;                     // blocks of k so far
-            bool ok = true;
-            for (uint32_t tile = first; ok && tile < a.tiles; tile += step) {
-                const uint32_t z = tile / (a.p_tiles * a.q_tiles), t = tile - z * a.p_tiles * a.q_tiles;
-                const int p0 = (int)(t % a.p_tiles) * kRowsTile, q0 = (int)(t / a.p_tiles) * BN;
-                const int zp = a.batched_p ? (int)z : 0, zq = a.batched_q ? (int)z : 0;
-                for (uint32_t kb = kb0; kb < kb1; ++kb, ++i) {
-                    const uint32_t s = i % S::kStages, round = i / S::kStages;
-                    if (round && !wait(smem_u32(&empty[s]), (round - 1) & 1, failed)) { ok = false; break; }
-                    const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(base + s * S::kStageBytes);
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "n"(S::kStageBytes) : "memory");
-                    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                                 :: "r"(dst), "l"(&map_p), "r"((int)(kb * kBlockK)), "r"(p0), "r"(zp), "r"(bar) : "memory");
-                    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                                 :: "r"(dst + kRowsTile * kBlockK), "l"(&map_q), "r"((int)(kb * kBlockK)), "r"(q0), "r"(zq), "r"(bar) : "memory");
-                }
-            }
-            if (!ok) {                          // nothing of this block's is on its way when it ends
-                for (uint32_t j = i > (uint32_t)S::kStages ? i - S::kStages : 0; j < i; ++j)
-                    for (uint32_t n = 0; n < kWaitLimit && !try_wait(smem_u32(&full[j % S::kStages]), (j / S::kStages) & 1); ++n) {}
-            }
-        }
-        __syncwarp();
-    } else if (warp == S::kEpilogueWarps + 1) { // products
-        if (lane == 0) {
-            uint32_t i = 0;
-            bool ok = true;
-            for (uint32_t tile = first; ok && tile < a.tiles; tile += step)
-                for (uint32_t kb = kb0; kb < kb1; ++kb, ++i) {
-                    const uint32_t s = i % S::kStages, acc = i % S::kAcc;
-                    if (i >= (uint32_t)S::kAcc && !wait(smem_u32(&acc_empty[acc]), (i / S::kAcc - 1) & 1, failed)) { ok = false; break; }
-                    if (!wait(smem_u32(&full[s]), (i / S::kStages) & 1, failed)) { ok = false; break; }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t at = smem_u32(base + s * S::kStageBytes);
-                    const uint64_t dp = tile_desc(at), dq = tile_desc(at + kRowsTile * kBlockK);
-#pragma unroll
-                    for (int j = 0; j < kBlockK / 32; ++j)
-                        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                                     " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
-                                     :: "r"(tmem + acc * BN), "l"(dp + 2 * j), "l"(dq + 2 * j), "r"(a.idesc), "r"(j) : "memory");
-                    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(smem_u32(&empty[s])) : "memory");
-                    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(smem_u32(&acc_full[acc])) : "memory");
-                }
-            if (!ok) {
-                asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(smem_u32(&drain)) : "memory");
-                for (uint32_t n = 0; n < kWaitLimit && !try_wait(smem_u32(&drain), 0); ++n) {}
-            }
-        }
-        __syncwarp();
-    } else {                                    // sums
+    if (warp < S::kEpilogueWarps) {             // sums
+        if constexpr (S::kUneven) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quarter = warp & 3, part = warp >> 2;
         const uint32_t row = 32 * quarter + lane;
         float* my_scales = scales + warp * 2 * S::kCols;
         uint32_t i = 0;
         bool ok = true;
         for (uint32_t tile = first; tile < a.tiles; tile += step) {
-            const uint32_t z = tile / (a.p_tiles * a.q_tiles), t = tile - z * a.p_tiles * a.q_tiles;
-            const uint32_t p = (t % a.p_tiles) * kRowsTile + row, q0 = (t / a.p_tiles) * BN + part * S::kCols;
-            const float* sp = a.sp + (a.batched_p ? z * a.sp_batch : 0) + (uint64_t)(min(p, a.p - 1) >> a.p_shift) * a.kb;
-            const float* sq = a.sq + (a.batched_q ? z * a.sq_batch : 0);
-            float sum[S::kCols];
+            const float *sp, *sq;               // this block's first scales of the thread's row, of its columns
+            uint32_t q_scales = 0;              // by column: how many of this lane's columns exist
+            {
+                uint32_t z, p, q0;
+                a.place<BN>(tile, z, p, q0);
+                p = min(p + row, a.p - 1);
+                q0 += part * S::kCols;
+                sp = a.sp + (a.batched_p ? z * a.sp_batch : 0) + (uint64_t)(p >> a.p_shift) * a.kb + kb0;
+                sq = a.sq + (a.batched_q ? z * a.sq_batch : 0) + kb0;
+                if constexpr (kByColumn) {
+                    sq += (uint64_t)(q0 + lane) * a.kb;
+                    q_scales = q0 + lane < a.q ? (min(a.q - q0, (uint32_t)S::kCols) - lane + 31) / 32 : 0;
+                    if (lane >= S::kCols) q_scales = 0;
+                } else {
+                    sq += (uint64_t)(min(q0, a.q - 1) >> 7) * a.kb;
+                }
+            }
+            Pair sum[S::kCols / 2];
 #pragma unroll
-            for (int j = 0; j < S::kCols; ++j) sum[j] = 0.0f;
+            for (int j = 0; j < S::kCols / 2; ++j) sum[j] = 0;
             // the next block's scales are fetched while this one's product is awaited
             float row_scale = 0.0f, col_scale[kByColumn ? (S::kCols + 31) / 32 : 1];
-            const auto fetch = [&](uint32_t kb) {
-                row_scale = __ldg(sp + kb);
+            const auto fetch = [&]() {
+                row_scale = __ldg(sp++);
                 if constexpr (kByColumn) {
 #pragma unroll
-                    for (int j = 0; j < (S::kCols + 31) / 32; ++j) {
-                        const uint32_t q = q0 + 32 * j + lane;
-                        col_scale[j] = q < a.q && 32 * j + lane < (uint32_t)S::kCols ? __ldg(sq + (uint64_t)q * a.kb + kb) : 0.0f;
-                    }
+                    for (uint32_t j = 0; j < (S::kCols + 31) / 32; ++j) col_scale[j] = j < q_scales ? __ldg(sq + (uint64_t)(32 * j) * a.kb) : 0.0f;
                 } else {
-                    col_scale[0] = q0 < a.q ? __ldg(sq + (uint64_t)(q0 >> 7) * a.kb + kb) : 0.0f;
+                    col_scale[0] = __ldg(sq);
                 }
+                ++sq;
             };
-            if (kb0 < kb1) fetch(kb0);
+            if (kb0 < kb1) fetch();
+#pragma unroll 1
             for (uint32_t kb = kb0; ok && kb < kb1; ++kb, ++i) {
                 const uint32_t acc = i % S::kAcc;
                 float scale = row_scale;
@@ -265,72 +275,169 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
                 } else {
                     scale *= col_scale[0];
                 }
-                if (kb + 1 < kb1) fetch(kb + 1);
+                const Pair scale2 = pair_of(scale, scale);
+                if (kb + 1 < kb1) fetch();
                 ok = wait(smem_u32(&acc_full[acc]), (i / S::kAcc) & 1, failed);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = __all_sync(0xffffffffu, ok);       // (one lane asking for its warp was 8 % slower)
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t at = tmem + acc * BN + part * S::kCols + ((32u * quarter) << 16);
-                constexpr int kPiece = S::kCols >= 32 ? 32 : 16;
-                uint32_t v[2][kPiece];
-                TmemLoad<kPiece>::load(v[0], at);
+                // two loads in flight; the next two go out as their registers are used up
+                constexpr int kPiece = S::kCols >= 32 ? 32 : 16, kFlight = S::kCols > kPiece ? 2 : 1;
+                uint32_t v[kFlight][kPiece];
 #pragma unroll
-                for (int j = 0; j < S::kCols; j += kPiece) {
-                    const int w = (j / kPiece) & 1;
+                for (int f = 0; f < kFlight; ++f) TmemLoad<kPiece>::load(v[f], at + f * kPiece);
+#pragma unroll
+                for (int j = 0; j < S::kCols; j += kFlight * kPiece) {
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (j + kPiece < S::kCols) TmemLoad<kPiece>::load(v[w ^ 1], at + j + kPiece);
-                    else {                      // everything is read: the accumulator is free
+                    if (j + kFlight * kPiece >= S::kCols) {     // everything is read: the accumulator is free
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         if (lane == 0)
                             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(smem_u32(&acc_empty[acc])) : "memory");
                     }
 #pragma unroll
-                    for (int e = 0; e < kPiece; ++e) {
-                        if constexpr (kByColumn) sum[j + e] = fmaf(__uint_as_float(v[w][e]), scale * by_column[j + e], sum[j + e]);
-                        else                     sum[j + e] = fmaf(__uint_as_float(v[w][e]), scale, sum[j + e]);
+                    for (int f = 0; f < kFlight; ++f) {
+#pragma unroll
+                        for (int e = 0; e < kPiece; e += 4) {
+                            const int to = j + f * kPiece + e;
+                            Pair by[2] = {scale2, scale2};
+                            if constexpr (kByColumn) {
+                                const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(by_column + to);
+                                by[0] = times(scale2, c.x);
+                                by[1] = times(scale2, c.y);
+                            }
+                            add_scaled(sum[to / 2], v[f][e], v[f][e + 1], by[0]);
+                            add_scaled(sum[to / 2 + 1], v[f][e + 2], v[f][e + 3], by[1]);
+                        }
+                        if (j + (kFlight + f) * kPiece < S::kCols) TmemLoad<kPiece>::load(v[f], at + j + (kFlight + f) * kPiece);
                     }
                 }
             }
             if (!ok)
 #pragma unroll
-                for (int j = 0; j < S::kCols; ++j) sum[j] = qnan();
+                for (int j = 0; j < S::kCols / 2; ++j) sum[j] = pair_of(qnan(), qnan());
 
             if constexpr (S::kReduceBytes > 0) {
                 if (a.split > 1) {
                     // block r of the cluster adds columns r * BN / split ..: part `rank` of everyone's, in the ranks' order
-                    const uint32_t mine = BN / a.split;
+                    const uint32_t log = kLog<BN> - a.split_log;        // of a share's columns
                     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");       // everyone has started
+                    // [rank][row][column], four columns at a time; rows' quads are permuted so that neighbouring lanes
+                    // meet different banks
 #pragma unroll
-                    for (int j = 0; j < S::kCols; ++j) {
-                        const uint32_t q = part * S::kCols + j, to = q / mine, slot = q - to * mine;
-                        const uint32_t local = smem_u32(reduce + (rank * mine + slot) * kRowsTile + row);
+                    for (int j = 0; j < S::kCols; j += 4) {
+                        const float2 f = both_of(sum[j / 2]), g = both_of(sum[j / 2 + 1]);
+                        const uint32_t q = part * S::kCols + j, to = q >> log, quad = (q & ((1u << log) - 1)) >> 2;
+                        const uint32_t local = smem_u32(reduce) + (((rank * kRowsTile + row) << log) << 2) +
+                                               ((quad ^ (row & ((1u << log) / 4 - 1) & 7)) << 4);
                         uint32_t remote;
                         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(to));
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" :: "r"(remote), "f"(sum[j]) : "memory");
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" :: "r"(remote), "f"(f.x), "f"(f.y), "f"(g.x), "f"(g.y) : "memory");
                     }
                 }
             }
+            uint32_t again = tile, z, p, q0;            // worked out anew: the sums leave no registers to keep it in
+            asm volatile("" : "+r"(again));
+            a.place<BN>(again, z, p, q0);
+            p += row;
+            q0 += part * S::kCols;
             if (a.split == 1 && p < a.p) {
-                const uint64_t at = z * a.c_batch + (uint64_t)p * a.ldp + (uint64_t)q0 * a.ldq;
+                uint64_t ldq = a.ldq;           // (nor to keep its multiples in)
+                asm volatile("" : "+l"(ldq));
+                uint64_t at = z * a.c_batch + (uint64_t)p * a.ldp + (uint64_t)q0 * ldq;
                 if (a.wide && q0 + S::kCols <= a.q) {
                     if (a.c_dtype == METAL_LINALG_FLOAT32) {
 #pragma unroll
-                        for (int j = 0; j < S::kCols; j += 4)
-                            *reinterpret_cast<float4*>(static_cast<float*>(a.c) + at + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+                        for (int j = 0; j < S::kCols; j += 4) {
+                            const float2 x = both_of(sum[j / 2]), y = both_of(sum[j / 2 + 1]);
+                            *reinterpret_cast<float4*>(static_cast<float*>(a.c) + at + j) = make_float4(x.x, x.y, y.x, y.y);
+                        }
                     } else {
 #pragma unroll
                         for (int j = 0; j < S::kCols; j += 8)
                             *reinterpret_cast<uint4*>(static_cast<__half*>(a.c) + at + j) =
-                                make_uint4(pack_two(a.c_dtype, sum[j], sum[j + 1]), pack_two(a.c_dtype, sum[j + 2], sum[j + 3]),
-                                           pack_two(a.c_dtype, sum[j + 4], sum[j + 5]), pack_two(a.c_dtype, sum[j + 6], sum[j + 7]));
+                                make_uint4(pack_two(a.c_dtype, both_of(sum[j / 2])), pack_two(a.c_dtype, both_of(sum[j / 2 + 1])),
+                                           pack_two(a.c_dtype, both_of(sum[j / 2 + 2])), pack_two(a.c_dtype, both_of(sum[j / 2 + 3])));
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < S::kCols; ++j)
-                        if (q0 + j < a.q) store_one(a.c, at + (uint64_t)j * a.ldq, a.c_dtype, sum[j]);
+                    for (int j = 0; j < S::kCols; ++j, at += ldq)
+                        if (q0 + j < a.q) store_one(a.c, at, a.c_dtype, j & 1 ? both_of(sum[j / 2]).y : both_of(sum[j / 2]).x);
                 }
             }
         }
+    } else {
+    if constexpr (S::kUneven) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == S::kEpilogueWarps) {            // loads
+        if (elect_one()) {
+            uint32_t i = 0;                     // blocks of k so far
+            bool ok = true;
+            const uint32_t full0 = smem_u32(&full[0]), empty0 = smem_u32(&empty[0]), ring = smem_u32(base);
+            uint32_t tile = first, kb = kb0, z, p0, q0;
+            if (tile < a.tiles) a.place<BN>(tile, z, p0, q0);
+            for (uint32_t round = 0; ok && tile < a.tiles; ++round) {
+#pragma unroll 1
+                for (int s = 0; s < S::kStages; ++s) {
+                    if (tile >= a.tiles) break;
+                    if (round && !wait(empty0 + 8 * s, (round - 1) & 1, failed)) { ok = false; break; }
+                    const uint32_t bar = full0 + 8 * s, dst = ring + s * S::kStageBytes;
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "n"(S::kStageBytes) : "memory");
+                    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                                 :: "r"(dst), "l"(&map_p), "r"((int)(kb * kBlockK)), "r"(p0), "r"(a.batched_p ? z : 0), "r"(bar) : "memory");
+                    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                                 :: "r"(dst + kRowsTile * kBlockK), "l"(&map_q), "r"((int)(kb * kBlockK)), "r"(q0), "r"(a.batched_q ? z : 0), "r"(bar) : "memory");
+                    ++i;
+                    if (++kb == kb1) {
+                        kb = kb0;
+                        tile += step;
+                        if (tile < a.tiles) a.place<BN>(tile, z, p0, q0);
+                    }
+                }
+            }
+            if (!ok) {                          // nothing of this block's is on its way when it ends
+                for (uint32_t j = i > (uint32_t)S::kStages ? i - S::kStages : 0; j < i; ++j)
+                    for (uint32_t n = 0; n < kWaitLimit && !try_wait(smem_u32(&full[j % S::kStages]), (j / S::kStages) & 1); ++n) {}
+            }
+        }
+        __syncwarp();
+    } else if (warp == S::kEpilogueWarps + 1) { // products
+        if (elect_one()) {
+            bool ok = true;
+            const uint32_t full0 = smem_u32(&full[0]), empty0 = smem_u32(&empty[0]), acc_full0 = smem_u32(&acc_full[0]),
+                           acc_empty0 = smem_u32(&acc_empty[0]);
+            const uint64_t ring = tile_desc(smem_u32(base));
+            uint32_t left = first < a.tiles ? ((a.tiles - 1 - first) / step + 1) * (kb1 - kb0) : 0;     // blocks of k to come
+            uint32_t acc = 0, acc_round = 0;
+            for (uint32_t round = 0; ok && left; ++round) {
+#pragma unroll 1
+                for (int s = 0; s < S::kStages; ++s) {
+                    if (!left) break;
+                    --left;
+                    // the operands first: they are there early, and the accumulator is what a product waits for
+                    if (!wait(full0 + 8 * s, round & 1, failed)) { ok = false; break; }
+                    if (acc_round && !wait(acc_empty0 + 8 * acc, (acc_round - 1) & 1, failed)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t dp = ring + (s * S::kStageBytes >> 4), dq = dp + (kRowsTile * kBlockK >> 4);
+#pragma unroll
+                    for (int j = 0; j < kBlockK / 32; ++j)
+                        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                                     " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
+                                     :: "r"(tmem + acc * BN), "l"(dp + 2 * j), "l"(dq + 2 * j), "r"(a.idesc), "r"(j) : "memory");
+                    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(empty0 + 8 * s) : "memory");
+                    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(acc_full0 + 8 * acc) : "memory");
+                    if (++acc == S::kAcc) {
+                        acc = 0;
+                        ++acc_round;
+                    }
+                }
+            }
+            if (!ok) {
+                asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(smem_u32(&drain)) : "memory");
+                for (uint32_t n = 0; n < kWaitLimit && !try_wait(smem_u32(&drain), 0); ++n) {}
+            }
+        }
+        __syncwarp();
+    }
     }
     if (a.split > 1) {
         // loads' and products' warps took no part in the first wait yet
@@ -338,16 +445,34 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");                   // every partial sum has come
         if constexpr (S::kReduceBytes > 0) {
-            const uint32_t mine = BN / a.split, tile = first;
-            const uint32_t z = tile / (a.p_tiles * a.q_tiles), t = tile - z * a.p_tiles * a.q_tiles;
-            const uint32_t p0 = (t % a.p_tiles) * kRowsTile, q0 = (t / a.p_tiles) * BN + rank * mine;
-            for (uint32_t e = threadIdx.x; e < mine * kRowsTile; e += S::kThreads) {
+            const uint32_t log = kLog<BN> - a.split_log, mine = 1u << log;
+            uint32_t z, p0, q0;
+            a.place<BN>(first, z, p0, q0);
+            q0 += rank << log;
+            for (uint32_t e = threadIdx.x; e < mine / 4 * kRowsTile; e += S::kThreads) {
                 // along whichever dimension C is contiguous
-                const uint32_t r = a.ldp == 1 ? e % kRowsTile : e / mine, j = a.ldp == 1 ? e / kRowsTile : e % mine;
-                if (p0 + r >= a.p || q0 + j >= a.q) continue;
-                float sum = 0.0f;
-                for (uint32_t w = 0; w < a.split; ++w) sum += reduce[(w * mine + j) * kRowsTile + r];
-                store_one(a.c, z * a.c_batch + (uint64_t)(p0 + r) * a.ldp + (uint64_t)(q0 + j) * a.ldq, a.c_dtype, sum);
+                const uint32_t r = a.ldp == 1 ? e % kRowsTile : e >> (log - 2), quad = a.ldp == 1 ? e / kRowsTile : e & (mine / 4 - 1);
+                if (p0 + r >= a.p || q0 + 4 * quad >= a.q) continue;
+                float sum[4] = {};
+#pragma unroll
+                for (uint32_t w = 0; w < kMaxSplit; ++w)
+                    if (w < a.split) {
+                        const float4 f = *reinterpret_cast<const float4*>(
+                            reduce + ((w * kRowsTile + r) << log) + ((quad ^ (r & (mine / 4 - 1) & 7)) << 2));
+                        sum[0] += f.x; sum[1] += f.y; sum[2] += f.z; sum[3] += f.w;
+                    }
+                const uint64_t at = z * a.c_batch + (uint64_t)(p0 + r) * a.ldp + (uint64_t)(q0 + 4 * quad) * a.ldq;
+                if (a.wide && q0 + 4 * quad + 4 <= a.q) {
+                    if (a.c_dtype == METAL_LINALG_FLOAT32)
+                        *reinterpret_cast<float4*>(static_cast<float*>(a.c) + at) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+                    else
+                        *reinterpret_cast<uint2*>(static_cast<__half*>(a.c) + at) =
+                            make_uint2(pack_two(a.c_dtype, make_float2(sum[0], sum[1])), pack_two(a.c_dtype, make_float2(sum[2], sum[3])));
+                } else {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j)
+                        if (q0 + 4 * quad + j < a.q) store_one(a.c, at + j * a.ldq, a.c_dtype, sum[j]);
+                }
             }
         }
     }
@@ -424,9 +549,13 @@ void launch_gemm(cudaStream_t stream, int device, const GemmOperand& oa, const G
     const uint64_t tiles = (uint64_t)a.p_tiles * a.q_tiles * batch;
     if (tiles >= 1ull << 28) throw std::invalid_argument("[matmul_fp8] the product is too large");
     a.tiles = (uint32_t)tiles;
-    a.split = 1;                    // shares of k: powers of two, no share without a block, no more blocks than multiprocessors
+    a.split = 1;
+    a.split_log = 0;                // shares of k: powers of two, four columns a share, none without a block of k, no more blocks than multiprocessors
     if (bn <= 128)
-        while (a.split < kMaxSplit && a.tiles * a.split * 2 <= (uint32_t)sms && a.split * 2 <= a.kb) a.split *= 2;
+        while (a.split < kMaxSplit && a.split * 8 <= bn && a.tiles * a.split * 2 <= (uint32_t)sms && a.split * 2 <= a.kb) {
+            a.split *= 2;
+            ++a.split_log;
+        }
     a.sp = p.scales; a.sq = q.scales;
     a.p_shift = p.block_rows == 128 ? 7 : 0;
     a.q_shift = q.block_rows == 128 ? 7 : 0;
