@@ -30,11 +30,11 @@ namespace delta {
 
 constexpr int kChunk = 64;
 constexpr int kTriTiles = 36;                            // 8 x 8 tiles of a lower triangle of 64
-constexpr int kTriFloats = kTriTiles * 32 * 4;           // a tile: 32 lanes x (hi, hi, lo, lo)
+constexpr int kTriFloats = kTriTiles * 32 * 2;           // a tile: 32 lanes x 2 values of a fragment
 
 // exp of a gate's running sums, a chunk and head.
 struct Gates {
-    double sum[kChunk];          // G
+    float  sum[kChunk], rest[kChunk];   // G, in two parts: a float32 and what it leaves of the 64-bit sum
     float  e[kChunk];            // e^G
     float  left[kChunk];         // e^{G_63 - G}
     float  beta[kChunk];

@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kDoThreads) delta_do_kernel(const Args p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int j = 16 * warp + g + 8 * (i >> 1), r = 8 * n + 2 * t + (i & 1);
-            pt[n][i] = r >= j ? p.scale * pt[n][i] * exp_of(sh.gates.sum[r] - sh.gates.sum[j]) : 0.0f;
+            pt[n][i] = r >= j ? p.scale * pt[n][i] * decay_of(sh.gates, r, j) : 0.0f;
         }
     for (int dv0 = 0; dv0 < (int)p.dvp; dv0 += 64) {
         __syncthreads();
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
         }
         // dR^T = dD^T T: tokens from the column's own on
         float d[kOwn][4] = {};
-        const uint4* tri = reinterpret_cast<const uint4*>(st.tri) + lane;
+        const float2* tri = reinterpret_cast<const float2*>(st.tri) + lane;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             TileTf32 a;
@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) 
                 const int r = m0 + g + 8 * (i >> 1), j = j0 + 8 * n + 2 * t + (i & 1);
                 float m = 0.0f, w = 0.0f;
                 if (j <= r) {
-                    const float dec = exp_of(sh.gates.sum[r] - sh.gates.sum[j]);
+                    const float dec = decay_of(sh.gates, r, j);
                     m = p.scale * dec * mo[n][i];
                     w = m * qk[n][i];
                     if (j < r) {

@@ -71,19 +71,21 @@ __global__ void __launch_bounds__(kIndexThreads) delta_index_kernel(const Args a
 // T = (I + A)^-1 and the decays
 // ---------------------------------------------------------------------------
 //
-// A block takes a chunk and a q/k head: K K^T once, then for every value head that reads it A, its inverse by blocks of
-// 16 (diagonal blocks by substitution, a column a lane; T_ij = -T_ii sum_m A_im T_mj outward from the diagonal on the
-// tensor cores, whose transposed inner product is the outer one's operand as it stands) and T as fragments for the
-// products that follow.
+// A block takes a chunk and a value head: K K^T (again for every value head that reads the same keys: a tenth of the
+// block's time, against twice the blocks), A from it in place, its inverse by blocks of 16 (diagonal blocks by substitution, a
+// column a lane; T_ij = -T_ii sum_m A_im T_mj outward from the diagonal on the tensor cores, whose transposed inner product is the
+// outer one's operand as it stands) and T as fragments for the products that follow. What bounds it is latency, so T takes the place of K
+// in shared memory and five blocks or more fit a multiprocessor.
 constexpr int kPrepThreads = 128;
 constexpr int kLdA = 72;            // row length of A and T in shared memory: 64-bit reads of a fragment meet no bank twice
 
 template <typename T, int DKP>
 struct PrepShared {
-    T      k[kChunk * (DKP + 8)];
-    float  kk[kChunk * kLdA];
+    union {
+        T      k[kChunk * (DKP + 8)];
+        float  t[kChunk * kLdA];
+    };
     float  a[kChunk * kLdA];
-    float  t[kChunk * kLdA];
     Gates  gates;
 };
 
@@ -92,12 +94,40 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const Args p, 
     extern __shared__ __align__(16) char raw[];
     PrepShared<T, DKP>& sh = *reinterpret_cast<PrepShared<T, DKP>*>(raw);
     constexpr int LD = DKP + 8;
-    const uint32_t c = blockIdx.x, h = blockIdx.y;
+    const uint32_t c = blockIdx.x, hv = blockIdx.y, h = hv / (p.value_heads / p.heads);
+    const size_t at = (size_t)c * p.value_heads + hv;
     const Chunk ch = chunk_at(p, c);
     if (ch.rows == 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     load_rows<T, kPrepThreads, DKP>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, threadIdx.x);
     cp_commit();
+    if (warp == 0) {            // the gates' sums, two tokens a lane
+        double x[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int r = 2 * lane + j;
+            const float gate = r < ch.rows ? p.g[at3(p.g_stride, ch.batch, ch.token + r, hv)] : 0.0f;
+            // e^-256 is zero in float32 with room to spare: a gate that closes for good, or -inf, adds no more than that,
+            // so that the sums behind it keep their last bits
+            x[j] = gate < -256.0f ? -256.0 : (double)gate;
+            sh.gates.beta[r] = r < ch.rows ? p.beta[at3(p.beta_stride, ch.batch, ch.token + r, hv)] : 0.0f;
+        }
+        double sum = x[0] + x[1];
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const double v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        const double end = __shfl_sync(0xffffffffu, sum, 31);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const double s = j ? sum : sum - x[1];
+            sh.gates.sum[2 * lane + j] = (float)s;
+            sh.gates.rest[2 * lane + j] = (float)(s - (double)(float)s);
+            sh.gates.e[2 * lane + j] = exp_of(s);
+            sh.gates.left[2 * lane + j] = exp_of(end - s);
+        }
+    }
     cp_wait<0>();
     __syncthreads();
     {       // K K^T: warp w the rows 16 w .. 16 w + 15, columns up to the diagonal's
@@ -109,117 +139,86 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const Args p, 
         }
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
-            *reinterpret_cast<float2*>(&sh.kk[(16 * warp + g) * kLdA + 8 * n + 2 * t]) = make_float2(acc[n][0], acc[n][1]);
-            *reinterpret_cast<float2*>(&sh.kk[(16 * warp + 8 + g) * kLdA + 8 * n + 2 * t]) = make_float2(acc[n][2], acc[n][3]);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = 16 * warp + 8 * half + g, q = 8 * n + 2 * t;
+                const float beta = sh.gates.beta[r];
+                *reinterpret_cast<float2*>(&sh.a[r * kLdA + q]) =
+                    make_float2(q < r ? beta * decay_of(sh.gates, r, q) * acc[n][2 * half] : 0.0f,
+                                q + 1 < r ? beta * decay_of(sh.gates, r, q + 1) * acc[n][2 * half + 1] : 0.0f);
+            }
         }
     }
-    const uint32_t up = p.value_heads / p.heads;
-    for (uint32_t i = 0; i < up; ++i) {
-        const uint32_t hv = h * up + i;
-        const size_t at = (size_t)c * p.value_heads + hv;
-        if (warp == 0) {            // the gates' sums, two tokens a lane
-            double x[2];
+    __syncthreads();
+    {
+        const float* src = reinterpret_cast<const float*>(&sh.gates);
+        float* dst = reinterpret_cast<float*>(p.gates + at);
+        for (int j = threadIdx.x; j < (int)(sizeof(Gates) / 4); j += kPrepThreads) dst[j] = src[j];
+    }
+    for (int j = threadIdx.x; j < kChunk * kChunk; j += kPrepThreads) sh.t[(j >> 6) * kLdA + (j & 63)] = 0.0f;
+    __syncthreads();
+    if (lane < 16) {            // diagonal blocks: column `lane` of block `warp`
+        const float* a = sh.a + (16 * warp) * kLdA + 16 * warp;
+        float x[16];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int r = 2 * lane + j;
-                const float gate = r < ch.rows ? p.g[at3(p.g_stride, ch.batch, ch.token + r, hv)] : 0.0f;
-                // e^-256 is zero in float32 with room to spare: a gate that closes for good, or -inf, adds no more than that,
-                // so that the sums behind it keep their last bits
-                x[j] = gate < -256.0f ? -256.0 : (double)gate;
-                sh.gates.beta[r] = r < ch.rows ? p.beta[at3(p.beta_stride, ch.batch, ch.token + r, hv)] : 0.0f;
-            }
-            double sum = x[0] + x[1];
+        for (int r = 0; r < 16; ++r) {
+            float v = r == lane ? 1.0f : 0.0f;
 #pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const double v = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += v;
-            }
-            const double end = __shfl_sync(0xffffffffu, sum, 31);
-            sh.gates.sum[2 * lane] = sum - x[1];
-            sh.gates.sum[2 * lane + 1] = sum;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const double s = j ? sum : sum - x[1];
-                sh.gates.e[2 * lane + j] = exp_of(s);
-                sh.gates.left[2 * lane + j] = exp_of(end - s);
-            }
+            for (int m = 0; m < r; ++m) v = fmaf(-a[r * kLdA + m], x[m], v);
+            x[r] = v;
         }
-        __syncthreads();
-        {
-            const float* src = reinterpret_cast<const float*>(&sh.gates);
-            float* dst = reinterpret_cast<float*>(p.gates + at);
-            for (int j = threadIdx.x; j < (int)(sizeof(Gates) / 4); j += kPrepThreads) dst[j] = src[j];
-        }
-        for (int j = threadIdx.x; j < kChunk * kChunk; j += kPrepThreads) {
-            const int r = j >> 6, q = j & 63;
-            sh.a[r * kLdA + q] = q < r ? sh.gates.beta[r] * exp_of(sh.gates.sum[r] - sh.gates.sum[q]) * sh.kk[r * kLdA + q] : 0.0f;
-            sh.t[r * kLdA + q] = 0.0f;
-        }
-        __syncthreads();
-        if (lane < 16) {            // diagonal blocks: column `lane` of block `warp`
-            const float* a = sh.a + (16 * warp) * kLdA + 16 * warp;
-            float x[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float v = r == lane ? 1.0f : 0.0f;
-#pragma unroll
-                for (int m = 0; m < r; ++m) v = fmaf(-a[r * kLdA + m], x[m], v);
-                x[r] = v;
+        for (int r = 0; r < 16; ++r) sh.t[(16 * warp + r) * kLdA + 16 * warp + lane] = x[r];
+    }
+    __syncthreads();
+    for (int dist = 1; dist < 4; ++dist) {
+        if (warp < 4 - dist) {
+            const int bj = warp, bi = warp + dist;
+            float w[2][4] = {};                                     // W^T, W = sum_m A_im T_mj: rows are T's columns
+            for (int m = bj; m < bi; ++m) {
+                const float* tm = sh.t + (16 * m) * kLdA + 16 * bj;     // T_mj
+                const float* am = sh.a + (16 * bi) * kLdA + 16 * m;     // A_im
+                const float x[4] = {tm[2 * t * kLdA + g], tm[(2 * t + 1) * kLdA + g], tm[2 * t * kLdA + g + 8], tm[(2 * t + 1) * kLdA + g + 8]};
+                const float y[4] = {tm[(2 * t + 8) * kLdA + g], tm[(2 * t + 9) * kLdA + g], tm[(2 * t + 8) * kLdA + g + 8],
+                                    tm[(2 * t + 9) * kLdA + g + 8]};
+                SplitTf32 s;
+                s.set(x, y);
+                mma_tile<float, 2, false>(w, s, am, kLdA, 0, 0);
             }
+            float out[2][4] = {};
+            const float* ti = sh.t + (16 * bi) * kLdA + 16 * bi;        // T_ii
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sh.t[(16 * warp + r) * kLdA + 16 * warp + lane] = x[r];
-        }
-        __syncthreads();
-        for (int dist = 1; dist < 4; ++dist) {
-            if (warp < 4 - dist) {
-                const int bj = warp, bi = warp + dist;
-                float w[2][4] = {};                                     // W^T, W = sum_m A_im T_mj: rows are T's columns
-                for (int m = bj; m < bi; ++m) {
-                    const float* tm = sh.t + (16 * m) * kLdA + 16 * bj;     // T_mj
-                    const float* am = sh.a + (16 * bi) * kLdA + 16 * m;     // A_im
-                    const float x[4] = {tm[2 * t * kLdA + g], tm[(2 * t + 1) * kLdA + g], tm[2 * t * kLdA + g + 8], tm[(2 * t + 1) * kLdA + g + 8]};
-                    const float y[4] = {tm[(2 * t + 8) * kLdA + g], tm[(2 * t + 9) * kLdA + g], tm[(2 * t + 8) * kLdA + g + 8],
-                                        tm[(2 * t + 9) * kLdA + g + 8]};
-                    SplitTf32 s;
-                    s.set(x, y);
-                    mma_tile<float, 2, false>(w, s, am, kLdA, 0, 0);
-                }
-                float out[2][4] = {};
-                const float* ti = sh.t + (16 * bi) * kLdA + 16 * bi;        // T_ii
-#pragma unroll
-                for (int k8 = 0; k8 < 2; ++k8) {
-                    const float2 u = *reinterpret_cast<const float2*>(ti + g * kLdA + 8 * k8 + 2 * t);
-                    const float2 v = *reinterpret_cast<const float2*>(ti + (g + 8) * kLdA + 8 * k8 + 2 * t);
-                    const float x[4] = {-u.x, -u.y, -v.x, -v.y};
-                    TileTf32 s;
-                    s.set(x);
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        const uint4 b = split_pair(w[k8][2 * n], w[k8][2 * n + 1]);
-#pragma unroll
-                        for (int term = 0; term < 3; ++term) mma_term8(out[n], s, b, term);
-                    }
-                }
+            for (int k8 = 0; k8 < 2; ++k8) {
+                const float2 u = *reinterpret_cast<const float2*>(ti + g * kLdA + 8 * k8 + 2 * t);
+                const float2 v = *reinterpret_cast<const float2*>(ti + (g + 8) * kLdA + 8 * k8 + 2 * t);
+                const float x[4] = {-u.x, -u.y, -v.x, -v.y};
+                TileTf32 s;
+                s.set(x);
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    float* o = sh.t + (16 * bi + g) * kLdA + 16 * bj + 8 * n + 2 * t;
-                    *reinterpret_cast<float2*>(o) = make_float2(out[n][0], out[n][1]);
-                    *reinterpret_cast<float2*>(o + 8 * kLdA) = make_float2(out[n][2], out[n][3]);
+                    const uint4 b = split_pair(w[k8][2 * n], w[k8][2 * n + 1]);
+#pragma unroll
+                    for (int term = 0; term < 3; ++term) mma_term8(out[n], s, b, term);
                 }
             }
-            __syncthreads();
-        }
-        for (int tile = warp; tile < kTriTiles; tile += kPrepThreads / 32) {
-            int ti = 0;
-            while (tri_tile(ti + 1, 0) <= tile) ++ti;
-            const int tj = tile - tri_tile(ti, 0);
-            const float2 f = *reinterpret_cast<const float2*>(sh.t + (8 * ti + g) * kLdA + 8 * tj + 2 * t);
-            reinterpret_cast<uint4*>(p.tri + at * kTriFloats)[tile * 32 + lane] = split_pair(f.x, f.y);
-            if (backward)
-                reinterpret_cast<uint4*>(p.tri_b + at * kTriFloats)[tile * 32 + lane] =
-                    split_pair(sh.t[(8 * ti + 2 * t) * kLdA + 8 * tj + g], sh.t[(8 * ti + 2 * t + 1) * kLdA + 8 * tj + g]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                float* o = sh.t + (16 * bi + g) * kLdA + 16 * bj + 8 * n + 2 * t;
+                *reinterpret_cast<float2*>(o) = make_float2(out[n][0], out[n][1]);
+                *reinterpret_cast<float2*>(o + 8 * kLdA) = make_float2(out[n][2], out[n][3]);
+            }
         }
         __syncthreads();
+    }
+    for (int tile = warp; tile < kTriTiles; tile += kPrepThreads / 32) {
+        int ti = 0;
+        while (tri_tile(ti + 1, 0) <= tile) ++ti;
+        const int tj = tile - tri_tile(ti, 0);
+        const float2 f = *reinterpret_cast<const float2*>(sh.t + (8 * ti + g) * kLdA + 8 * tj + 2 * t);
+        reinterpret_cast<float2*>(p.tri + at * kTriFloats)[tile * 32 + lane] = f;
+        if (backward)
+            reinterpret_cast<float2*>(p.tri_b + at * kTriFloats)[tile * 32 + lane] =
+                make_float2(sh.t[(8 * ti + 2 * t) * kLdA + 8 * tj + g], sh.t[(8 * ti + 2 * t + 1) * kLdA + 8 * tj + g]);
     }
 }
 
@@ -370,7 +369,7 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
         if constexpr (KS > 1) asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
         // D^T = R^T T^T, a k of 8 at a time against the rows of T that reach it
         float d[kOwn][4] = {};
-        const uint4* tri = reinterpret_cast<const uint4*>(st.tri) + lane;
+        const float2* tri = reinterpret_cast<const float2*>(st.tri) + lane;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             TileTf32 a;
@@ -433,24 +432,29 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
 //
 // A block takes a chunk and a value head; a warp 16 value columns of all 64 tokens: O^T = S^T (e^G Q)^T + D^T P^T, with S and D
 // read from memory as A operands (each value once, split once), Q from shared memory, and P (20 tiles of 16 x 8 over the
-// warps) kept there as the B fragments that its accumulators are.
+// warps) kept there as the B fragments that its accumulators are. What bounds it is memory's latency and the tensor core
+// about equally: half of a warp's S is on its way while P is made, each further part while the one before it is multiplied.
 constexpr int kOutThreads = 256;
+constexpr int kOutCols = 16 * (kOutThreads / 32);       // value columns at a time
 
 template <typename T, int DKP>
 struct OutShared {
-    alignas(16) T     q[kChunk * (DKP + 8)];
-    alignas(16) T     k[kChunk * (DKP + 8)];
-    alignas(16) uint4 p[kTriTiles * 32];
-    alignas(16) Gates gates;
+    alignas(16) T q[kChunk * (DKP + 8)];
+    union {
+        alignas(16) T k[kChunk * (DKP + 8)];
+        T o[kChunk * (kOutCols + 8)];                   // the outputs on their way to memory, whole rows at a time
+    };
+    alignas(16) float2 p[kTriTiles * 32];
+    alignas(16) Gates  gates;
 };
 
 template <typename T, int DKP>
-__global__ void __launch_bounds__(kOutThreads) delta_output_kernel(const Args p) {
+__global__ void __launch_bounds__(kOutThreads, 2) delta_output_kernel(const Args p) {
     extern __shared__ __align__(16) char raw[];
     using Sh = OutShared<T, DKP>;
     using Sp = typename Split<T>::type;
     Sh& sh = *reinterpret_cast<Sh*>(raw);
-    constexpr int LD = DKP + 8;
+    constexpr int LD = DKP + 8, kHeld = DKP / 32, LDO = kOutCols + 8;
     const uint32_t c = blockIdx.x, hv = blockIdx.y, h = hv / (p.value_heads / p.heads);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     T* o = static_cast<T*>(p.o);
@@ -470,6 +474,31 @@ __global__ void __launch_bounds__(kOutThreads) delta_output_kernel(const Args p)
     load_rows<T, kOutThreads, DKP>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, threadIdx.x);
     load_floats<kOutThreads, sizeof(Gates) / 4>(reinterpret_cast<float*>(&sh.gates), reinterpret_cast<const float*>(p.gates + at), threadIdx.x);
     cp_commit();
+    // a k of 16 of S^T or D^T as two accumulator tiles: rows 2t, 2t + 1, 2t + 8, 2t + 9 of columns g, g + 8
+    float held[kHeld][8];
+    const auto fetch = [&](const float* base, int row, float (&to)[8]) {
+        const float* src = base + (size_t)(row + 2 * t) * p.dvp + g;
+        to[0] = src[0];
+        to[2] = src[8];
+        to[1] = src[p.dvp];
+        to[3] = src[p.dvp + 8];
+        src += 8 * p.dvp;
+        to[4] = src[0];
+        to[6] = src[8];
+        to[5] = src[p.dvp];
+        to[7] = src[p.dvp + 8];
+    };
+    const auto tiles = [](const float (&from)[8], float (&x)[4], float (&y)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = from[i];
+            y[i] = from[4 + i];
+        }
+    };
+    const float *s = p.states + at * p.dkp * p.dvp, *d = p.d + at * kChunk * p.dvp;
+    if (16 * warp < (int)p.dvp)
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) fetch(s + 16 * warp, 16 * i, held[i]);
     cp_wait<0>();
     __syncthreads();
     // P's tiles of 16 x 8 on and below the diagonal, two neighbours at a time: (0, 0), (1, 0), (1, 1), (2, 0) ...
@@ -486,53 +515,72 @@ __global__ void __launch_bounds__(kOutThreads) delta_output_kernel(const Args p)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = 16 * a + g + 8 * (i >> 1), q = 16 * j16 + 8 * n + 2 * t + (i & 1);
-                f[i] = q <= r ? acc[n][i] * exp_of(sh.gates.sum[r] - sh.gates.sum[q]) : 0.0f;
+                f[i] = q <= r ? acc[n][i] * decay_of(sh.gates, r, q) : 0.0f;
             }
             const int j8 = 2 * j16 + n;
-            if (j8 <= 2 * a) sh.p[tri_tile(2 * a, j8) * 32 + lane] = split_pair(f[0], f[1]);
-            sh.p[tri_tile(2 * a + 1, j8) * 32 + lane] = split_pair(f[2], f[3]);
+            if (j8 <= 2 * a) sh.p[tri_tile(2 * a, j8) * 32 + lane] = make_float2(f[0], f[1]);
+            sh.p[tri_tile(2 * a + 1, j8) * 32 + lane] = make_float2(f[2], f[3]);
         }
     }
     __syncthreads();
-    for (int dv0 = 16 * warp; dv0 < (int)p.dvp; dv0 += 16 * (kOutThreads / 32)) {
-        float acc[8][4] = {};
-        const float* s = p.states + at * p.dkp * p.dvp + dv0 + g;
-#pragma unroll 2
-        for (int k0 = 0; k0 < DKP; k0 += 16) {
-            float x[4], y[4];
+    for (int pass = 0; pass < (int)p.dvp; pass += kOutCols) {
+        const int dv0 = pass + 16 * warp;
+        if (dv0 < (int)p.dvp) {
+            const float *sv = s + dv0, *dv = d + dv0;
+            if (pass)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] = s[(size_t)(k0 + 2 * t + (i & 1)) * p.dvp + 8 * (i >> 1)];
-                y[i] = s[(size_t)(k0 + 8 + 2 * t + (i & 1)) * p.dvp + 8 * (i >> 1)];
+                for (int i = 0; i < kHeld; ++i) fetch(sv, 16 * i, held[i]);
+            float acc[8][4] = {};
+#pragma unroll
+            for (int kk = 0; kk < 2 * kHeld; ++kk) {
+                float x[4], y[4];
+                tiles(held[kk % kHeld], x, y);
+                if (kk < kHeld) fetch(sv, 16 * (kHeld + kk), held[kk]);
+                else            fetch(dv, 16 * (kk - kHeld), held[kk - kHeld]);
+                Sp a;
+                a.set(x, y);
+                mma_tile<T, 8, false>(acc, a, sh.q, LD, 0, 16 * kk);
             }
-            Sp a;
-            a.set(x, y);
-            mma_tile<T, 8, false>(acc, a, sh.q, LD, 0, k0);
-        }
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[n][i] *= sh.gates.e[8 * n + 2 * t + (i & 1)];
-        const float* d = p.d + at * kChunk * p.dvp + dv0 + g;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = d[(size_t)(8 * j + 2 * t + (i & 1)) * p.dvp + 8 * (i >> 1)];
-            TileTf32 a;
-            a.set(x);
-            mma_triangle(acc, a, [&](int n) { return n >= j; }, [&](int n) { return sh.p[tri_tile(n, j) * 32 + lane]; });
-        }
-        // a lane's eight neighbours g write 8 values that lie next to one another: 16 or 32 bytes of every token's row
-#pragma unroll
-        for (int n = 0; n < 8; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int tok = 8 * n + 2 * t + (i & 1), column = dv0 + g + 8 * (i >> 1);
-                if (tok < ch.rows && column < (int)p.dv)
-                    o[(((size_t)ch.batch * p.tokens + ch.token + tok) * p.value_heads + hv) * p.dv + column] =
-                        from_f<T>(p.scale * acc[n][i]);
+            for (int n = 0; n < 8; ++n) {
+                const float2 e = *reinterpret_cast<const float2*>(sh.gates.e + 8 * n + 2 * t);
+                acc[n][0] *= e.x; acc[n][1] *= e.y; acc[n][2] *= e.x; acc[n][3] *= e.y;
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float x[2][4];
+                tiles(held[j % kHeld], x[0], x[1]);
+                if (j + kHeld < 4) fetch(dv, 16 * (j + kHeld), held[j % kHeld]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    TileTf32 a;
+                    a.set(x[i]);
+                    mma_triangle(acc, a, [&](int n) { return n >= 2 * j + i; }, [&](int n) { return sh.p[tri_tile(n, 2 * j + i) * 32 + lane]; });
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    sh.o[(8 * n + 2 * t + (i & 1)) * LDO + 16 * warp + g + 8 * (i >> 1)] = from_f<T>(p.scale * acc[n][i]);
+        }
+        __syncthreads();
+        const int width = min(kOutCols, (int)p.dv - pass);
+        T* to = o + (((size_t)ch.batch * p.tokens + ch.token) * p.value_heads + hv) * p.dv + pass;
+        const size_t step = (size_t)p.value_heads * p.dv;
+        constexpr int kPer = 16 / sizeof(T), kPieces = kOutCols / kPer;
+        if (p.dv % kPer == 0 && (reinterpret_cast<size_t>(o) & 15) == 0) {
+            for (int i = threadIdx.x; i < ch.rows * kPieces; i += kOutThreads) {
+                const int r = i / kPieces, q = (i % kPieces) * kPer;
+                if (q < width) *reinterpret_cast<uint4*>(to + r * step + q) = *reinterpret_cast<const uint4*>(sh.o + r * LDO + q);
+            }
+        } else {
+            for (int i = threadIdx.x; i < ch.rows * kOutCols; i += kOutThreads) {
+                const int r = i / kOutCols, q = i % kOutCols;
+                if (q < width) to[r * step + q] = sh.o[r * LDO + q];
+            }
+        }
+        if (pass + kOutCols < (int)p.dvp) __syncthreads();
     }
 }
 
@@ -544,7 +592,7 @@ template <typename T, int DKP>
 void prepare_as(const Args& a, cudaStream_t stream, bool backward) {
     const size_t bytes = sizeof(PrepShared<T, DKP>);
     opt_in(delta_prep_kernel<T, DKP>, bytes);
-    delta_prep_kernel<T, DKP><<<dim3(a.chunks, a.heads), kPrepThreads, bytes, stream>>>(a, backward);
+    delta_prep_kernel<T, DKP><<<dim3(a.chunks, a.value_heads), kPrepThreads, bytes, stream>>>(a, backward);
     cuda_check(cudaGetLastError(), "delta rule preparation");
 }
 

@@ -318,7 +318,8 @@ __device__ __forceinline__ uint4 split_pair(float x, float y) {
     split_tf32(y, r.y, r.w);
     return r;
 }
-// acc[i] += a k of 8 of a float32 operand times fragment(i) for every i that wanted(i) names, as mma_tile.
+// acc[i] += a k of 8 of a float32 operand times fragment(i), a lane's k 2t and k 2t + 1, for every i that wanted(i) names, as
+// mma_tile.
 template <int N, typename Wanted, typename Fragment>
 __device__ __forceinline__ void mma_triangle(float (&acc)[N][4], const TileTf32& a, Wanted wanted, Fragment fragment) {
     constexpr int kGroup = N < 4 ? N : 4;
@@ -328,7 +329,10 @@ __device__ __forceinline__ void mma_triangle(float (&acc)[N][4], const TileTf32&
         uint4 b[kGroup];
 #pragma unroll
         for (int n = 0; n < kGroup; ++n)
-            if (wanted(n0 + n)) b[n] = fragment(n0 + n);
+            if (wanted(n0 + n)) {
+                const float2 f = fragment(n0 + n);
+                b[n] = split_pair(f.x, f.y);
+            }
 #pragma unroll
         for (int term = 0; term < 3; ++term)
 #pragma unroll
@@ -413,15 +417,16 @@ __device__ __forceinline__ long long at3(const long long (&stride)[3], long long
     return b * stride[0] + t * stride[1] + h * stride[2];
 }
 
-// exp(x) for x <= 0 given in 64 bits (and a little above), rounded once from about 2^-30: the float exp of the leading part
-// times 1 + the rest.
-__device__ __forceinline__ float exp_of(double x) {
-    const float h = (float)x;
+// exp of x = h + l, l the small rest: the float exp of h times 1 + l.
+__device__ __forceinline__ float exp_of(float h, float l) {
     if (!(h > -104.0f)) return h != h ? h : 0.0f;      // below the smallest float32
     if (h > 88.8f) return __int_as_float(0x7F800000);
     const float e = expf(h);
-    return fmaf(e, (float)(x - (double)h), e);
+    return fmaf(e, l, e);
 }
+__device__ __forceinline__ float exp_of(double x) { return exp_of((float)x, (float)(x - (double)(float)x)); }
+// e^{G_i - G_j}. The difference of the leading parts is rounded once, 2^-24 of it: e^-x x 2^-24 is at most 2^-25 of e^0.
+__device__ __forceinline__ float decay_of(const Gates& g, int i, int j) { return exp_of(g.sum[i] - g.sum[j], g.rest[i] - g.rest[j]); }
 
 // Of a chain's 8 token tiles, the i-th that warp `part` of its KS computes: 0 and 7 together, 1 and 6 ..., so that the
 // triangle's work is even.
