@@ -16,7 +16,6 @@
 #include "delta.h"
 #include "delta_tiles.cuh"
 #include "runtime.h"
-#include <cstdlib>
 
 namespace mlb {
 namespace delta {
@@ -340,9 +339,11 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
 // dQ, dK, dV, dbeta, dg of a chunk
 // ---------------------------------------------------------------------------
 //
-// Eight warps: 16 tokens (warp % 4) x half of the key columns (warp / 4) of dO S^T, dR S^T and D dS'^T, and as much of
-// dO D^T and dR D^T, summed over slices of 16 value columns that are fetched one ahead; then M, N and K K^T, Q K^T.
-constexpr int kGradThreads = 256;
+// Sixteen warps: 16 tokens (warp % 4) x a quarter of the key columns (warp / 4) of dO S^T, dR S^T and D dS'^T, and as much of
+// dO D^T and dR D^T, summed over slices of 16 value columns that are fetched one ahead; then M, N and K K^T, Q K^T. One block
+// fills a multiprocessor. (Eight warps of twice the columns split fewer operands, but leave the tensor core waiting for
+// them: 39 % of its cycles used.)
+constexpr int kGradThreads = 512;
 constexpr int kLdS = 24;            // row length of a slice: 64-bit fragment reads meet no bank twice
 constexpr int kLdM = 72;
 
@@ -361,8 +362,8 @@ struct GradShared {
     alignas(16) float m[kChunk * kLdM];
     alignas(16) float n[kChunk * kLdM];        // N + N^T
     alignas(16) Gates gates;
-    float row_w[2][kChunk], row_u[2][kChunk], col_w[4][kChunk];
-    float qx[2][kChunk], kx2[2][kChunk], kx3[2][kChunk];
+    float row_w[4][kChunk], row_u[4][kChunk], col_w[4][kChunk];
+    float qx[4][kChunk], kx2[4][kChunk], kx3[4][kChunk];
     float drv[kChunk], pair[kGradThreads / 32];
 };
 
@@ -401,24 +402,17 @@ __device__ __forceinline__ void slice_a(SplitTf32& a, const T* tile, int m0) {
         a.set(x, y);
     }
 }
-// c += A B^T of a slice: kExact: A has one part.
-template <bool kExact>
-__device__ __forceinline__ void mma_slice(float (&c)[4], const SplitTf32& a, const FragB<float>& b, int term) {
-    if (kExact && term == 0) return;
-    mma_term(c, a, b, term);
-}
-
 template <typename T, int DKP>
 __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) {
     extern __shared__ __align__(16) char raw[];
     using Sh = GradShared<T, DKP>;
     using Sp = typename Split<T>::type;
     Sh& sh = *reinterpret_cast<Sh*>(raw);
-    constexpr int LD = DKP + 8, NT = DKP / 16;
+    constexpr int LD = DKP + 8, NT = DKP / 32;
     constexpr bool kExact = Is16<T>::value;
     const uint32_t c = blockIdx.x, hv = blockIdx.y, up = p.value_heads / p.heads, h = hv / up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int m0 = 16 * (warp & 3), half = warp >> 2, n0 = half * (DKP / 2), j0 = 32 * half;
+    const int m0 = 16 * (warp & 3), part = warp >> 2, n0 = part * (DKP / 4), j0 = 16 * part;
     T *dq = static_cast<T*>(p.dq), *dk = static_cast<T*>(p.dk_out), *dv = static_cast<T*>(p.dv_out);
     const Chunk ch = chunk_at(p, c);
     const auto put_qk = [&](size_t token, int column, float q0, float q1, float k0, float k1) {     // columns `column`, + 1
@@ -467,9 +461,9 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) 
         const float* d = p.d + at * kChunk * p.dvp + dv0;
         const float* dr = p.dr + at * kChunk * p.dvp + dv0;
         {
-            const int r = threadIdx.x >> 2, q = (threadIdx.x & 3) * 4;
-            cp_async16(sl.d + r * kLdS + q, d + (size_t)r * p.dvp + q, true);
-            cp_async16(sl.dr + r * kLdS + q, dr + (size_t)r * p.dvp + q, true);
+            const int r = (threadIdx.x & 255) >> 2, q = (threadIdx.x & 3) * 4;
+            if (threadIdx.x < 256) cp_async16(sl.d + r * kLdS + q, d + (size_t)r * p.dvp + q, true);
+            else                   cp_async16(sl.dr + r * kLdS + q, dr + (size_t)r * p.dvp + q, true);
         }
         load_rows<T, kGradThreads, 16>(sl.d_o, kLdS, p.d_o, at3(p.do_stride, ch.batch, ch.token, hv) + dv0, p.do_stride[1], ch.rows,
                                        (int)p.dv - dv0, p.vec, threadIdx.x);
@@ -482,65 +476,59 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) 
     load_floats<kGradThreads, sizeof(Gates) / 4>(reinterpret_cast<float*>(&sh.gates), reinterpret_cast<const float*>(p.gates + at), threadIdx.x);
     fetch(0, 0);
 
-    float x1[NT][4] = {}, x2[NT][4] = {}, x3[NT][4] = {}, mo[4][4] = {}, mr[4][4] = {};
+    float x1[NT][4] = {}, x2[NT][4] = {}, x3[NT][4] = {}, mo[2][4] = {}, mr[2][4] = {};
     float drv = 0.0f, pair = 0.0f;
     for (int dv0 = 0; dv0 < (int)p.dvp; dv0 += 16) {
         const typename Sh::Slice& sl = sh.slice[(dv0 >> 4) & 1];
         cp_wait<0>();
         __syncthreads();
         if (dv0 + 16 < (int)p.dvp) fetch(dv0 + 16, ((dv0 >> 4) + 1) & 1);
-        SplitTf32 a_do, a_dr, a_d;
-        slice_a<T>(a_do, sl.d_o, m0);
-        slice_a<float>(a_dr, sl.dr, m0);
-        slice_a<float>(a_d, sl.d, m0);
+        {
+            SplitTf32 a_do, a_dr;
+            slice_a<T>(a_do, sl.d_o, m0);
+            slice_a<float>(a_dr, sl.dr, m0);
+            // two tiles of dO and dR against rows of `tile`; every slice from nothing, then added in float32 (see mma_tile)
+            const auto both = [&](const float* tile, int row, float (&u)[4], float (&v)[4], float (&w)[4], float (&x)[4]) {
+                FragB<float> b[2];
+                load_b_rows<float>(b, tile, kLdS, row, 0);
+                float c[4][4];
 #pragma unroll
-        for (int n = 0; n < NT; n += 2) {
-            FragB<float> b[2];
-            load_b_rows<float>(b, sl.s, kLdS, n0 + 8 * n, 0);
-            float c[4][4] = {};             // every slice from nothing, then added in float32 (see mma_tile)
+                for (int j = 0; j < 2; ++j) { mma_term<0, kExact>(c[j], a_do, b[j]); mma_term<0>(c[2 + j], a_dr, b[j]); }
 #pragma unroll
-            for (int term = 0; term < 3; ++term)
+                for (int j = 0; j < 2; ++j) { mma_term<1, kExact>(c[j], a_do, b[j]); mma_term<1>(c[2 + j], a_dr, b[j]); }
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    mma_slice<kExact>(c[j], a_do, b[j], term);
-                    mma_slice<false>(c[2 + j], a_dr, b[j], term);
-                }
-            load_b_rows<float>(b, sl.ds, kLdS, n0 + 8 * n, 0);
-            float e[2][4] = {};
+                for (int j = 0; j < 2; ++j) { mma_term<2, kExact>(c[j], a_do, b[j]); mma_term<2>(c[2 + j], a_dr, b[j]); }
+                add_to(u, c[0]);
+                add_to(v, c[1]);
+                add_to(w, c[2]);
+                add_to(x, c[3]);
+            };
 #pragma unroll
-            for (int term = 0; term < 3; ++term)
+            for (int n = 0; n < NT; n += 2) both(sl.s, n0 + 8 * n, x1[n], x1[n + 1], x2[n], x2[n + 1]);
+            if (j0 <= m0) both(sl.d, j0, mo[0], mo[1], mr[0], mr[1]);      // above the diagonal: nothing
+        }
+        {
+            SplitTf32 a_d;
+            slice_a<float>(a_d, sl.d, m0);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) mma_slice<false>(e[j], a_d, b[j], term);
+            for (int n = 0; n < NT; n += 2) {
+                FragB<float> b[2];
+                load_b_rows<float>(b, sl.ds, kLdS, n0 + 8 * n, 0);
+                float e[2][4];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                add_to(x1[n + j], c[j]);
-                add_to(x2[n + j], c[2 + j]);
-                add_to(x3[n + j], e[j]);
+                for (int j = 0; j < 2; ++j) mma_term<0>(e[j], a_d, b[j]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma_term<1>(e[j], a_d, b[j]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma_term<2>(e[j], a_d, b[j]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) add_to(x3[n + j], e[j]);
             }
         }
+        {           // dV = beta dR, dR . V: a token's two columns a thread
+            const int r = threadIdx.x >> 3, q = (threadIdx.x & 7) * 2;
 #pragma unroll
-        for (int n = 0; n < 4; n += 2) {
-            if (j0 + 8 * n > m0 + 15) continue;             // above the diagonal
-            FragB<float> b[2];
-            load_b_rows<float>(b, sl.d, kLdS, j0 + 8 * n, 0);
-            float c[4][4] = {};
-#pragma unroll
-            for (int term = 0; term < 3; ++term)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    mma_slice<kExact>(c[j], a_do, b[j], term);
-                    mma_slice<false>(c[2 + j], a_dr, b[j], term);
-                }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                add_to(mo[n + j], c[j]);
-                add_to(mr[n + j], c[2 + j]);
-            }
-        }
-        {           // dV = beta dR, dR . V: a token's four columns a thread
-            const int r = threadIdx.x >> 2, q = (threadIdx.x & 3) * 4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 2; ++i) {
                 const float x = sl.dr[r * kLdS + q + i];
                 drv = fmaf(x, to_f(sl.v[r * kLdS + q + i]), drv);
                 if (r < ch.rows && dv0 + q + i < (int)p.dv)
@@ -552,22 +540,24 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) 
     }
     drv += __shfl_xor_sync(0xffffffffu, drv, 1);
     drv += __shfl_xor_sync(0xffffffffu, drv, 2);
-    if ((threadIdx.x & 3) == 0) sh.drv[threadIdx.x >> 2] = drv;
+    drv += __shfl_xor_sync(0xffffffffu, drv, 4);
+    if ((threadIdx.x & 7) == 0) sh.drv[threadIdx.x >> 3] = drv;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) pair += __shfl_xor_sync(0xffffffffu, pair, o);
     if (lane == 0) sh.pair[warp] = pair;
 
     // M, N, and what their products with Q K^T and K K^T give the gates
     {
-        float qk[4][4] = {}, kk[4][4] = {};
+        float qk[2][4] = {}, kk[2][4] = {};
+        if (j0 <= m0)
 #pragma unroll
-        for (int k0 = 0; k0 < DKP; k0 += 16) {
-            mma_rows_rows<T, 4>(qk, sh.q, LD, m0, sh.k, LD, j0, k0);
-            mma_rows_rows<T, 4>(kk, sh.k, LD, m0, sh.k, LD, j0, k0);
-        }
+            for (int k0 = 0; k0 < DKP; k0 += 16) {
+                mma_rows_rows<T, 2>(qk, sh.q, LD, m0, sh.k, LD, j0, k0);
+                mma_rows_rows<T, 2>(kk, sh.k, LD, m0, sh.k, LD, j0, k0);
+            }
         float row_w[2] = {0.0f, 0.0f}, row_u[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < 2; ++n) {
             float col[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -620,11 +610,11 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) 
             }
             if (t == 0) {
                 const int r = m0 + g + 8 * i;
-                sh.row_w[half][r] = row_w[i];
-                sh.row_u[half][r] = row_u[i];
-                sh.qx[half][r] = dots[0][i];
-                sh.kx2[half][r] = dots[1][i];
-                sh.kx3[half][r] = dots[2][i];
+                sh.row_w[part][r] = row_w[i];
+                sh.row_u[part][r] = row_u[i];
+                sh.qx[part][r] = dots[0][i];
+                sh.kx2[part][r] = dots[1][i];
+                sh.kx3[part][r] = dots[2][i];
             }
         }
     }
@@ -689,11 +679,11 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) 
         for (int j = 0; j < 2; ++j) {
             const int r = 2 * lane + j;
             const float e = sh.gates.e[r], beta = sh.gates.beta[r];
-            const float kx2 = e * (sh.kx2[0][r] + sh.kx2[1][r]);
-            w[j] = sh.gates.left[r] * (sh.kx3[0][r] + sh.kx3[1][r]);
-            dg[j] = sh.row_w[0][r] + sh.row_w[1][r] - (sh.col_w[0][r] + sh.col_w[1][r] + sh.col_w[2][r] + sh.col_w[3][r]) +
-                    p.scale * e * (sh.qx[0][r] + sh.qx[1][r]) - beta * kx2 - w[j];
-            if (r < ch.rows) p.dbeta[(token0 + r) * p.value_heads + hv] = sh.drv[r] - kx2 + (sh.row_u[0][r] + sh.row_u[1][r]);
+            const auto sum = [&](const float (&x)[4][kChunk]) { return (x[0][r] + x[1][r]) + (x[2][r] + x[3][r]); };
+            const float kx2 = e * sum(sh.kx2);
+            w[j] = sh.gates.left[r] * sum(sh.kx3);
+            dg[j] = sum(sh.row_w) - sum(sh.col_w) + p.scale * e * sum(sh.qx) - beta * kx2 - w[j];
+            if (r < ch.rows) p.dbeta[(token0 + r) * p.value_heads + hv] = sh.drv[r] - kx2 + sum(sh.row_u);
         }
         float all = w[0] + w[1];
 #pragma unroll
@@ -747,11 +737,12 @@ void backward_as(const Args& a, cudaStream_t stream, int sm_count) {
         delta_do_kernel<T, DKP><<<dim3(a.chunks, a.value_heads), kDoThreads, sizeof(DoShared<T, DKP>), stream>>>(a);
         cuda_check(cudaGetLastError(), "delta rule P^T dO");
     }
-    const uint64_t chains = (uint64_t)(a.dvp / 16) * a.value_heads * a.seqs;        // as the forward's
-    const char* ks = getenv("DELTA_KS");
-    const int k = ks ? atoi(ks) : chains <= (uint64_t)sm_count ? 4 : chains <= 2 * (uint64_t)sm_count ? 2 : 1;
-    if (k == 4) reverse_as<T, DKP, 4>(a, stream);
-    else if (k == 2) reverse_as<T, DKP, 2>(a, stream);
+    // Four warps to a chain while there is at most one chain a multiprocessor, two up to two chains (or where sequences of
+    // uneven lengths leave the longest ones running alone), one beyond. 64 chunks of 128 x 128: 128 chains 242 (KS 4) 272 (2) 490 us
+    // (1); 256 chains 318, 272, 491; 512 chains 622, 540, 493; 1408 chains of eleven ragged sequences 287, 258, 312.
+    const uint64_t chains = (uint64_t)(a.dvp / 16) * a.value_heads * a.seqs;
+    if (chains <= (uint64_t)sm_count) reverse_as<T, DKP, 4>(a, stream);
+    else if (chains <= 2 * (uint64_t)sm_count || a.sequences) reverse_as<T, DKP, 2>(a, stream);
     else reverse_as<T, DKP, 1>(a, stream);
     if (a.chunks) {
         opt_in(delta_grad_kernel<T, DKP>, sizeof(GradShared<T, DKP>));

@@ -3,7 +3,6 @@
 #include "delta.h"
 #include "delta_tiles.cuh"
 #include "runtime.h"
-#include <cstdlib>
 
 namespace mlb {
 namespace delta {
@@ -197,8 +196,11 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const Args p, 
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const uint4 b = split_pair(w[k8][2 * n], w[k8][2 * n + 1]);
-#pragma unroll
-                    for (int term = 0; term < 3; ++term) mma_term8(out[n], s, b, term);
+                    float c[4];
+                    mma_term8<0>(c, s, b);
+                    mma_term8<1>(c, s, b);
+                    mma_term8<2>(c, s, b);
+                    add_to(out[n], c);
                 }
             }
 #pragma unroll
@@ -228,8 +230,8 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const Args p, 
 //
 // A chain is 16 value columns: S^T [16 x dk] lives in accumulators. X^T = S^T K^T; R^T = beta (V^T - e^G X^T);
 // D^T = R^T T^T; S^T = e^{G_63} S^T + (D^T e^{G_63 - G}) K: every product's accumulators are the next one's A operand, and K
-// comes from shared memory as B operands both ways round. KS warps share a chain where there are too few chains to fill the
-// GPU: each holds dk / KS of S's rows; partial X crosses through shared memory as whole fragments (a lane's 16 bytes, no bank
+// comes from shared memory as B operands both ways round. KS warps share a chain, each with dk / KS of S's rows, since a
+// chain is a sequence of dependent products and there are few chains; partial X crosses through shared memory as whole fragments (a lane's 16 bytes, no bank
 // met twice), R and D already in their parts. A fifth warp fetches the next chunk meanwhile.
 constexpr int kStateThreads = 160;
 
@@ -244,8 +246,8 @@ struct StateShared {
         alignas(16) float gates[3 * kChunk];        // e, left, beta
     } stage[2];
     // [warp][tile][lane]: partial X; then, when every R is there, [chain][tile]: e^{G_63 - G} D in parts
-    uint4 part[KS > 1 ? 4 * 8 * 32 : 1];
-    uint4 r[KS > 1 ? kGroups * 8 * kTileWords : 1]; // [chain][tile]: R in parts
+    uint4 part[4 * 8 * 32];
+    uint4 r[kGroups * 8 * kTileWords];              // [chain][tile]: R in parts
 };
 
 template <typename T, int DKP, int KS>
@@ -302,8 +304,8 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
             s[n][i] = p.initial_state && row(n, i) < (int)p.dk && col(i) < (int)p.dv
                           ? p.initial_state[state0 + (size_t)row(n, i) * p.dv + col(i)] : 0.0f;
 
-    uint4* r_parts = sh.r + (KS > 1 ? chain * 8 * kTileWords : 0);
-    uint4* d_parts = sh.part + (KS > 1 ? chain * 8 * kTileWords : 0);
+    uint4* r_parts = sh.r + chain * 8 * kTileWords;
+    uint4* d_parts = sh.part + chain * 8 * kTileWords;
     for (uint32_t c = c0; c < c1; ++c) {
         const typename Sh::Stage& st = sh.stage[(c - c0) & 1];
         __syncthreads();                                // this chunk is here, and every warp is done with the one before
@@ -330,26 +332,20 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
             a.set(s[2 * kk], s[2 * kk + 1]);
             mma_tile<T, 8, false>(x, a, st.k, LD, 0, k_base + 16 * kk);
         }
-        if constexpr (KS > 1) {
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
-                *reinterpret_cast<float4*>(sh.part + (warp * 8 + n) * 32 + lane) = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
-            asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
-        }
+        for (int n = 0; n < 8; ++n)
+            *reinterpret_cast<float4*>(sh.part + (warp * 8 + n) * 32 + lane) = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
+        asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
         // R for this warp's token tiles
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
-            const int n = KS > 1 ? own_tile<KS>(part, i) : i;
+            const int n = own_tile<KS>(part, i);
             float f[4] = {};
-            if constexpr (KS > 1) {
 #pragma unroll
-                for (int w = 0; w < KS; ++w) {          // always in the same order
-                    const float4 q = *reinterpret_cast<const float4*>(sh.part + ((chain * KS + w) * 8 + n) * 32 + lane);
-                    const float u[4] = {q.x, q.y, q.z, q.w};
-                    add_to(f, u);
-                }
-            } else {
-                add_to(f, x[i]);
+            for (int w = 0; w < KS; ++w) {          // always in the same order
+                const float4 q = *reinterpret_cast<const float4*>(sh.part + ((chain * KS + w) * 8 + n) * 32 + lane);
+                const float u[4] = {q.x, q.y, q.z, q.w};
+                add_to(f, u);
             }
             const float2 be = *reinterpret_cast<const float2*>(beta + 8 * n + 2 * t), ee = *reinterpret_cast<const float2*>(e + 8 * n + 2 * t);
             const T* v = st.v + (8 * n + 2 * t) * Sh::kLdV + 16 * chain + g;
@@ -357,33 +353,27 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
             f[1] = be.y * fmaf(-ee.y, f[1], to_f(v[Sh::kLdV]));
             f[2] = be.x * fmaf(-ee.x, f[2], to_f(v[8]));
             f[3] = be.y * fmaf(-ee.y, f[3], to_f(v[Sh::kLdV + 8]));
-            if constexpr (KS > 1) {
-                TileTf32 a;
-                a.set(f);
-                a.put(r_parts, n, lane);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[i][j] = f[j];
-            }
+            TileTf32 a;
+            a.set(f);
+            a.put(r_parts, n, lane);
         }
-        if constexpr (KS > 1) asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
+        asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
         // D^T = R^T T^T, a k of 8 at a time against the rows of T that reach it
         float d[kOwn][4] = {};
         const float2* tri = reinterpret_cast<const float2*>(st.tri) + lane;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             TileTf32 a;
-            if constexpr (KS > 1) a.get(r_parts, j, lane);
-            else                  a.set(x[j]);
+            a.get(r_parts, j, lane);
             // of a pair of tiles one lies above row 4 and one below: which products there are is mostly known
-            mma_triangle(d, a, [&](int i) { return KS == 1 ? i >= j : i < kOwn / 2 ? j < 4 && own_tile<KS>(part, i) >= j
-                                                                                   : j <= 4 || own_tile<KS>(part, i) >= j; },
-                         [&](int i) { return tri[tri_tile(KS > 1 ? own_tile<KS>(part, i) : i, j) * 32]; });
+            mma_triangle(d, a, [&](int i) { return i < kOwn / 2 ? j < 4 && own_tile<KS>(part, i) >= j
+                                                                   : j <= 4 || own_tile<KS>(part, i) >= j; },
+                         [&](int i) { return tri[tri_tile(own_tile<KS>(part, i), j) * 32]; });
         }
         float* d_out = p.d + at * kChunk * p.dvp + (size_t)(2 * t) * p.dvp + dv0 + g;
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
-            const int n = KS > 1 ? own_tile<KS>(part, i) : i;
+            const int n = own_tile<KS>(part, i);
             if (live) {
                 float* out = d_out + (size_t)(8 * n) * p.dvp;
                 out[0] = d[i][0];
@@ -393,13 +383,11 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
             }
             const float2 le = *reinterpret_cast<const float2*>(left + 8 * n + 2 * t);
             d[i][0] *= le.x; d[i][1] *= le.y; d[i][2] *= le.x; d[i][3] *= le.y;
-            if constexpr (KS > 1) {
-                Tile a;
-                a.set(d[i]);
-                a.put(d_parts, n, lane);
-            }
+            Tile a;
+            a.set(d[i]);
+            a.put(d_parts, n, lane);
         }
-        if constexpr (KS > 1) asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
+        asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
         // S' = e^{G_63} S + (e^{G_63 - G} K)^T D
         const float whole = e[kChunk - 1];
 #pragma unroll
@@ -407,14 +395,10 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             Sp a;
-            if constexpr (KS > 1) {
-                Tile u, v;
-                u.get(d_parts, 2 * j, lane);
-                v.get(d_parts, 2 * j + 1, lane);
-                a.set(u, v);
-            } else {
-                a.set(d[2 * j], d[2 * j + 1]);
-            }
+            Tile u, v;
+            u.get(d_parts, 2 * j, lane);
+            v.get(d_parts, 2 * j + 1, lane);
+            a.set(u, v);
             mma_tile<T, NT, true>(s, a, st.k, LD, k_base, 16 * j);
         }
     }
@@ -607,13 +591,11 @@ void states_as(const Args& a, cudaStream_t stream) {
 
 template <typename T, int DKP>
 void states_of(const Args& a, cudaStream_t stream, int sm_count) {
-    // A chain to four warps while the blocks so made fit the multiprocessors, to two while those do, else to one.
+    // Four warps to a chain while there are at most two chains a multiprocessor, two beyond. 64 chunks of 128 x 128: 128 chains
+    // 134 (four) 210 us (two); 256 chains 190, 212; 512 chains 372, 310. (One warp a chain: 367 us whatever their number up to 512.)
     const uint64_t chains = (uint64_t)(a.dvp / 16) * a.value_heads * a.seqs;
-    const char* ks = getenv("DELTA_KS");
-    const int k = ks ? atoi(ks) : chains <= (uint64_t)sm_count ? 4 : chains <= 2 * (uint64_t)sm_count ? 2 : 1;
-    if (k == 4) states_as<T, DKP, 4>(a, stream);
-    else if (k == 2) states_as<T, DKP, 2>(a, stream);
-    else states_as<T, DKP, 1>(a, stream);
+    if (chains <= 2 * (uint64_t)sm_count) states_as<T, DKP, 4>(a, stream);
+    else states_as<T, DKP, 2>(a, stream);
 }
 
 template <typename T, int DKP>

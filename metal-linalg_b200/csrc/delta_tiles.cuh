@@ -33,18 +33,31 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ bf16 from_f<bf16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
+// c = a b (kFirst) or c += a b. Not volatile: products of different accumulators may pass one another.
+template <bool kFirst>
 __device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if constexpr (kFirst)
+        asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+template <bool kFirst>
 __device__ __forceinline__ void mma_16(bf16, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    if constexpr (kFirst)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+template <bool kFirst>
 __device__ __forceinline__ void mma_16(__half, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    static_assert(kFirst, "two float16 operands are multiplied a k of 16 at a time");
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // x to the nearest tf32 (halves away from zero) and what is left, exact in float32; the tensor core cuts the rest's
@@ -171,23 +184,26 @@ template <> struct Split<bf16>   { using type = SplitBf16; using tile = TileBf16
 template <> struct Split<__half> { using type = SplitTf32; using tile = TileTf32; static constexpr int kTerms = 2; };
 template <> struct Split<float>  { using type = SplitTf32; using tile = TileTf32; static constexpr int kTerms = 3; };
 
-// c += one part of the product of a float32 operand with a tile's; term 0 is the smallest.
-__device__ __forceinline__ void mma_term(float (&c)[4], const SplitBf16& a, const FragB<bf16>& b, int term) {
-    mma_16(bf16(), c, a.part[2 - term], b.r[0], b.r[1]);
+// One part of the product of a float32 operand with a tile's; term 0 is the smallest, and c's first.
+template <int kTerm>
+__device__ __forceinline__ void mma_term(float (&c)[4], const SplitBf16& a, const FragB<bf16>& b) {
+    mma_16<kTerm == 0>(bf16(), c, a.part[2 - kTerm], b.r[0], b.r[1]);
 }
-__device__ __forceinline__ void mma_term(float (&c)[4], const SplitTf32& a, const FragB<__half>& b, int term) {
-    const uint32_t (&p)[8] = term == 0 ? a.lo : a.hi;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b.r[h]));
-        mma_tf32(c, p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3], __float_as_uint(f.x), __float_as_uint(f.y));
-    }
+template <int kTerm>
+__device__ __forceinline__ void mma_term(float (&c)[4], const SplitTf32& a, const FragB<__half>& b) {
+    const uint32_t (&p)[8] = kTerm == 0 ? a.lo : a.hi;
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b.r[0])), g = __half22float2(*reinterpret_cast<const __half2*>(&b.r[1]));
+    mma_tf32<kTerm == 0>(c, p[0], p[1], p[2], p[3], __float_as_uint(f.x), __float_as_uint(f.y));
+    mma_tf32<false>(c, p[4], p[5], p[6], p[7], __float_as_uint(g.x), __float_as_uint(g.y));
 }
-__device__ __forceinline__ void mma_term(float (&c)[4], const SplitTf32& a, const FragB<float>& b, int term) {
-    const uint32_t (&p)[8] = term == 0 ? a.lo : a.hi;
-    const uint32_t (&q)[4] = term == 1 ? b.lo : b.hi;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) mma_tf32(c, p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3], q[2 * h], q[2 * h + 1]);
+// kExact: the A operand is exact in its first part, so that term 1 is c's first.
+template <int kTerm, bool kExact = false>
+__device__ __forceinline__ void mma_term(float (&c)[4], const SplitTf32& a, const FragB<float>& b) {
+    if constexpr (kExact && kTerm == 0) return;
+    const uint32_t (&p)[8] = kTerm == 0 ? a.lo : a.hi;
+    const uint32_t (&q)[4] = kTerm == 1 ? b.lo : b.hi;
+    mma_tf32<kTerm == (kExact ? 1 : 0)>(c, p[0], p[1], p[2], p[3], q[0], q[1]);
+    mma_tf32<false>(c, p[4], p[5], p[6], p[7], q[2], q[3]);
 }
 
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -257,11 +273,14 @@ __device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const typename Spl
             if constexpr (kCols) load_b_cols<T>(b[j], tile, ld, n0 + 8 * (n + 2 * j), k0);
             else                 load_b_rows<T>(b[j], tile, ld, n0 + 8 * (n + 2 * j), k0);
         }
-        float c[kGroup][4] = {};
+        float c[kGroup][4];
 #pragma unroll
-        for (int term = 0; term < Split<T>::kTerms; ++term)
+        for (int j = 0; j < kGroup; ++j) mma_term<0>(c[j], a, b[j / 2][j & 1]);
 #pragma unroll
-            for (int j = 0; j < kGroup; ++j) mma_term(c[j], a, b[j / 2][j & 1], term);
+        for (int j = 0; j < kGroup; ++j) mma_term<1>(c[j], a, b[j / 2][j & 1]);
+        if constexpr (Split<T>::kTerms == 3)
+#pragma unroll
+            for (int j = 0; j < kGroup; ++j) mma_term<2>(c[j], a, b[j / 2][j & 1]);
 #pragma unroll
         for (int j = 0; j < kGroup; ++j) add_to(acc[n + j], c[j]);
     }
@@ -281,9 +300,9 @@ __device__ __forceinline__ void mma_rows_rows(float (&acc)[NT][4], const T* a_ti
         for (int n = 0; n < NT; n += 2) {
             FragB<T> b[2];
             load_b_rows<T>(b, b_tile, ldb, n0 + 8 * n, k0);
-            float c[2][4] = {};
-            mma_16(T(), c[0], a, b[0].r[0], b[0].r[1]);
-            mma_16(T(), c[1], a, b[1].r[0], b[1].r[1]);
+            float c[2][4];
+            mma_16<true>(T(), c[0], a, b[0].r[0], b[0].r[1]);
+            mma_16<true>(T(), c[1], a, b[1].r[0], b[1].r[1]);
             add_to(acc[n], c[0]);
             add_to(acc[n + 1], c[1]);
         }
@@ -306,11 +325,12 @@ __device__ __forceinline__ void mma_rows_rows(float (&acc)[NT][4], const T* a_ti
 // The tiles of a lower triangle, (row tile i, column tile j <= i), one after another.
 __device__ __forceinline__ constexpr int tri_tile(int i, int j) { return i * (i + 1) / 2 + j; }
 
-// c += one part of a k of 8 of a float32 operand times a tile of fragments in tf32 parts (a lane's uint4: hi of k 2t, hi of
-// k 2t + 1, lo, lo).
-__device__ __forceinline__ void mma_term8(float (&c)[4], const TileTf32& a, const uint4& b, int term) {
-    const uint4& p = term == 0 ? a.lo : a.hi;
-    mma_tf32(c, p.x, p.y, p.z, p.w, term == 1 ? b.z : b.x, term == 1 ? b.w : b.y);
+// One part of a k of 8 of a float32 operand times a fragment in tf32 parts (hi of k 2t, hi of k 2t + 1, lo, lo); term 0 is c's
+// first.
+template <int kTerm>
+__device__ __forceinline__ void mma_term8(float (&c)[4], const TileTf32& a, const uint4& b) {
+    const uint4& p = kTerm == 0 ? a.lo : a.hi;
+    mma_tf32<kTerm == 0>(c, p.x, p.y, p.z, p.w, kTerm == 1 ? b.z : b.x, kTerm == 1 ? b.w : b.y);
 }
 __device__ __forceinline__ uint4 split_pair(float x, float y) {
     uint4 r;
@@ -325,7 +345,7 @@ __device__ __forceinline__ void mma_triangle(float (&acc)[N][4], const TileTf32&
     constexpr int kGroup = N < 4 ? N : 4;
 #pragma unroll
     for (int n0 = 0; n0 < N; n0 += kGroup) {
-        float c[kGroup][4] = {};
+        float c[kGroup][4];
         uint4 b[kGroup];
 #pragma unroll
         for (int n = 0; n < kGroup; ++n)
@@ -334,10 +354,14 @@ __device__ __forceinline__ void mma_triangle(float (&acc)[N][4], const TileTf32&
                 b[n] = split_pair(f.x, f.y);
             }
 #pragma unroll
-        for (int term = 0; term < 3; ++term)
+        for (int n = 0; n < kGroup; ++n)
+            if (wanted(n0 + n)) mma_term8<0>(c[n], a, b[n]);
 #pragma unroll
-            for (int n = 0; n < kGroup; ++n)
-                if (wanted(n0 + n)) mma_term8(c[n], a, b[n], term);
+        for (int n = 0; n < kGroup; ++n)
+            if (wanted(n0 + n)) mma_term8<1>(c[n], a, b[n]);
+#pragma unroll
+        for (int n = 0; n < kGroup; ++n)
+            if (wanted(n0 + n)) mma_term8<2>(c[n], a, b[n]);
 #pragma unroll
         for (int n = 0; n < kGroup; ++n)
             if (wanted(n0 + n)) add_to(acc[n0 + n], c[n]);
