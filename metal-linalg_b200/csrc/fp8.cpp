@@ -54,8 +54,8 @@ void quantize_fp8(const void* x, uint32_t dtype, uint32_t batch, uint32_t rows, 
     if (batch == 0 || rows == 0 || cols == 0) return;
     if (col_stride != 1 && row_stride != 1) refuse(who, "one of row_stride and col_stride must be 1");
     if (batch > 65535) refuse(who, "batch must be at most 65535");
-    if (rows >= 1u << 30 || cols >= 1u << 30 || (uint64_t)rows * ((cols + 127) / 128) >= 1ull << 32)
-        refuse(who, "rows and cols must be below 2^30, and the matrix below 2^39 elements");
+    if (rows >= 1u << 30 || cols >= 1u << 30 || (uint64_t)rows * ((cols + 127) / 128) >= 1ull << 31)
+        refuse(who, "rows and cols must be below 2^30, and the matrix below 2^38 elements");
     if (!aligned16(values) || values_stride % 16 || values_stride < cols)
         refuse(who, "values must be on a 16-byte boundary, its rows a multiple of 16 bytes apart and no shorter than cols");
     int device = place(who, x, "x", -1);

@@ -5,9 +5,9 @@
 // The quotient is correctly rounded, so that the values are the definition's bit for bit. Every kernel reads x once: what
 // bounds them is memory.
 //   rows     x contiguous along columns, 1 x 128: 16 lanes a block, eight values a lane
-//   tiles    the same in 128 x 128: 256 threads hold the tile in registers
+//   tiles    the same in 128 x 128: 512 threads hold the tile in registers
 //   turned   x contiguous along rows (a transposed matrix): a 128 x 128 tile through shared memory as it lies, read back a
-//            row of the result a thread pair, either block shape
+//            quarter of a row of the result a thread, either block shape
 #include "fp8.h"
 #include "runtime.h"
 
@@ -19,50 +19,91 @@ namespace fp8 {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kRowThreads = 256;       // quantize_rows_kernel's
+constexpr int kTileThreads = 256;      // quantize_tiles_kernel's
+constexpr int kThreads = 512;          // quantize_turned_kernel's
 constexpr int kB = 128;
 
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
 
-// The larger of two magnitudes; NaN wins.
+// The largest of two (three) magnitudes; NaN wins.
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// Pairs of float32 in one instruction.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair_of(float x, float y) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// x / y, correctly rounded, with r the correctly rounded reciprocal of y: q + (x - q y) r in fused operations for q = x r
+// (Markstein, IBM J. Res. Dev. 34, 1990), as long as the remainder is exact. Outside 2^-100 .. 2^120 the remainder can underflow
+// (or y is infinite or NaN): there it is the division itself.
+__device__ __forceinline__ bool markstein_holds(float y) { return y >= 0x1p-100f && y <= 0x1p120f; }
+
 template <bool kE5m2>
 __device__ __forceinline__ float scale_of(float top) {
-    const float s = __fdiv_rn(top, kE5m2 ? 57344.0f : 448.0f);
+    constexpr float kMost = kE5m2 ? 57344.0f : 448.0f, kInverse = 1.0f / kMost;
+    if (markstein_holds(top)) {                     // the remainder of top / M is as far from underflow as top is
+        const float q = top * kInverse;
+        return fmaf(fmaf(-q, kMost, top), kInverse, q);
+    }
+    const float s = __fdiv_rn(top, kMost);
     return s < 1.17549435e-38f ? 1.17549435e-38f : s;          // NaN stays
 }
 template <bool kE5m2>
-__device__ __forceinline__ uint32_t pair_of(float low, float high) {
+__device__ __forceinline__ uint32_t bytes_of(float low, float high) {
     uint16_t r;
     if constexpr (kE5m2) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(high), "f"(low));
     else                 asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(high), "f"(low));
     return r;
 }
-// x / scale, correctly rounded, for one scale and many x. With r the correctly rounded reciprocal and q = x r,
-// q + (x - q scale) r in fused operations is the correctly rounded quotient (Markstein, IBM J. Res. Dev. 34, 1990) as long
-// as the remainder is exact: three operations a value instead of a division's ten or so. Outside 2^-100 .. 2^120 the
-// remainder can underflow (or the scale is infinite or NaN): there it is the division itself.
-struct Quotient {
-    float scale, r;
-    bool  plain;
-    __device__ __forceinline__ explicit Quotient(float s) : scale(s), r(1.0f / s), plain(!(s >= 0x1p-100f && s <= 0x1p120f)) {}
-    __device__ __forceinline__ float operator()(float x) const {
-        const float q = x * r;
-        return fmaf(fmaf(-q, scale, x), r, q);
+// N values (a multiple of four) divided by their scale, packed.
+template <bool kE5m2, int N>
+__device__ __forceinline__ void divided(const float (&v)[N], float scale, uint32_t (&out)[N / 4]) {
+    if (!markstein_holds(scale)) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            out[i / 4] = bytes_of<kE5m2>(__fdiv_rn(v[i], scale), __fdiv_rn(v[i + 1], scale)) |
+                         (bytes_of<kE5m2>(__fdiv_rn(v[i + 2], scale), __fdiv_rn(v[i + 3], scale)) << 16);
+        return;
     }
-};
-template <bool kE5m2>
-__device__ __forceinline__ uint32_t four_of(const float* v, const Quotient& by) {
-    if (by.plain)
-        return pair_of<kE5m2>(__fdiv_rn(v[0], by.scale), __fdiv_rn(v[1], by.scale)) |
-               (pair_of<kE5m2>(__fdiv_rn(v[2], by.scale), __fdiv_rn(v[3], by.scale)) << 16);
-    return pair_of<kE5m2>(by(v[0]), by(v[1])) | (pair_of<kE5m2>(by(v[2]), by(v[3])) << 16);
+    const float r = 1.0f / scale;
+    const Pair r2 = pair_of(r, r), minus = pair_of(-scale, -scale);
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        uint32_t half[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const Pair x = pair_of(v[i + 2 * j], v[i + 2 * j + 1]), q = mul2(x, r2), y = fma2(fma2(q, minus, x), r2, q);
+            float low, high;
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(low), "=f"(high) : "l"(y));
+            half[j] = bytes_of<kE5m2>(low, high);
+        }
+        out[i / 4] = half[0] | (half[1] << 16);
+    }
 }
 
 // Eight neighbouring values from column c on as they lie in memory; zero behind the last.
@@ -90,34 +131,63 @@ template <typename T> struct Eight {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = as_float(e[i]);
     }
+    __device__ __forceinline__ float top() const {
+        float v[8], t = 0.0f;
+        get(v);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) t = max_nan(t, fabsf(v[i]), fabsf(v[i + 1]));
+        return t;
+    }
+    template <bool kE5m2> __device__ __forceinline__ uint2 divided_by(float scale) const {
+        float v[8];
+        uint32_t out[2];
+        get(v);
+        divided<kE5m2, 8>(v, scale, out);
+        return make_uint2(out[0], out[1]);
+    }
 };
 
-template <typename T, bool kE5m2>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeArgs a) {
+// kUnits blocks of 128 for every 16 lanes, all fetched before the first is used.
+template <typename T, bool kE5m2, int kUnits>
+__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const QuantizeArgs a) {
     const uint32_t blocks = (a.cols + kB - 1) / kB, z = blockIdx.y;
-    const uint64_t unit = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) >> 4;
-    const uint64_t units = (uint64_t)a.rows * blocks;
-    const bool there = unit < units;                    // whole warps take part in the exchange
-    const uint32_t row = there ? (uint32_t)(unit / blocks) : 0, block = there ? (uint32_t)(unit - (uint64_t)row * blocks) : 0;
-    const uint32_t c = block * kB + (threadIdx.x & 15) * 8;
-    Eight<T> x;
-    x.clear();
-    if (there) x.load(static_cast<const T*>(a.x) + z * a.batch_stride + (long long)row * a.row_stride, c, a.cols, a.vec);
-    float v[8], top = 0.0f;
-    x.get(v);
+    const uint32_t first = blockIdx.x * (kRowThreads / 16 * kUnits) + (threadIdx.x >> 4);
+    const uint32_t in = (threadIdx.x & 15) * 8;
+    // one division; the next units are 16 further along the row, or in rows behind it
+    uint32_t row[kUnits], block[kUnits];
+    row[0] = first / blocks;
+    block[0] = first - row[0] * blocks;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(v[i]));
+    for (int i = 1; i < kUnits; ++i) {
+        row[i] = row[i - 1];
+        block[i] = block[i - 1] + kRowThreads / 16;
+        while (block[i] >= blocks) {
+            block[i] -= blocks;
+            ++row[i];
+        }
+    }
+    Eight<T> x[kUnits];
+    const T* src = static_cast<const T*>(a.x) + z * a.batch_stride;
 #pragma unroll
-    for (int o = 1; o < 16; o *= 2) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float scale = scale_of<kE5m2>(top);
-    if (!there) return;
-    const Quotient by(scale);
-    if (c < a.cols)
-        *reinterpret_cast<uint2*>(a.values + z * a.values_batch + row * a.values_stride + c) =
-            make_uint2(four_of<kE5m2>(v, by), four_of<kE5m2>(v + 4, by));
-    if ((threadIdx.x & 15) == 0) a.scales[((uint64_t)z * a.rows + row) * blocks + block] = scale;
+    for (int i = 0; i < kUnits; ++i) {
+        if (row[i] < a.rows) x[i].load(src + (long long)row[i] * a.row_stride, block[i] * kB + in, a.cols, a.vec);
+        else                 x[i].clear();          // a unit past the last takes part in the exchange all the same
+    }
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+        float top = x[i].top();
+#pragma unroll
+        for (int o = 1; o < 16; o *= 2) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (row[i] >= a.rows) continue;
+        const uint32_t c = block[i] * kB + in;
+        const float scale = scale_of<kE5m2>(top);
+        if (c < a.cols)
+            *reinterpret_cast<uint2*>(a.values + z * a.values_batch + row[i] * a.values_stride + c) = x[i].template divided_by<kE5m2>(scale);
+        if ((threadIdx.x & 15) == 0) a.scales[((uint64_t)z * a.rows + row[i]) * blocks + block[i]] = scale;
+    }
 }
 
+template <int kCount>
 __device__ __forceinline__ float block_max(float top, float* shared) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -125,53 +195,50 @@ __device__ __forceinline__ float block_max(float top, float* shared) {
     __syncthreads();
     top = shared[0];
 #pragma unroll
-    for (int i = 1; i < kThreads / 32; ++i) top = max_nan(top, shared[i]);
+    for (int i = 1; i < kCount / 32; ++i) top = max_nan(top, shared[i]);
     return top;
 }
 
 template <typename T, bool kE5m2>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) quantize_tiles_kernel(const QuantizeArgs a) {
-    __shared__ float tops[kThreads / 32];
+__global__ void __launch_bounds__(kTileThreads, sizeof(T) == 2 ? 4 : 2) quantize_tiles_kernel(const QuantizeArgs a) {
+    constexpr int kRows = kTileThreads / 16, kHeld = kB / kRows;
+    __shared__ float tops[kTileThreads / 32];
     const uint32_t blocks = (a.cols + kB - 1) / kB, z = blockIdx.y;
     const uint32_t br = blockIdx.x / blocks, bc = blockIdx.x - br * blocks;
     const uint32_t c = bc * kB + (threadIdx.x & 15) * 8, r0 = br * kB + (threadIdx.x >> 4);
     const T* x = static_cast<const T*>(a.x) + z * a.batch_stride;
-    Eight<T> held[8];
+    Eight<T> held[kHeld];
     float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t r = r0 + 16 * i;
+    for (int i = 0; i < kHeld; ++i) {
+        const uint32_t r = r0 + kRows * i;
         if (r < a.rows) held[i].load(x + (long long)r * a.row_stride, c, a.cols, a.vec);
         else            held[i].clear();
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float v[8];
-        held[i].get(v);
+    for (int i = 0; i < kHeld; ++i) top = max_nan(top, held[i].top());
+    const float scale = scale_of<kE5m2>(block_max<kTileThreads>(top, tops));
+    // as they lie in memory until here: unpacked twice, they take half the registers
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(v[j]));
-    }
-    const float scale = scale_of<kE5m2>(block_max(top, tops));
-    const Quotient by(scale);
+    for (int i = 0; i < kHeld; ++i)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t r = r0 + 16 * i;
-        float v[8];
-        held[i].get(v);
+        for (int j = 0; j < Eight<T>::kWords; ++j) asm volatile("" : "+r"(held[i].w[j].x), "+r"(held[i].w[j].y), "+r"(held[i].w[j].z), "+r"(held[i].w[j].w));
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const uint32_t r = r0 + kRows * i;
         if (r < a.rows && c < a.cols)
-            *reinterpret_cast<uint2*>(a.values + z * a.values_batch + r * a.values_stride + c) =
-                make_uint2(four_of<kE5m2>(v, by), four_of<kE5m2>(v + 4, by));
+            *reinterpret_cast<uint2*>(a.values + z * a.values_batch + r * a.values_stride + c) = held[i].template divided_by<kE5m2>(scale);
     }
     if (threadIdx.x == 0) a.scales[((uint64_t)z * ((a.rows + kB - 1) / kB) + br) * blocks + bc] = scale;
 }
 
-// x(r, c) at c * col_stride + r. The tile lies in shared memory as [column][row]; thread (r, half) then takes 64 columns of
+// x(r, c) at c * col_stride + r. The tile lies in shared memory as [column][row]; thread (r, part) then takes 32 columns of
 // row r, neighbouring lanes neighbouring rows.
 template <typename T, bool kE5m2>
-__global__ void __launch_bounds__(kThreads) quantize_turned_kernel(const QuantizeArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) quantize_turned_kernel(const QuantizeArgs a) {
     extern __shared__ __align__(16) char raw[];
     T* tile = reinterpret_cast<T*>(raw);
-    __shared__ float tops[2 * kB];
+    __shared__ float tops[kThreads];
     const uint32_t blocks = (a.cols + kB - 1) / kB, z = blockIdx.y;
     const uint32_t br = blockIdx.x / blocks, bc = blockIdx.x - br * blocks;
     const uint32_t r0 = br * kB, c0 = bc * kB;
@@ -205,31 +272,33 @@ __global__ void __launch_bounds__(kThreads) quantize_turned_kernel(const Quantiz
         }
     }
     __syncthreads();
-    const uint32_t r = threadIdx.x & (kB - 1), half = threadIdx.x / kB;
-    float v[kB / 2];
+    constexpr int kMine = kB * kB / kThreads;
+    const uint32_t r = threadIdx.x & (kB - 1), part = threadIdx.x / kB;
+    float v[kMine];
     float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kB / 2; ++i) {
-        v[i] = as_float(tile[(half * (kB / 2) + i) * kB + r]);
-        top = max_nan(top, fabsf(v[i]));
+    for (int i = 0; i < kMine; ++i) {
+        v[i] = as_float(tile[(part * kMine + i) * kB + r]);
+        if (i & 1) top = max_nan(top, fabsf(v[i - 1]), fabsf(v[i]));
     }
     if (a.block_rows == 1) {
         tops[threadIdx.x] = top;
         __syncthreads();
-        top = max_nan(tops[r], tops[kB + r]);
+        top = max_nan(max_nan(tops[r], tops[kB + r]), max_nan(tops[2 * kB + r], tops[3 * kB + r]));
     } else {
-        top = block_max(top, tops);
+        top = block_max<kThreads>(top, tops);
     }
     const float scale = scale_of<kE5m2>(top);
-    const Quotient by(scale);
     if (r0 + r < a.rows) {
-        uint8_t* out = a.values + z * a.values_batch + (r0 + r) * a.values_stride + c0 + half * (kB / 2);
+        uint8_t* out = a.values + z * a.values_batch + (r0 + r) * a.values_stride + c0 + part * kMine;
 #pragma unroll
-        for (int i = 0; i < kB / 2; i += 16)
-            if (c0 + half * (kB / 2) + i < a.cols)
-                *reinterpret_cast<uint4*>(out + i) = make_uint4(four_of<kE5m2>(v + i, by), four_of<kE5m2>(v + i + 4, by),
-                                                               four_of<kE5m2>(v + i + 8, by), four_of<kE5m2>(v + i + 12, by));
-        if (a.block_rows == 1 && half == 0) a.scales[((uint64_t)z * a.rows + r0 + r) * blocks + bc] = scale;
+        for (int i = 0; i < kMine; i += 16)
+            if (c0 + part * kMine + i < a.cols) {
+                uint32_t bytes[4];
+                divided<kE5m2, 16>(*reinterpret_cast<const float (*)[16]>(v + i), scale, bytes);
+                *reinterpret_cast<uint4*>(out + i) = make_uint4(bytes[0], bytes[1], bytes[2], bytes[3]);
+            }
+        if (a.block_rows == 1 && part == 0) a.scales[((uint64_t)z * a.rows + r0 + r) * blocks + bc] = scale;
     }
     if (a.block_rows != 1 && threadIdx.x == 0) a.scales[((uint64_t)z * ((a.rows + kB - 1) / kB) + br) * blocks + bc] = scale;
 }
@@ -243,10 +312,14 @@ void quantize_as(const QuantizeArgs& a, cudaStream_t stream) {
                    "quantize shared memory");
         quantize_turned_kernel<T, kE5m2><<<dim3((unsigned)tiles, a.batch), kThreads, bytes, stream>>>(a);
     } else if (a.block_rows == 1) {
-        const uint64_t grid = (a.rows * blocks + kThreads / 16 - 1) / (kThreads / 16);
-        quantize_rows_kernel<T, kE5m2><<<dim3((unsigned)grid, a.batch), kThreads, 0, stream>>>(a);
+        // four blocks of 128 a thread where that still leaves every multiprocessor two thread blocks
+        const uint64_t units = a.rows * blocks, each = kRowThreads / 16;
+        if (units * a.batch >= 4 * each * 2 * (uint64_t)sm_count(current_device()))
+            quantize_rows_kernel<T, kE5m2, 4><<<dim3((unsigned)((units + 4 * each - 1) / (4 * each)), a.batch), kRowThreads, 0, stream>>>(a);
+        else
+            quantize_rows_kernel<T, kE5m2, 1><<<dim3((unsigned)((units + each - 1) / each), a.batch), kRowThreads, 0, stream>>>(a);
     } else {
-        quantize_tiles_kernel<T, kE5m2><<<dim3((unsigned)tiles, a.batch), kThreads, 0, stream>>>(a);
+        quantize_tiles_kernel<T, kE5m2><<<dim3((unsigned)tiles, a.batch), kTileThreads, 0, stream>>>(a);
     }
     cuda_check(cudaGetLastError(), "quantize launch");
 }
