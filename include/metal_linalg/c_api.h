@@ -155,7 +155,9 @@ typedef enum metal_linalg_dtype {
  * behind the last sequence give outputs and gradients of zero. A sequence may be empty: its state
  * passes through.
  *
- * All pointers are CUDA device pointers on one GPU; the work is enqueued on the
+ * All pointers are CUDA device pointers on one GPU: `device` names it, which the
+ * caller vouches for, or is -1 and the call looks each pointer up (about 0.3 us a
+ * pointer) and refuses those that are not. The work is enqueued on the
  * calling thread's stream (metal_linalg_set_stream). Nothing is allocated: the
  * caller gives the workspace, so that calls on several streams, or in several
  * captured graphs, each have their own. */
@@ -165,6 +167,8 @@ typedef struct metal_linalg_delta {
     uint32_t     dtype;                                       /* a metal_linalg_dtype */
     uint32_t     index_bytes;                                 /* of cu_seqlens and slots: 4 or 8 */
     float        scale;
+    int32_t      device;                                      /* the GPU that every pointer is on, vouched for by the caller; -1: look */
+    uint32_t     reserved;                                    /* 0 */
     const void  *q, *k, *v;
     const float *g, *beta;
     const float *initial_state;                               /* [sequences or batch, value_heads, key_dim, value_dim], or NULL: zero */
@@ -213,11 +217,13 @@ metal_linalg_status metal_linalg_gated_delta_step(const metal_linalg_delta* p, v
  * block_rows (1 or 128) x 128: scale = max(max|x| / M, 2^-126) with M the type's
  * largest value (448 or 57344), value = x / scale, a float32 rounded to the nearest, ties to even.
  * scales [batch, ceil(rows / block_rows), ceil(cols / 128)]. A block with a NaN or an
- * infinity stands for NaN throughout. (A transposed matrix is given by its strides.) */
+ * infinity stands for NaN throughout. (A transposed matrix is given by its strides.)
+ * device: the GPU that every pointer is on, vouched for by the caller, or -1: the call
+ * looks each pointer up (about 0.3 us a pointer) and refuses those that are not on one GPU. */
 metal_linalg_status metal_linalg_quantize_fp8(const void* x, metal_linalg_dtype dtype, uint32_t batch, uint32_t rows,
                                               uint32_t cols, int64_t batch_stride, int64_t row_stride, int64_t col_stride,
                                               uint32_t block_rows, metal_linalg_dtype kind, void* values,
-                                              uint64_t values_stride, float* scales);
+                                              uint64_t values_stride, float* scales, int device);
 
 /* One operand of metal_linalg_matmul_fp8: `values` with k contiguous, rows
  * `stride` bytes and matrices `batch_stride` bytes apart (0: one matrix for the
@@ -233,10 +239,11 @@ typedef struct metal_linalg_fp8_operand {
 } metal_linalg_fp8_operand;
 
 /* c [batch, m, n] = a [batch, m, k] b [batch, n, k]^T (float32, bfloat16 or float16, contiguous):
- * products of 128 along k on the tensor cores, times both blocks' scales and summed in float32. */
+ * products of 128 along k on the tensor cores, times both blocks' scales and summed in float32.
+ * device: as for metal_linalg_quantize_fp8. */
 metal_linalg_status metal_linalg_matmul_fp8(const metal_linalg_fp8_operand* a, const metal_linalg_fp8_operand* b,
                                             uint32_t batch, uint32_t m, uint32_t n, uint32_t k, void* c,
-                                            metal_linalg_dtype c_dtype);
+                                            metal_linalg_dtype c_dtype, int device);
 
 /* ---------------------------------------------------------------------------
  * CUDA placement (no counterpart in the reference, whose memory is unified)

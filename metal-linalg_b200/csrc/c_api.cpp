@@ -228,18 +228,18 @@ metal_linalg_status metal_linalg_gated_delta_step(const metal_linalg_delta* p, v
 
 metal_linalg_status metal_linalg_quantize_fp8(const void* x, metal_linalg_dtype dtype, uint32_t batch, uint32_t rows, uint32_t cols,
                                               int64_t batch_stride, int64_t row_stride, int64_t col_stride, uint32_t block_rows,
-                                              metal_linalg_dtype kind, void* values, uint64_t values_stride, float* scales) {
+                                              metal_linalg_dtype kind, void* values, uint64_t values_stride, float* scales, int device) {
     return run([&] {
         ml::core::quantize_fp8(x, (uint32_t)dtype, batch, rows, cols, batch_stride, row_stride, col_stride, block_rows, (uint32_t)kind,
-                               values, values_stride, scales);
+                               values, values_stride, scales, device);
     });
 }
 
 metal_linalg_status metal_linalg_matmul_fp8(const metal_linalg_fp8_operand* a, const metal_linalg_fp8_operand* b, uint32_t batch,
-                                            uint32_t m, uint32_t n, uint32_t k, void* c, metal_linalg_dtype c_dtype) {
+                                            uint32_t m, uint32_t n, uint32_t k, void* c, metal_linalg_dtype c_dtype, int device) {
     return run([&] {
         if (!a || !b) throw std::invalid_argument("[matmul_fp8] an operand is NULL");
-        ml::core::matmul_fp8(*a, *b, batch, m, n, k, c, (uint32_t)c_dtype);
+        ml::core::matmul_fp8(*a, *b, batch, m, n, k, c, (uint32_t)c_dtype, device);
     });
 }
 

@@ -40,13 +40,20 @@ void check_sequences(const char* who, const metal_linalg_delta& p) {
 // Every pointer is on one GPU, which is returned.
 struct Placement {
     const char* who;
-    int device = -1;
+    int  device;
+    bool known;                 // the caller vouches for it
+    bool any = false;           // there is a pointer at all
+    Placement(const char* w, int d) : who(w), device(d), known(d >= 0) {
+        if (d < -1) refuse(w, "device must be a GPU or -1");
+    }
     void need(const void* ptr, const char* name) {
         if (!ptr) refuse(who, std::string(name) + " is NULL");
         optional(ptr, name);
     }
     void optional(const void* ptr, const char* name) {
         if (!ptr) return;
+        any = true;
+        if (known) return;
         const int d = mlb::pointer_device(ptr);
         if (d < 0) refuse(who, std::string(name) + " is not a device pointer");
         if (device < 0) device = d;
@@ -119,8 +126,8 @@ uint64_t carve(Args& a, char* base, bool backward) {
     return w.at;
 }
 
-// The inputs of either direction, checked; nothing to do (no states and no outputs) gives device -1.
-int check_inputs(const char* who, const metal_linalg_delta& p, Placement& where) {
+// The inputs of either direction, checked.
+void check_inputs(const char* who, const metal_linalg_delta& p, Placement& where) {
     check_shape(who, p);
     check_sequences(who, p);
     if (cpu_only()) throw std::runtime_error(std::string(who) + " this thread is set CPU-only, and this build has no CPU path");
@@ -136,7 +143,6 @@ int check_inputs(const char* who, const metal_linalg_delta& p, Placement& where)
         where.need(p.beta, "beta");
     }
     where.optional(p.initial_state, "initial_state");
-    return where.device;
 }
 
 void check_workspace(const char* who, uint64_t need, void* workspace, uint64_t bytes, Placement& where) {
@@ -157,13 +163,13 @@ uint64_t gated_delta_rule_workspace_bytes(const metal_linalg_delta& p, bool back
 
 void gated_delta_rule(const metal_linalg_delta& p, void* o, float* final_state, void* workspace, uint64_t bytes) {
     const char* who = "[gated_delta_rule]";
-    Placement where{who};
+    Placement where(who, p.device);
     check_inputs(who, p, where);
     if ((uint64_t)p.batch * p.tokens) where.need(o, "o");
     where.optional(final_state, "final_state");
     Args a = args_of(p);
     check_workspace(who, carve(a, nullptr, false), workspace, bytes, where);
-    if (where.device < 0 || a.seqs == 0) return;
+    if (!where.any || a.seqs == 0) return;
     carve(a, static_cast<char*>(workspace), false);
     a.o = o;
     a.final_state = final_state;
@@ -175,7 +181,7 @@ void gated_delta_rule_backward(const metal_linalg_delta& p, const void* d_o, con
                                const float* d_final_state, void* dq, void* dk, void* dv, float* dg, float* dbeta,
                                float* d_initial_state, void* workspace, uint64_t bytes) {
     const char* who = "[gated_delta_rule_backward]";
-    Placement where{who};
+    Placement where(who, p.device);
     check_inputs(who, p, where);
     Args a = args_of(p);
     if ((uint64_t)p.batch * p.tokens) {
@@ -193,7 +199,7 @@ void gated_delta_rule_backward(const metal_linalg_delta& p, const void* d_o, con
     where.optional(d_final_state, "d_final_state");
     where.optional(d_initial_state, "d_initial_state");
     check_workspace(who, carve(a, nullptr, true), workspace, bytes, where);
-    if (where.device < 0 || a.seqs == 0) return;
+    if (!where.any || a.seqs == 0) return;
     carve(a, static_cast<char*>(workspace), true);
     a.d_o = d_o;
     a.d_final = d_final_state;
@@ -212,7 +218,7 @@ void gated_delta_step(const metal_linalg_delta& p, void* o, float* pool, int64_t
     if ((uint64_t)p.batch * p.tokens == 0) return;
     const int64_t state = (int64_t)p.value_heads * p.key_dim * p.value_dim;
     if (pool_size > 1 && pool_stride < state) refuse(who, "pool_stride is smaller than a state");
-    Placement where{who};
+    Placement where(who, p.device);
     where.need(p.q, "q");
     where.need(p.k, "k");
     where.need(p.v, "v");

@@ -724,7 +724,7 @@ __global__ void __launch_bounds__(256) delta_fold_kernel(const Args p) {
 template <typename T, int DKP, int KS>
 void reverse_as(const Args& a, cudaStream_t stream) {
     using Sh = ReverseShared<T, DKP, KS>;
-    opt_in(delta_reverse_kernel<T, DKP, KS>, sizeof(Sh));
+    opt_in<delta_reverse_kernel<T, DKP, KS>>(sizeof(Sh));
     const dim3 grid((a.dvp / 16 + Sh::kGroups - 1) / Sh::kGroups, a.value_heads, a.seqs);
     delta_reverse_kernel<T, DKP, KS><<<grid, kReverseThreads, sizeof(Sh), stream>>>(a);
     cuda_check(cudaGetLastError(), "delta rule states backward");
@@ -733,7 +733,7 @@ void reverse_as(const Args& a, cudaStream_t stream) {
 template <typename T, int DKP>
 void backward_as(const Args& a, cudaStream_t stream, int sm_count) {
     if (a.chunks) {
-        opt_in(delta_do_kernel<T, DKP>, sizeof(DoShared<T, DKP>));
+        opt_in<delta_do_kernel<T, DKP>>(sizeof(DoShared<T, DKP>));
         delta_do_kernel<T, DKP><<<dim3(a.chunks, a.value_heads), kDoThreads, sizeof(DoShared<T, DKP>), stream>>>(a);
         cuda_check(cudaGetLastError(), "delta rule P^T dO");
     }
@@ -745,7 +745,7 @@ void backward_as(const Args& a, cudaStream_t stream, int sm_count) {
     else if (chains <= 2 * (uint64_t)sm_count || a.sequences) reverse_as<T, DKP, 2>(a, stream);
     else reverse_as<T, DKP, 1>(a, stream);
     if (a.chunks) {
-        opt_in(delta_grad_kernel<T, DKP>, sizeof(GradShared<T, DKP>));
+        opt_in<delta_grad_kernel<T, DKP>>(sizeof(GradShared<T, DKP>));
         delta_grad_kernel<T, DKP><<<dim3(a.chunks + (a.sequences ? 1 : 0), a.value_heads), kGradThreads, sizeof(GradShared<T, DKP>), stream>>>(a);
         cuda_check(cudaGetLastError(), "delta rule gradients");
         if (a.value_heads != a.heads) {

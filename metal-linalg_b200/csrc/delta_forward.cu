@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(kOutThreads, 2) delta_output_kernel(const Args
 template <typename T, int DKP>
 void prepare_as(const Args& a, cudaStream_t stream, bool backward) {
     const size_t bytes = sizeof(PrepShared<T, DKP>);
-    opt_in(delta_prep_kernel<T, DKP>, bytes);
+    opt_in<delta_prep_kernel<T, DKP>>(bytes);
     delta_prep_kernel<T, DKP><<<dim3(a.chunks, a.value_heads), kPrepThreads, bytes, stream>>>(a, backward);
     cuda_check(cudaGetLastError(), "delta rule preparation");
 }
@@ -583,7 +583,7 @@ void prepare_as(const Args& a, cudaStream_t stream, bool backward) {
 template <typename T, int DKP, int KS>
 void states_as(const Args& a, cudaStream_t stream) {
     using Sh = StateShared<T, DKP, KS>;
-    opt_in(delta_state_kernel<T, DKP, KS>, sizeof(Sh));
+    opt_in<delta_state_kernel<T, DKP, KS>>(sizeof(Sh));
     const dim3 grid((a.dvp / 16 + Sh::kGroups - 1) / Sh::kGroups, a.value_heads, a.seqs);
     delta_state_kernel<T, DKP, KS><<<grid, kStateThreads, sizeof(Sh), stream>>>(a);
     cuda_check(cudaGetLastError(), "delta rule states");
@@ -601,7 +601,7 @@ void states_of(const Args& a, cudaStream_t stream, int sm_count) {
 template <typename T, int DKP>
 void output_as(const Args& a, cudaStream_t stream) {
     const size_t bytes = sizeof(OutShared<T, DKP>);
-    opt_in(delta_output_kernel<T, DKP>, bytes);
+    opt_in<delta_output_kernel<T, DKP>>(bytes);
     // one block more than there can be chunks: a ragged batch's tokens behind the last sequence have a block to clear them
     delta_output_kernel<T, DKP><<<dim3(a.chunks + (a.sequences ? 1 : 0), a.value_heads), kOutThreads, bytes, stream>>>(a);
     cuda_check(cudaGetLastError(), "delta rule outputs");

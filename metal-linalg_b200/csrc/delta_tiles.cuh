@@ -464,10 +464,14 @@ __device__ __forceinline__ int own_tile(int part, int i) {
 // Launches
 // ---------------------------------------------------------------------------
 
-// More than 48 KB of shared memory (recorded per GPU, and cheap, so it is not remembered).
-template <typename K>
-void opt_in(K kernel, size_t bytes) {
-    cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "delta rule shared memory");
+// More than 48 KB of shared memory, recorded per GPU and kernel.
+template <auto kKernel>
+void opt_in(size_t bytes) {
+    static PerDeviceOnce once;
+    if (const int device = current_device(); once.first(device)) {
+        cuda_check(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "delta rule shared memory");
+        once.mark(device);
+    }
 }
 
 // F<T, DKP> for the problem's type and width.

@@ -17,21 +17,31 @@ namespace {
 bool is_fp8(uint32_t kind) { return kind == METAL_LINALG_FLOAT8_E4M3 || kind == METAL_LINALG_FLOAT8_E5M2; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-int place(const char* who, const void* p, const char* name, int device) {
-    if (!p) refuse(who, std::string(name) + " is NULL");
-    const int d = mlb::pointer_device(p);
-    if (d < 0) refuse(who, std::string(name) + " is not a device pointer");
-    if (device >= 0 && d != device) refuse(who, std::string(name) + " lives on another GPU than the rest");
-    return d;
-}
+// Where a call's pointers live: the device its caller vouches for, or what each of them is found to be on.
+struct Place {
+    const char* who;
+    int  device;
+    bool known;
+    Place(const char* w, int d) : who(w), device(d), known(d >= 0) {
+        if (d < -1) refuse(w, "device must be a GPU or -1");
+    }
+    void need(const void* p, const char* name) {
+        if (!p) refuse(who, std::string(name) + " is NULL");
+        if (known) return;
+        const int d = mlb::pointer_device(p);
+        if (d < 0) refuse(who, std::string(name) + " is not a device pointer");
+        if (device >= 0 && d != device) refuse(who, std::string(name) + " lives on another GPU than the rest");
+        device = d;
+    }
+};
 
-mlb::fp8::GemmOperand operand(const char* who, const char* name, const metal_linalg_fp8_operand& o, uint32_t rows, uint32_t k,
-                              uint32_t batch, int& device) {
-    const std::string n(name);
+mlb::fp8::GemmOperand operand(Place& where, char name, const metal_linalg_fp8_operand& o, uint32_t rows, uint32_t k, uint32_t batch) {
+    const char* who = where.who;
+    const std::string n(1, name);
     if (!is_fp8(o.kind)) refuse(who, n + ".kind must be METAL_LINALG_FLOAT8_E4M3 or _E5M2");
     if (o.block_rows != 1 && o.block_rows != 128) refuse(who, n + ".block_rows must be 1 or 128");
-    device = place(who, o.values, (n + ".values").c_str(), device);
-    device = place(who, o.scales, (n + ".scales").c_str(), device);
+    where.need(o.values, name == 'a' ? "a.values" : "b.values");
+    where.need(o.scales, name == 'a' ? "a.scales" : "b.scales");
     if (!aligned16(o.values) || o.stride % 16 || o.batch_stride % 16)
         refuse(who, n + ".values and its strides must be multiples of 16 bytes");
     if (o.stride < k) refuse(who, n + ".stride is smaller than a row");
@@ -45,7 +55,7 @@ mlb::fp8::GemmOperand operand(const char* who, const char* name, const metal_lin
 
 void quantize_fp8(const void* x, uint32_t dtype, uint32_t batch, uint32_t rows, uint32_t cols, int64_t batch_stride,
                   int64_t row_stride, int64_t col_stride, uint32_t block_rows, uint32_t kind, void* values, uint64_t values_stride,
-                  float* scales) {
+                  float* scales, int device) {
     const char* who = "[quantize_fp8]";
     if (dtype > METAL_LINALG_FLOAT16) refuse(who, "dtype must be float32, bfloat16 or float16");
     if (!is_fp8(kind)) refuse(who, "kind must be METAL_LINALG_FLOAT8_E4M3 or _E5M2");
@@ -58,9 +68,10 @@ void quantize_fp8(const void* x, uint32_t dtype, uint32_t batch, uint32_t rows, 
         refuse(who, "rows and cols must be below 2^30, and the matrix below 2^38 elements");
     if (!aligned16(values) || values_stride % 16 || values_stride < cols)
         refuse(who, "values must be on a 16-byte boundary, its rows a multiple of 16 bytes apart and no shorter than cols");
-    int device = place(who, x, "x", -1);
-    device = place(who, values, "values", device);
-    device = place(who, scales, "scales", device);
+    Place where(who, device);
+    where.need(x, "x");
+    where.need(values, "values");
+    where.need(scales, "scales");
     const int64_t size = dtype == METAL_LINALG_FLOAT32 ? 4 : 2;
     const int64_t across = col_stride == 1 ? row_stride : col_stride;
     mlb::fp8::QuantizeArgs a{};
@@ -72,27 +83,28 @@ void quantize_fp8(const void* x, uint32_t dtype, uint32_t batch, uint32_t rows, 
     a.values_stride = values_stride;
     a.values_batch = values_stride * rows;
     a.scales = scales;
-    mlb::DeviceGuard guard(device);
+    mlb::DeviceGuard guard(where.device);
     mlb::fp8::launch_quantize(a, dtype, kind == METAL_LINALG_FLOAT8_E5M2, mlb::thread_stream());
 }
 
 void matmul_fp8(const metal_linalg_fp8_operand& a, const metal_linalg_fp8_operand& b, uint32_t batch, uint32_t m, uint32_t n,
-                uint32_t k, void* c, uint32_t c_dtype) {
+                uint32_t k, void* c, uint32_t c_dtype, int device) {
     const char* who = "[matmul_fp8]";
     if (c_dtype > METAL_LINALG_FLOAT16) refuse(who, "c must be float32, bfloat16 or float16");
     if (cpu_only()) throw std::runtime_error(std::string(who) + " this thread is set CPU-only, and this build has no CPU path");
     if (batch == 0 || m == 0 || n == 0) return;
     if (m >= 1u << 30 || n >= 1u << 30 || k >= 1u << 30) refuse(who, "m, n and k must be below 2^30");
-    int device = place(who, c, "c", -1);
+    Place where(who, device);
+    where.need(c, "c");
     if (k == 0) {
-        mlb::DeviceGuard guard(device);
+        mlb::DeviceGuard guard(where.device);
         mlb::cuda_check(cudaMemsetAsync(c, 0, (size_t)batch * m * n * (c_dtype == METAL_LINALG_FLOAT32 ? 4 : 2), mlb::thread_stream()),
                         "cudaMemsetAsync");
         return;
     }
-    const auto oa = operand(who, "a", a, m, k, batch, device), ob = operand(who, "b", b, n, k, batch, device);
-    mlb::DeviceGuard guard(device);
-    mlb::fp8::launch_gemm(mlb::thread_stream(), device, oa, ob, batch, k, c, c_dtype, mlb::context(device).status);
+    const auto oa = operand(where, 'a', a, m, k, batch), ob = operand(where, 'b', b, n, k, batch);
+    mlb::DeviceGuard guard(where.device);
+    mlb::fp8::launch_gemm(mlb::thread_stream(), where.device, oa, ob, batch, k, c, c_dtype, mlb::status_word(where.device));
 }
 
 } // namespace core

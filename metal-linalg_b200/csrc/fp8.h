@@ -44,9 +44,9 @@ namespace core {
 // What the C entry points of the same names do (fp8.cpp); std::invalid_argument for what they refuse.
 void quantize_fp8(const void* x, uint32_t dtype, uint32_t batch, uint32_t rows, uint32_t cols, int64_t batch_stride,
                   int64_t row_stride, int64_t col_stride, uint32_t block_rows, uint32_t kind, void* values, uint64_t values_stride,
-                  float* scales);
+                  float* scales, int device);
 void matmul_fp8(const metal_linalg_fp8_operand& a, const metal_linalg_fp8_operand& b, uint32_t batch, uint32_t m, uint32_t n,
-                uint32_t k, void* c, uint32_t c_dtype);
+                uint32_t k, void* c, uint32_t c_dtype, int device);
 
 } // namespace core
 } // namespace metal_linalg

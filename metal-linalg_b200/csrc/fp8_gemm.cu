@@ -514,8 +514,12 @@ CUtensorMap tile_map(const GemmOperand& o, uint32_t batch, uint32_t k, uint32_t 
 template <int BN, bool kByColumn>
 void gemm_as(cudaStream_t stream, const CUtensorMap& mp, const CUtensorMap& mq, const GemmArgs& a, int sm_count) {
     using S = Shape<BN>;
-    cuda_check(cudaFuncSetAttribute(fp8_gemm_kernel<BN, kByColumn>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kShared),
-               "fp8 product shared memory");
+    static PerDeviceOnce once;          // the opt-in is recorded per GPU
+    if (const int device = current_device(); once.first(device)) {
+        cuda_check(cudaFuncSetAttribute(fp8_gemm_kernel<BN, kByColumn>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kShared),
+                   "fp8 product shared memory");
+        once.mark(device);
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.split > 1 ? a.tiles * a.split : std::min<uint32_t>(a.tiles, (uint32_t)sm_count));
     cfg.blockDim = dim3(S::kThreads);

@@ -308,8 +308,12 @@ void quantize_as(const QuantizeArgs& a, cudaStream_t stream) {
     const uint64_t blocks = (a.cols + kB - 1) / kB, tiles = (a.rows + kB - 1) / kB * blocks;
     if (a.col_stride != 1) {
         const size_t bytes = sizeof(T) * kB * kB;
-        cuda_check(cudaFuncSetAttribute(quantize_turned_kernel<T, kE5m2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
-                   "quantize shared memory");
+        static PerDeviceOnce once;          // the opt-in is recorded per GPU
+        if (const int device = current_device(); once.first(device)) {
+            cuda_check(cudaFuncSetAttribute(quantize_turned_kernel<T, kE5m2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
+                       "quantize shared memory");
+            once.mark(device);
+        }
         quantize_turned_kernel<T, kE5m2><<<dim3((unsigned)tiles, a.batch), kThreads, bytes, stream>>>(a);
     } else if (a.block_rows == 1) {
         // four blocks of 128 a thread where that still leaves every multiprocessor two thread blocks

@@ -49,6 +49,14 @@ int sm_count(int device) {
     return n;
 }
 
+unsigned* status_word(int device) {
+    static std::atomic<unsigned*> known[64];
+    std::atomic<unsigned*>& slot = known[device & 63];
+    unsigned* word = slot.load(std::memory_order_acquire);
+    if (!word) slot.store(word = context(device).status, std::memory_order_release);
+    return word;
+}
+
 DeviceGuard::DeviceGuard(int device) {
     cuda_check(cudaGetDevice(&previous_), "cudaGetDevice");
     if (device != previous_) cuda_check(cudaSetDevice(device), "cudaSetDevice");

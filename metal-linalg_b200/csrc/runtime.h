@@ -99,6 +99,7 @@ private:
 
 int            device_count();
 int            sm_count(int device);          // multiprocessors; asked of the driver once per GPU, creates no context
+unsigned*      status_word(int device);       // context(device).status, looked up once per GPU
 DeviceContext& context(int device);   // created on first use; throws without a GPU
 
 // Launches `kernel`, whose first statement is dependency_wait() (common.cuh), so that it may be

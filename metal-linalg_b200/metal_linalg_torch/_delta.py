@@ -24,7 +24,7 @@ __all__ = ["gated_delta_rule", "gated_delta_step"]
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _FLOATING = frozenset((torch.float32, torch.bfloat16, torch.float16, torch.float64))
 _PLACES = frozenset(("cuda", "meta"))
-_PROBLEM = struct.Struct("=9If7Q15q")
+_PROBLEM = struct.Struct("=9IfiI7Q15q")
 
 
 def _fail(name, message, kind=ValueError):
@@ -97,7 +97,7 @@ def _problem(q, k, v, g, beta, scale, initial=None, cu=None, index_bytes=4):
     k0, k1, k2, _ = k.stride()
     v0, v1, v2, _ = v.stride()
     return _PROBLEM.pack(b, t, h, hv, dk, dv, 0 if cu is None else cu.numel() - 1, _DTYPES[q.dtype], index_bytes, scale,
-                         q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+                         q.get_device(), 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
                          0 if initial is None else initial.data_ptr(), 0 if cu is None else cu.data_ptr(),
                          q0, q1, q2, k0, k1, k2, v0, v1, v2, *g.stride(), *beta.stride())
 

@@ -65,9 +65,9 @@ def _quantize(x, block_rows, transpose, dtype):
         x = x.contiguous()
         across = x.stride(0) if x.dim() == 3 else 0
         rows, cols = (1, m) if transpose else (n, 1)
-    _lib.use_stream_of(x)
+    device = _lib.use_stream_of(x)
     _lib.check(_lib.lib.metal_linalg_quantize_fp8(x.data_ptr(), _DTYPES[x.dtype], batch, m, n, across, rows, cols, block_rows,
-                                                  _KINDS[dtype], values.data_ptr(), -(-n // 16) * 16, scales.data_ptr()))
+                                                  _KINDS[dtype], values.data_ptr(), -(-n // 16) * 16, scales.data_ptr(), device))
     return values, scales
 
 
@@ -156,8 +156,8 @@ def _matmul(a, a_scale, b, b_scale, a_rows, b_rows, out_dtype):
             a, m, batch = a.flatten(0, 1), batch * m, 1      # one matrix for the whole batch: the rows behind one another
     pa, keep_a = _operand(a, a_scale, a_rows, batch > 1)
     pb, keep_b = _operand(b, b_scale, b_rows, batch > 1 and b.dim() == 3)
-    _lib.use_stream_of(out)
-    _lib.check(_lib.lib.metal_linalg_matmul_fp8(pa, pb, batch, m, n, k, out.data_ptr(), _DTYPES[out_dtype]))
+    device = _lib.use_stream_of(out)
+    _lib.check(_lib.lib.metal_linalg_matmul_fp8(pa, pb, batch, m, n, k, out.data_ptr(), _DTYPES[out_dtype], device))
     return out
 
 

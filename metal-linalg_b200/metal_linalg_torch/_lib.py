@@ -49,8 +49,8 @@ def _load():
         "metal_linalg_gated_delta_rule_backward": (ctypes.c_int, [_ptr] * 11 + [_u64]),
         "metal_linalg_gated_delta_step": (ctypes.c_int, [_ptr, _ptr, _ptr, ctypes.c_int64, _u32, _ptr]),
         "metal_linalg_quantize_fp8": (ctypes.c_int, [_ptr, ctypes.c_int, _u32, _u32, _u32] + [ctypes.c_int64] * 3 +
-                                      [_u32, ctypes.c_int, _ptr, _u64, _ptr]),
-        "metal_linalg_matmul_fp8": (ctypes.c_int, [_ptr, _ptr, _u32, _u32, _u32, _u32, _ptr, ctypes.c_int]),
+                                      [_u32, ctypes.c_int, _ptr, _u64, _ptr, ctypes.c_int]),
+        "metal_linalg_matmul_fp8": (ctypes.c_int, [_ptr, _ptr, _u32, _u32, _u32, _u32, _ptr, ctypes.c_int, ctypes.c_int]),
         "metal_linalg_set_stream": (None, [_ptr]),
         "metal_linalg_stream": (_ptr, []),
         "metal_linalg_set_device": (ctypes.c_int, [ctypes.c_int]),
@@ -106,13 +106,15 @@ _raw_stream = None
 
 
 def use_stream_of(x):
-    """Sets this thread's stream to torch's current one on tensor x's device (the kernels run on the pointers' device,
-    whichever is current)."""
+    """Sets this thread's stream to torch's current one on tensor x's device, and returns that device's number (the kernels
+    run on the pointers' device, whichever is current)."""
     global _raw_stream
     if _raw_stream is None:
         import torch
         _raw_stream = torch._C._cuda_getCurrentRawStream
-    lib.metal_linalg_set_stream(_raw_stream(x.get_device()))
+    device = x.get_device()
+    lib.metal_linalg_set_stream(_raw_stream(device))
+    return device
 
 
 def qr(a, batch, rows, cols, q, r, mode="reduced", stream=None):

@@ -138,8 +138,8 @@ def test_c_entries_refuse_without_a_gpu():
     from metal_linalg_torch._delta import _PROBLEM
     lib = _lib.lib
 
-    def problem(b=1, t=4, h=1, hv=1, dk=8, dv=8, seqs=0, dtype=0, index=4, ptr=0):
-        return _PROBLEM.pack(b, t, h, hv, dk, dv, seqs, dtype, index, 1.0, *[ptr] * 7, *[0] * 15)
+    def problem(b=1, t=4, h=1, hv=1, dk=8, dv=8, seqs=0, dtype=0, index=4, ptr=0, device=-1):
+        return _PROBLEM.pack(b, t, h, hv, dk, dv, seqs, dtype, index, 1.0, device, 0, *[ptr] * 7, *[0] * 15)
 
     size = lib.metal_linalg_gated_delta_rule_workspace_bytes
     assert size(problem(), 0) > 0 and size(problem(), 1) > size(problem(), 0)
@@ -155,6 +155,7 @@ def test_c_entries_refuse_without_a_gpu():
     assert lib.metal_linalg_gated_delta_rule(problem(ptr=host.ctypes.data), None, None, None, 0) == _lib.INVALID_ARGUMENT
     assert "device pointer" in _lib.last_error()
     assert lib.metal_linalg_gated_delta_step(problem(ptr=host.ctypes.data), host.ctypes.data, host.ctypes.data, 64, 1, None) == _lib.INVALID_ARGUMENT
+    assert lib.metal_linalg_gated_delta_rule(problem(device=-2), None, None, None, 0) == _lib.INVALID_ARGUMENT
     assert lib.metal_linalg_gated_delta_rule(problem(t=0), None, None, None, 0) == _lib.OK       # nothing to do, nowhere to put it
     with mlt.CpuOnly():
         assert lib.metal_linalg_gated_delta_rule(problem(), None, None, None, 0) == _lib.RUNTIME_ERROR

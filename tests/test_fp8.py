@@ -102,17 +102,17 @@ def test_c_entries_refuse_without_a_gpu():
     lib = _lib.lib
     host = np.zeros(4096, np.float32)
     at = (host.ctypes.data + 15) // 16 * 16
-    quantize = lambda dtype=0, rows=4, cols=8, strides=(32, 8, 1), block=1, kind=3, values=at, stride=16: lib.metal_linalg_quantize_fp8(  # noqa: E731
-        at, dtype, 1, rows, cols, *strides, block, kind, values, stride, at)
+    quantize = lambda dtype=0, rows=4, cols=8, strides=(32, 8, 1), block=1, kind=3, values=at, stride=16, device=-1: lib.metal_linalg_quantize_fp8(  # noqa: E731
+        at, dtype, 1, rows, cols, *strides, block, kind, values, stride, at, device)
     for bad in (dict(dtype=3), dict(kind=0), dict(block=2), dict(strides=(32, 8, 2)), dict(values=at + 4), dict(stride=24), dict(stride=0),
-                dict(rows=1 << 30), {}):                    # the last: host pointers
+                dict(rows=1 << 30), dict(device=-2), {}):   # the last: host pointers
         assert quantize(**bad) == _lib.INVALID_ARGUMENT and "[quantize_fp8]" in _lib.last_error()
     assert quantize(rows=0) == _lib.OK
     operand = lambda values=at, scales=at, stride=128, across=0, kind=3, block=1: _OPERAND.pack(values, scales, stride, across, kind, block)  # noqa: E731
-    matmul = lambda a=operand(), b=operand(), m=4, k=128, dtype=0: lib.metal_linalg_matmul_fp8(a, b, 1, m, 4, k, at, dtype)  # noqa: E731
+    matmul = lambda a=operand(), b=operand(), m=4, k=128, dtype=0: lib.metal_linalg_matmul_fp8(a, b, 1, m, 4, k, at, dtype, -1)  # noqa: E731
     for bad in (dict(dtype=3), dict(m=1 << 30), {}):
         assert matmul(**bad) == _lib.INVALID_ARGUMENT and "[matmul_fp8]" in _lib.last_error()
-    assert lib.metal_linalg_matmul_fp8(None, operand(), 1, 4, 4, 128, at, 0) == _lib.INVALID_ARGUMENT
+    assert lib.metal_linalg_matmul_fp8(None, operand(), 1, 4, 4, 128, at, 0, -1) == _lib.INVALID_ARGUMENT
     assert matmul(m=0) == _lib.OK
     with mlt.CpuOnly():
         assert matmul() == _lib.RUNTIME_ERROR and quantize() == _lib.RUNTIME_ERROR
