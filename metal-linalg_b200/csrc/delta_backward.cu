@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kDoThreads) delta_do_kernel(const Args p) {
 //
 // The forward's chain with dS'^T in the accumulators: Y^T = dS'^T K^T, dD^T = e^{G_63 - G} Y^T + (scale P^T dO)^T,
 // dR^T = dD^T T, dS^T = e^{G_63} dS'^T + (scale e^G dO)^T Q - (beta e^G dR)^T K.
-constexpr int kReverseThreads = 160;
+constexpr int kReverseThreads = 192;      // two fetching warps, as the forward's
 
 template <typename T, int DKP, int KS>
 struct ReverseShared {
@@ -136,19 +136,20 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
         c0 = seq * p.row_chunks;
         c1 = c0 + p.row_chunks;
     }
-    if (warp == 4) {
+    if (warp >= 4) {
+        const int tid = threadIdx.x - 128;
         const auto fetch = [&](uint32_t c, int which) {
             typename Sh::Stage& st = sh.stage[which];
             const Chunk ch = chunk_at(p, c);
             const size_t at = (size_t)c * p.value_heads + hv;
-            load_rows<T, 32, DKP>(st.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, lane);
-            load_rows<T, 32, DKP>(st.q, LD, p.q, at3(p.q_stride, ch.batch, ch.token, h), p.q_stride[1], ch.rows, (int)p.dk, p.vec, lane);
-            load_rows<T, 32, 16 * Sh::kGroups>(st.d_o, LDV, p.d_o, at3(p.do_stride, ch.batch, ch.token, hv) + dv_block, p.do_stride[1],
-                                               ch.rows, (int)p.dv - dv_block, p.vec, lane);
-            load_rows<float, 32, 16 * Sh::kGroups>(st.dd, LDV, p.dr, (long long)(at * kChunk * p.dvp) + dv_block, p.dvp, kChunk,
-                                                   (int)p.dvp - dv_block, true, lane);
-            load_floats<32, kTriFloats>(st.tri, p.tri_b + at * kTriFloats, lane);
-            load_floats<32, 3 * kChunk>(st.gates, p.gates[at].e, lane);
+            load_rows<T, 64, DKP>(st.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, tid);
+            load_rows<T, 64, DKP>(st.q, LD, p.q, at3(p.q_stride, ch.batch, ch.token, h), p.q_stride[1], ch.rows, (int)p.dk, p.vec, tid);
+            load_rows<T, 64, 16 * Sh::kGroups>(st.d_o, LDV, p.d_o, at3(p.do_stride, ch.batch, ch.token, hv) + dv_block, p.do_stride[1],
+                                               ch.rows, (int)p.dv - dv_block, p.vec, tid);
+            load_rows<float, 64, 16 * Sh::kGroups>(st.dd, LDV, p.dr, (long long)(at * kChunk * p.dvp) + dv_block, p.dvp, kChunk,
+                                                   (int)p.dvp - dv_block, true, tid);
+            load_floats<64, kTriFloats>(st.tri, p.tri_b + at * kTriFloats, tid);
+            load_floats<64, 3 * kChunk>(st.gates, p.gates[at].e, tid);
             cp_commit();
         };
         if (Sh::kStages == 2 && c0 < c1) fetch(c1 - 1, 0);

@@ -232,8 +232,10 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const Args p, 
 // D^T = R^T T^T; S^T = e^{G_63} S^T + (D^T e^{G_63 - G}) K: every product's accumulators are the next one's A operand, and K
 // comes from shared memory as B operands both ways round. KS warps share a chain, each with dk / KS of S's rows, since a
 // chain is a sequence of dependent products and there are few chains; partial X crosses through shared memory as whole fragments (a lane's 16 bytes, no bank
-// met twice), R and D already in their parts. A fifth warp fetches the next chunk meanwhile.
-constexpr int kStateThreads = 160;
+// met twice), R and D already in their parts. Two more warps fetch the next chunk meanwhile (one took longer to issue its copies than the
+// chain to use them). A chain is alone on its quarter of the multiprocessor, so what a product needs besides the one before it
+// is read ahead of the barrier that opens it.
+constexpr int kStateThreads = 192;
 
 template <typename T, int DKP, int KS>
 struct StateShared {
@@ -251,7 +253,7 @@ struct StateShared {
 };
 
 template <typename T, int DKP, int KS>
-__global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p) {
+__global__ void __launch_bounds__(kStateThreads, sizeof(T) == 2 ? 2 : 1) delta_state_kernel(const Args p) {
     using Sh = StateShared<T, DKP, KS>;
     using Sp = typename Split<T>::type;
     using Tile = typename Split<T>::tile;
@@ -269,16 +271,17 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
         c0 = seq * p.row_chunks;
         c1 = c0 + p.row_chunks;
     }
-    if (warp == 4) {            // the fetching warp: a chunk ahead, complete at the barrier that opens it
+    if (warp >= 4) {            // the fetching warps: a chunk ahead, complete at the barrier that opens it
+        const int tid = threadIdx.x - 128;
         const auto fetch = [&](uint32_t c, int which) {
             typename Sh::Stage& st = sh.stage[which];
             const Chunk ch = chunk_at(p, c);
             const size_t at = (size_t)c * p.value_heads + hv;
-            load_rows<T, 32, DKP>(st.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, lane);
-            load_rows<T, 32, 16 * Sh::kGroups>(st.v, Sh::kLdV, p.v, at3(p.v_stride, ch.batch, ch.token, hv) + dv_block, p.v_stride[1],
-                                               ch.rows, (int)p.dv - dv_block, p.vec, lane);
-            load_floats<32, kTriFloats>(st.tri, p.tri + at * kTriFloats, lane);
-            load_floats<32, 3 * kChunk>(st.gates, p.gates[at].e, lane);
+            load_rows<T, 64, DKP>(st.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, tid);
+            load_rows<T, 64, 16 * Sh::kGroups>(st.v, Sh::kLdV, p.v, at3(p.v_stride, ch.batch, ch.token, hv) + dv_block, p.v_stride[1],
+                                               ch.rows, (int)p.dv - dv_block, p.vec, tid);
+            load_floats<64, kTriFloats>(st.tri, p.tri + at * kTriFloats, tid);
+            load_floats<64, 3 * kChunk>(st.gates, p.gates[at].e, tid);
             cp_commit();
         };
         if (c0 < c1) fetch(c0, 0);
@@ -325,18 +328,48 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
             }
         }
 
+        // X^T, the next k's operands on their way while one is multiplied
         float x[8][4] = {};
+        {
+            Columns<T, 8, false> f[2];
+            f[0].load(st.k, LD, 0, k_base);
 #pragma unroll
-        for (int kk = 0; kk < NT / 2; ++kk) {
-            Sp a;
-            a.set(s[2 * kk], s[2 * kk + 1]);
-            mma_tile<T, 8, false>(x, a, st.k, LD, 0, k_base + 16 * kk);
+            for (int kk = 0; kk < NT / 2; ++kk) {
+                if (kk + 1 < NT / 2) f[(kk + 1) & 1].load(st.k, LD, 0, k_base + 16 * (kk + 1));
+                Sp a;
+                a.set(s[2 * kk], s[2 * kk + 1]);
+                mma_columns<T, 8, false>(x, a, f[kk & 1]);
+            }
         }
 #pragma unroll
         for (int n = 0; n < 8; ++n)
             *reinterpret_cast<float4*>(sh.part + (warp * 8 + n) * 32 + lane) = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
+        // what R and D of this warp's token tiles need besides
+        float value[kOwn][4];
+        float2 beta2[kOwn], e2[kOwn], left2[kOwn], t_lo[kOwn / 2][4], t_hi[kOwn / 2][8];
+        const float2* tri = reinterpret_cast<const float2*>(st.tri) + lane;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            const int n = own_tile<KS>(part, i);
+            const T* v = st.v + (8 * n + 2 * t) * Sh::kLdV + 16 * chain + g;
+            value[i][0] = to_f(v[0]);
+            value[i][1] = to_f(v[Sh::kLdV]);
+            value[i][2] = to_f(v[8]);
+            value[i][3] = to_f(v[Sh::kLdV + 8]);
+            beta2[i] = *reinterpret_cast<const float2*>(beta + 8 * n + 2 * t);
+            e2[i] = *reinterpret_cast<const float2*>(e + 8 * n + 2 * t);
+            left2[i] = *reinterpret_cast<const float2*>(left + 8 * n + 2 * t);
+        }
+        // T's tiles: own_tile's first half lies in rows 0-3, the second in rows 4-7; those past the diagonal are not used
+#pragma unroll
+        for (int i = 0; i < kOwn / 2; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t_lo[i][j] = tri[tri_tile(own_tile<KS>(part, i), min(j, own_tile<KS>(part, i))) * 32];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                t_hi[i][j] = tri[tri_tile(own_tile<KS>(part, kOwn / 2 + i), min(j, own_tile<KS>(part, kOwn / 2 + i))) * 32];
+        }
         asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
-        // R for this warp's token tiles
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
             const int n = own_tile<KS>(part, i);
@@ -347,46 +380,62 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
                 const float u[4] = {q.x, q.y, q.z, q.w};
                 add_to(f, u);
             }
-            const float2 be = *reinterpret_cast<const float2*>(beta + 8 * n + 2 * t), ee = *reinterpret_cast<const float2*>(e + 8 * n + 2 * t);
-            const T* v = st.v + (8 * n + 2 * t) * Sh::kLdV + 16 * chain + g;
-            f[0] = be.x * fmaf(-ee.x, f[0], to_f(v[0]));
-            f[1] = be.y * fmaf(-ee.y, f[1], to_f(v[Sh::kLdV]));
-            f[2] = be.x * fmaf(-ee.x, f[2], to_f(v[8]));
-            f[3] = be.y * fmaf(-ee.y, f[3], to_f(v[Sh::kLdV + 8]));
+            f[0] = beta2[i].x * fmaf(-e2[i].x, f[0], value[i][0]);
+            f[1] = beta2[i].y * fmaf(-e2[i].y, f[1], value[i][1]);
+            f[2] = beta2[i].x * fmaf(-e2[i].x, f[2], value[i][2]);
+            f[3] = beta2[i].y * fmaf(-e2[i].y, f[3], value[i][3]);
             TileTf32 a;
             a.set(f);
             a.put(r_parts, n, lane);
         }
         asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
-        // D^T = R^T T^T, a k of 8 at a time against the rows of T that reach it
+        // D^T = R^T T^T, two k's of 8 at a time against the rows of T that reach them
         float d[kOwn][4] = {};
-        const float2* tri = reinterpret_cast<const float2*>(st.tri) + lane;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            TileTf32 a;
-            a.get(r_parts, j, lane);
-            // of a pair of tiles one lies above row 4 and one below: which products there are is mostly known
-            mma_triangle(d, a, [&](int i) { return i < kOwn / 2 ? j < 4 && own_tile<KS>(part, i) >= j
-                                                                   : j <= 4 || own_tile<KS>(part, i) >= j; },
-                         [&](int i) { return tri[tri_tile(own_tile<KS>(part, i), j) * 32]; });
+        for (int j = 0; j < 8; j += 2) {
+            TileTf32 a[2];
+            a[0].get(r_parts, j, lane);
+            a[1].get(r_parts, j + 1, lane);
+            float c[2][kOwn][4];
+            uint4 b[2][kOwn];
+            const auto wanted = [&](int i, int u) {     // mostly known beforehand
+                return i < kOwn / 2 ? u < 4 && own_tile<KS>(part, i) >= u : u <= 4 || own_tile<KS>(part, i) >= u;
+            };
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i)
+                    if (wanted(i, j + u)) {
+                        const float2 f = i < kOwn / 2 ? t_lo[i][(j + u) & 3] : t_hi[i - kOwn / 2][j + u];
+                        b[u][i] = split_pair(f.x, f.y);
+                        mma_term8<0>(c[u][i], a[u], b[u][i]);
+                    }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i)
+                    if (wanted(i, j + u)) mma_term8<1>(c[u][i], a[u], b[u][i]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i)
+                    if (wanted(i, j + u)) mma_term8<2>(c[u][i], a[u], b[u][i]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i)
+                    if (wanted(i, j + u)) add_to(d[i], c[u][i]);
         }
-        float* d_out = p.d + at * kChunk * p.dvp + (size_t)(2 * t) * p.dvp + dv0 + g;
+        // e^{G_63 - G} D to the chain's other warps, D itself to memory
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
-            const int n = own_tile<KS>(part, i);
-            if (live) {
-                float* out = d_out + (size_t)(8 * n) * p.dvp;
-                out[0] = d[i][0];
-                out[8] = d[i][2];
-                out[p.dvp] = d[i][1];
-                out[p.dvp + 8] = d[i][3];
-            }
-            const float2 le = *reinterpret_cast<const float2*>(left + 8 * n + 2 * t);
-            d[i][0] *= le.x; d[i][1] *= le.y; d[i][2] *= le.x; d[i][3] *= le.y;
+            const float f[4] = {d[i][0] * left2[i].x, d[i][1] * left2[i].y, d[i][2] * left2[i].x, d[i][3] * left2[i].y};
             Tile a;
-            a.set(d[i]);
-            a.put(d_parts, n, lane);
+            a.set(f);
+            a.put(d_parts, own_tile<KS>(part, i), lane);
         }
+        Columns<T, NT, true> f[2];
+        f[0].load(st.k, LD, k_base, 0);
         asm volatile("bar.sync %0, %1;" :: "r"(1 + chain), "n"(32 * KS) : "memory");
         // S' = e^{G_63} S + (e^{G_63 - G} K)^T D
         const float whole = e[kChunk - 1];
@@ -394,12 +443,24 @@ __global__ void __launch_bounds__(kStateThreads) delta_state_kernel(const Args p
         for (int n = 0; n < NT; ++n) scale_by(s[n], whole);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            if (j < 3) f[(j + 1) & 1].load(st.k, LD, k_base, 16 * (j + 1));
             Sp a;
             Tile u, v;
             u.get(d_parts, 2 * j, lane);
             v.get(d_parts, 2 * j + 1, lane);
             a.set(u, v);
-            mma_tile<T, NT, true>(s, a, st.k, LD, k_base, 16 * j);
+            mma_columns<T, NT, true>(s, a, f[j & 1]);
+        }
+        if (live) {
+            float* d_out = p.d + at * kChunk * p.dvp + (size_t)(2 * t) * p.dvp + dv0 + g;
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                float* out = d_out + (size_t)(8 * own_tile<KS>(part, i)) * p.dvp;
+                out[0] = d[i][0];
+                out[8] = d[i][2];
+                out[p.dvp] = d[i][1];
+                out[p.dvp + 8] = d[i][3];
+            }
         }
     }
     if (p.final_state)

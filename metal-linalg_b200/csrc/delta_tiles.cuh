@@ -256,33 +256,46 @@ __device__ __forceinline__ void load_b_cols(FragB<T> (&b)[2], const T* tile, int
     }
 }
 
-// acc[NT] += the float32 operand `a` times the tile's columns n0 .. n0 + 8 NT - 1, k0 .. k0 + 15. The tensor core cuts its
-// sums instead of rounding them, always towards zero, so every k of 16 is summed from nothing, smallest parts first, and
-// added in float32: with one accumulator all along the gradients were 2e-6 off, an error that grows with the number of
-// additions. Four columns' parts are issued in turn, so that a column's lie four apart (21 clocks of latency against 4 x 8.2).
+// The B operands of columns n0 .. n0 + 8 NT - 1, k0 .. k0 + 15 of a tile.
+template <typename T, int NT, bool kCols>
+struct Columns {
+    FragB<T> b[NT / 2][2];
+    __device__ __forceinline__ void load(const T* tile, int ld, int n0, int k0) {
+        static_assert(NT % 2 == 0, "columns come in pairs of eight");
+#pragma unroll
+        for (int j = 0; j < NT / 2; ++j) {
+            if constexpr (kCols) load_b_cols<T>(b[j], tile, ld, n0 + 16 * j, k0);
+            else                 load_b_rows<T>(b[j], tile, ld, n0 + 16 * j, k0);
+        }
+    }
+};
+// acc[n] += the float32 operand `a` times NT columns of eight. The tensor core cuts its sums instead of rounding them, always
+// towards zero, so every k of 16 is summed from nothing, smallest parts first, and added in float32: with one accumulator
+// all along the gradients were 2e-6 off, an error that grows with the number of additions. The columns' parts are
+// issued in turn, so that one's lie NT apart (21 clocks of latency against NT x 8.2).
+template <typename T, int NT, bool kCols>
+__device__ __forceinline__ void mma_columns(float (*acc)[4], const typename Split<T>::type& a, const Columns<T, NT, kCols>& f) {
+    float c[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) mma_term<0>(c[j], a, f.b[j / 2][j & 1]);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) mma_term<1>(c[j], a, f.b[j / 2][j & 1]);
+    if constexpr (Split<T>::kTerms == 3)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mma_term<2>(c[j], a, f.b[j / 2][j & 1]);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) add_to(acc[j], c[j]);
+}
+// acc[NT] += `a` times the tile's columns n0 .. n0 + 8 NT - 1, k0 .. k0 + 15, four columns of eight at a time.
 template <typename T, int NT, bool kCols>
 __device__ __forceinline__ void mma_tile(float (&acc)[NT][4], const typename Split<T>::type& a, const T* tile, int ld, int n0,
                                          int k0) {
     constexpr int kGroup = NT % 4 == 0 ? 4 : 2;
-    static_assert(NT % 2 == 0, "columns come in pairs of eight");
 #pragma unroll
     for (int n = 0; n < NT; n += kGroup) {
-        FragB<T> b[kGroup / 2][2];
-#pragma unroll
-        for (int j = 0; j < kGroup / 2; ++j) {
-            if constexpr (kCols) load_b_cols<T>(b[j], tile, ld, n0 + 8 * (n + 2 * j), k0);
-            else                 load_b_rows<T>(b[j], tile, ld, n0 + 8 * (n + 2 * j), k0);
-        }
-        float c[kGroup][4];
-#pragma unroll
-        for (int j = 0; j < kGroup; ++j) mma_term<0>(c[j], a, b[j / 2][j & 1]);
-#pragma unroll
-        for (int j = 0; j < kGroup; ++j) mma_term<1>(c[j], a, b[j / 2][j & 1]);
-        if constexpr (Split<T>::kTerms == 3)
-#pragma unroll
-            for (int j = 0; j < kGroup; ++j) mma_term<2>(c[j], a, b[j / 2][j & 1]);
-#pragma unroll
-        for (int j = 0; j < kGroup; ++j) add_to(acc[n + j], c[j]);
+        Columns<T, kGroup, kCols> f;
+        f.load(tile, ld, n0 + 8 * n, k0);
+        mma_columns<T, kGroup, kCols>(&acc[n], a, f);
     }
 }
 
