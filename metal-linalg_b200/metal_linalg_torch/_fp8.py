@@ -8,6 +8,7 @@
 A block of 128 along k is multiplied on the tensor cores, its product scaled and added in float32; the result is rounded
 once. Calls take CUDA tensors and enqueue on torch's current stream of the tensors' device.
 """
+import math
 import struct
 
 import torch
@@ -267,7 +268,7 @@ def linear_fp8(x, w):
         _fail(name, f"expected x [..., K] and w [N, K], got {tuple(x.shape)} and {tuple(w.shape)}")
     if w.device != x.device:
         _fail(name, f"w is on {w.device}, x on {x.device}")
-    flat = x.reshape(-1, x.shape[-1])
+    flat = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
     if torch.compiler.is_compiling() or x.device.type == "meta":
         y = torch.ops.metal_linalg.linear_fp8(flat, w)
     elif torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):

@@ -584,6 +584,83 @@ def test_compiled():
 
 
 @pytest.mark.gpu
+def test_compiled_step():
+    q, k, v, g, beta, s0 = inputs(3, 1, 1, 2, 32, 32, torch.bfloat16)
+    slots = torch.tensor([2, -1, 0], device="cuda")
+
+    def f(q, k, v, g, beta, state):
+        return mlt.gated_delta_step(q, k, v, g, beta, state, slots=slots) * 2
+
+    a, b = s0.clone(), s0.clone()
+    want = f(q, k, v, g, beta, a)
+    got = torch.compile(f, backend="aot_eager", fullgraph=True)(q, k, v, g, beta, b)
+    assert torch.equal(got, want) and torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once():
+    """The library's stream is the calling thread's: calls of several threads, each on its own stream, do not meet."""
+    import threading
+    calls = [inputs(1, 200 + 64 * i, 2, 2, 64, 64, torch.bfloat16, seed=i) for i in range(4)]
+    want = [mlt.gated_delta_rule(*c[:5], initial_state=c[5]) for c in calls]
+    torch.cuda.synchronize()
+    got = [None] * len(calls)
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = mlt.gated_delta_rule(*calls[i][:5], initial_state=calls[i][5])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for (a, b), (c, d) in zip(got, want):
+        assert torch.equal(a, c) and torch.equal(b, d)
+
+
+@pytest.mark.gpu
+def test_ragged_without_tokens():
+    q, k, v, g, beta, s0 = inputs(1, 0, 1, 2, 16, 24, torch.bfloat16, n=3)
+    cu = torch.zeros(4, dtype=torch.int32, device="cuda")
+    leaves = [x.requires_grad_() for x in (q, k, v, g, beta, s0)]
+    o, s = mlt.gated_delta_rule(*leaves[:5], initial_state=leaves[5], cu_seqlens=cu)
+    assert o.shape == (1, 0, 2, 24) and torch.equal(s, s0)
+    ds = torch.randn_like(s)
+    grads = torch.autograd.grad((o, s), leaves, (torch.zeros_like(o), ds))
+    assert torch.equal(grads[5], ds) and grads[0].shape == q.shape
+    o = mlt.gated_delta_step(*(x.detach()[:, :0] for x in leaves[:5]), s0.detach())
+    assert o.shape == (1, 0, 2, 24)
+
+
+@pytest.mark.gpu
+def test_expanded_gradients():
+    """sum().backward() hands in a gradient of stride 0."""
+    args = inputs(1, 70, 1, 1, 16, 16, torch.float32)
+    leaves = [x.detach().requires_grad_() for x in args]
+    o, s = mlt.gated_delta_rule(*leaves[:5], initial_state=leaves[5])
+    (o.sum() + s.sum()).backward()
+    for name, x, y in zip(NAMES, leaves, wanted_grads(args, torch.ones_like(o), torch.ones_like(s))):
+        near(x.grad, y, GRAD, name)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Tokens 2^26 elements apart: the last ones lie behind 2^31."""
+    q, k, v, g, beta, s0 = inputs(1, 40, 1, 1, 32, 32, torch.bfloat16)
+    far = torch.empty_strided((1, 40, 1, 32), (0, 1 << 26, 32, 1), dtype=torch.bfloat16, device="cuda")
+    want = mlt.gated_delta_rule(q, k, v, g, beta, initial_state=s0)
+    far.copy_(k)
+    got = mlt.gated_delta_rule(q, far, v, g, beta, initial_state=s0)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    far.copy_(v)
+    got = mlt.gated_delta_rule(q, k, far, g, beta, initial_state=s0)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
 def test_prompt_then_tokens():
     """A prompt in two pieces, then single tokens by the step, is the whole sequence at once."""
     q, k, v, g, beta, s0 = inputs(2, 140, 2, 4, 64, 64, torch.float32, seed=9)

@@ -341,6 +341,74 @@ def test_linear_gradient_by_differences():
 
 
 @pytest.mark.gpu
+def test_linear_of_nothing():
+    for rows, n, k in ((0, 5, 16), (3, 0, 16), (3, 5, 0)):
+        x = torch.randn(rows, k, device="cuda").requires_grad_()
+        w = torch.randn(n, k, device="cuda").requires_grad_()
+        y = mlt.linear_fp8(x, w)
+        dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+        assert y.shape == (rows, n) and not y.any() and dx.shape == x.shape and dw.shape == w.shape
+        assert not dx.any() and not dw.any()
+
+
+@pytest.mark.gpu
+def test_a_mixing_layer_as_it_is_used():
+    """Projections in 8 bits, the gated delta rule over a ragged batch of prompts, the projection back, with gradients; then
+    the next token of every sequence from the final states. Against the same layer with the operators' own definitions."""
+    from test_delta import recurrence
+    torch.manual_seed(5)
+    d, h, hv, dk, dv = 128, 2, 4, 32, 32
+    lens = [70, 1, 130]
+    cu = torch.tensor([0] + lens).cumsum(0)
+    total = int(cu[-1])
+    x = (torch.randn(total + 3, d, device="cuda") * 0.5).requires_grad_()
+    w_in = (torch.randn(2 * h * dk + hv * dv + 2 * hv, d, device="cuda") / math.sqrt(d)).requires_grad_()
+    w_out = (torch.randn(d, hv * dv, device="cuda") / math.sqrt(hv * dv)).requires_grad_()
+
+    def layer(x, linear, mix):
+        y = linear(x, w_in)
+        q, k, v, g, beta = y.split([h * dk, h * dk, hv * dv, hv, hv], -1)
+        unit = lambda t: torch.nn.functional.normalize(t.reshape(-1, h, dk), dim=-1)  # noqa: E731
+        o, s = mix(unit(q), unit(k), v.reshape(-1, hv, dv), -torch.nn.functional.softplus(g), torch.sigmoid(beta))
+        return linear(o.reshape(-1, hv * dv), w_out), s
+
+    def operators(q, k, v, g, beta):
+        o, s = mlt.gated_delta_rule(*(t[None] for t in (q, k, v, g, beta)), cu_seqlens=cu.cuda())
+        return o[0], s
+
+    def definitions(q, k, v, g, beta):
+        outs, states = [], []
+        for a, b in zip(cu.tolist(), cu.tolist()[1:]):
+            o, s = recurrence(*(t[None, a:b] for t in (q, k, v, g, beta)), torch.zeros(1, hv, dk, dv))
+            outs.append(o[0])
+            states.append(s)
+        return torch.cat(outs).float().cuda(), torch.cat(states).float().cuda()
+
+    y, s = layer(x[:total], mlt.linear_fp8, operators)
+    grads = torch.autograd.grad((y, s), (x, w_in, w_out), (torch.ones_like(y), torch.ones_like(s)), retain_graph=True)
+    want_y, want_s = layer(x[:total], mlt.linear_fp8, definitions)
+    want = torch.autograd.grad((want_y, want_s), (x, w_in, w_out), (torch.ones_like(want_y), torch.ones_like(want_s)))
+    # both sides quantise the same numbers but for their last bits; a value next to a rounding border of e4m3 then moves by a
+    # whole step, 2^-3 of it at most: among the up to 2^14 values of a quantised operand a few do, (few * 2^-6 / 2^14)^1/2 < 2^-8
+    for a, b in zip((y, s, *grads), (want_y, want_s, *want)):
+        assert (a - b).norm() <= 2.0 ** -8 * b.norm()
+
+    with torch.no_grad():
+        pool = s.detach().clone()
+        nxt, _ = layer(x[total:], mlt.linear_fp8, lambda q, k, v, g, beta: (
+            mlt.gated_delta_step(*(t[:, None] for t in (q, k, v, g, beta)), pool)[:, 0], pool))
+        after = [None]
+
+        def one(q, k, v, g, beta):
+            o, after[0] = recurrence(*(t[:, None] for t in (q, k, v, g, beta)), s)
+            return o[:, 0].float().cuda(), after[0]
+
+        want_next, _ = layer(x[total:], mlt.linear_fp8, one)
+    assert (nxt - want_next).norm() <= 2.0 ** -8 * want_next.norm()
+    assert (pool.double().cpu() - after[0]).norm() <= 2.0 ** -18 * after[0].norm()
+
+
+@pytest.mark.gpu
 def test_streams_and_graphs():
     x, w = torch.randn(200, 256, device="cuda").bfloat16(), torch.randn(130, 256, device="cuda").bfloat16()
     want = mlt.linear_fp8(x, w)
