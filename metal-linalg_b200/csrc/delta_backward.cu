@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
     const bool live = dv0 < (int)p.dvp;
     float s[NT][4];                     // dS'^T
     const size_t state0 = ((size_t)seq * p.value_heads + hv) * p.dk * p.dv;
-    const auto col = [&](int i) { return dv0 + g + 8 * (i >> 1); };
+    const auto col = [&](int i) { return dv0 + 2 * g + (i >> 1); };
     const auto row = [&](int n, int i) { return k_base + 8 * n + 2 * t + (i & 1); };
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -190,15 +190,9 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
         const size_t at = (size_t)c * p.value_heads + hv;
         const float *e = st.gates, *left = e + kChunk, *beta = left + kChunk;
         if (live) {
-            float* out = p.d_states + at * p.dkp * p.dvp + (size_t)(k_base + 2 * t) * p.dvp + dv0 + g;
+            float* out = p.d_states + at * p.dkp * p.dvp + (size_t)(k_base + 2 * t) * p.dvp + dv0 + 2 * g;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                out[0] = s[n][0];
-                out[8] = s[n][2];
-                out[p.dvp] = s[n][1];
-                out[p.dvp + 8] = s[n][3];
-                out += 8 * p.dvp;
-            }
+            for (int n = 0; n < NT; ++n, out += 8 * p.dvp) put_tile(out, p.dvp, s[n]);
         }
         float x[8][4] = {};
 #pragma unroll
@@ -228,11 +222,12 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
                 add_to(f, x[i]);
             }
             const float2 le = *reinterpret_cast<const float2*>(left + 8 * n + 2 * t);
-            const float* dd = st.dd + (8 * n + 2 * t) * LDV + 16 * chain + g;
-            f[0] = fmaf(le.x, f[0], dd[0]);
-            f[1] = fmaf(le.y, f[1], dd[LDV]);
-            f[2] = fmaf(le.x, f[2], dd[8]);
-            f[3] = fmaf(le.y, f[3], dd[LDV + 8]);
+            const float* dd = st.dd + (8 * n + 2 * t) * LDV + 16 * chain + 2 * g;
+            const float2 d0 = pair_at(dd), d1 = pair_at(dd + LDV);
+            f[0] = fmaf(le.x, f[0], d0.x);
+            f[1] = fmaf(le.y, f[1], d1.x);
+            f[2] = fmaf(le.x, f[2], d0.y);
+            f[3] = fmaf(le.y, f[3], d1.y);
             if constexpr (KS > 1) {
                 TileTf32 a;
                 a.set(f);
@@ -244,11 +239,12 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
         }
         const auto out_tile = [&](int n, float (&u)[4]) {          // scale e^G dO of token tile n
             const float2 ee = *reinterpret_cast<const float2*>(e + 8 * n + 2 * t);
-            const T* d_o = st.d_o + (8 * n + 2 * t) * LDV + 16 * chain + g;
-            u[0] = p.scale * ee.x * to_f(d_o[0]);
-            u[1] = p.scale * ee.y * to_f(d_o[LDV]);
-            u[2] = p.scale * ee.x * to_f(d_o[8]);
-            u[3] = p.scale * ee.y * to_f(d_o[LDV + 8]);
+            const T* d_o = st.d_o + (8 * n + 2 * t) * LDV + 16 * chain + 2 * g;
+            const float2 o0 = pair_at(d_o), o1 = pair_at(d_o + LDV);
+            u[0] = p.scale * ee.x * o0.x;
+            u[1] = p.scale * ee.y * o1.x;
+            u[2] = p.scale * ee.x * o0.y;
+            u[3] = p.scale * ee.y * o1.y;
         };
         if constexpr (KS > 1) {
 #pragma unroll
@@ -274,17 +270,11 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
                                                                                    : j >= 4 && own_tile<KS>(part, i) <= j; },
                          [&](int i) { return tri[tri_tile(j, KS > 1 ? own_tile<KS>(part, i) : i) * 32]; });
         }
-        float* d_out = p.dr + at * kChunk * p.dvp + (size_t)(2 * t) * p.dvp + dv0 + g;
+        float* d_out = p.dr + at * kChunk * p.dvp + (size_t)(2 * t) * p.dvp + dv0 + 2 * g;
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
             const int n = KS > 1 ? own_tile<KS>(part, i) : i;
-            if (live) {
-                float* out = d_out + (size_t)(8 * n) * p.dvp;
-                out[0] = d[i][0];
-                out[8] = d[i][2];
-                out[p.dvp] = d[i][1];
-                out[p.dvp + 8] = d[i][3];
-            }
+            if (live) put_tile(d_out + (size_t)(8 * n) * p.dvp, p.dvp, d[i]);
             const float2 be = *reinterpret_cast<const float2*>(beta + 8 * n + 2 * t), ee = *reinterpret_cast<const float2*>(e + 8 * n + 2 * t);
             d[i][0] *= -be.x * ee.x; d[i][1] *= -be.y * ee.y; d[i][2] *= -be.x * ee.x; d[i][3] *= -be.y * ee.y;
             if constexpr (KS > 1) {
@@ -415,11 +405,22 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int m0 = 16 * (warp & 3), part = warp >> 2, n0 = part * (DKP / 4), j0 = 16 * part;
     T *dq = static_cast<T*>(p.dq), *dk = static_cast<T*>(p.dk_out), *dv = static_cast<T*>(p.dv_out);
+    const bool pairs = p.dk % 2 == 0 && ((reinterpret_cast<size_t>(dq) | reinterpret_cast<size_t>(dk)) & 7) == 0;
     const Chunk ch = chunk_at(p, c);
     const auto put_qk = [&](size_t token, int column, float q0, float q1, float k0, float k1) {     // columns `column`, + 1
         const size_t to = (token * p.value_heads + hv) * p.dk + column;     // heads and value heads are the same where up is 1
         const bool two = column + 1 < (int)p.dk;
         if (column >= (int)p.dk) return;
+        if (pairs) {
+            if (up == 1) {
+                put_pair(dq + to, q0, q1);
+                put_pair(dk + to, k0, k1);
+            } else {
+                put_pair(p.fold_q + to, q0, q1);
+                put_pair(p.fold_k + to, k0, k1);
+            }
+            return;
+        }
         if (up == 1) {
             dq[to] = from_f<T>(q0);
             dk[to] = from_f<T>(k0);

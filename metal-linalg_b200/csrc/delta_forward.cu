@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kStateThreads, sizeof(T) == 2 ? 2 : 1) delta_s
 
     float s[NT][4];
     const size_t state0 = ((size_t)seq * p.value_heads + hv) * p.dk * p.dv;
-    const auto col = [&](int i) { return dv0 + g + 8 * (i >> 1); };
+    const auto col = [&](int i) { return dv0 + 2 * g + (i >> 1); };
     const auto row = [&](int n, int i) { return k_base + 8 * n + 2 * t + (i & 1); };
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -317,15 +317,9 @@ __global__ void __launch_bounds__(kStateThreads, sizeof(T) == 2 ? 2 : 1) delta_s
 
         // the state at the chunk's start
         if (live) {
-            float* out = p.states + at * p.dkp * p.dvp + (size_t)(k_base + 2 * t) * p.dvp + dv0 + g;
+            float* out = p.states + at * p.dkp * p.dvp + (size_t)(k_base + 2 * t) * p.dvp + dv0 + 2 * g;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                out[0] = s[n][0];
-                out[8] = s[n][2];
-                out[p.dvp] = s[n][1];
-                out[p.dvp + 8] = s[n][3];
-                out += 8 * p.dvp;
-            }
+            for (int n = 0; n < NT; ++n, out += 8 * p.dvp) put_tile(out, p.dvp, s[n]);
         }
 
         // X^T, the next k's operands on their way while one is multiplied
@@ -351,11 +345,12 @@ __global__ void __launch_bounds__(kStateThreads, sizeof(T) == 2 ? 2 : 1) delta_s
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
             const int n = own_tile<KS>(part, i);
-            const T* v = st.v + (8 * n + 2 * t) * Sh::kLdV + 16 * chain + g;
-            value[i][0] = to_f(v[0]);
-            value[i][1] = to_f(v[Sh::kLdV]);
-            value[i][2] = to_f(v[8]);
-            value[i][3] = to_f(v[Sh::kLdV + 8]);
+            const T* v = st.v + (8 * n + 2 * t) * Sh::kLdV + 16 * chain + 2 * g;
+            const float2 v0 = pair_at(v), v1 = pair_at(v + Sh::kLdV);
+            value[i][0] = v0.x;
+            value[i][1] = v1.x;
+            value[i][2] = v0.y;
+            value[i][3] = v1.y;
             beta2[i] = *reinterpret_cast<const float2*>(beta + 8 * n + 2 * t);
             e2[i] = *reinterpret_cast<const float2*>(e + 8 * n + 2 * t);
             left2[i] = *reinterpret_cast<const float2*>(left + 8 * n + 2 * t);
@@ -452,15 +447,9 @@ __global__ void __launch_bounds__(kStateThreads, sizeof(T) == 2 ? 2 : 1) delta_s
             mma_columns<T, NT, true>(s, a, f[j & 1]);
         }
         if (live) {
-            float* d_out = p.d + at * kChunk * p.dvp + (size_t)(2 * t) * p.dvp + dv0 + g;
+            float* d_out = p.d + at * kChunk * p.dvp + (size_t)(2 * t) * p.dvp + dv0 + 2 * g;
 #pragma unroll
-            for (int i = 0; i < kOwn; ++i) {
-                float* out = d_out + (size_t)(8 * own_tile<KS>(part, i)) * p.dvp;
-                out[0] = d[i][0];
-                out[8] = d[i][2];
-                out[p.dvp] = d[i][1];
-                out[p.dvp + 8] = d[i][3];
-            }
+            for (int i = 0; i < kOwn; ++i) put_tile(d_out + (size_t)(8 * own_tile<KS>(part, i)) * p.dvp, p.dvp, d[i]);
         }
     }
     if (p.final_state)
@@ -519,25 +508,23 @@ __global__ void __launch_bounds__(kOutThreads, 2) delta_output_kernel(const Args
     load_rows<T, kOutThreads, DKP>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, threadIdx.x);
     load_floats<kOutThreads, sizeof(Gates) / 4>(reinterpret_cast<float*>(&sh.gates), reinterpret_cast<const float*>(p.gates + at), threadIdx.x);
     cp_commit();
-    // a k of 16 of S^T or D^T as two accumulator tiles: rows 2t, 2t + 1, 2t + 8, 2t + 9 of columns g, g + 8
-    float held[kHeld][8];
-    const auto fetch = [&](const float* base, int row, float (&to)[8]) {
-        const float* src = base + (size_t)(row + 2 * t) * p.dvp + g;
-        to[0] = src[0];
-        to[2] = src[8];
-        to[1] = src[p.dvp];
-        to[3] = src[p.dvp + 8];
+    // a k of 16 of S^T or D^T as two accumulator tiles: rows 2t, 2t + 1, 2t + 8, 2t + 9 of columns 2g, 2g + 1
+    float2 held[kHeld][4];
+    const auto fetch = [&](const float* base, int row, float2 (&to)[4]) {
+        const float* src = base + (size_t)(row + 2 * t) * p.dvp + 2 * g;
+        to[0] = *reinterpret_cast<const float2*>(src);
+        to[1] = *reinterpret_cast<const float2*>(src + p.dvp);
         src += 8 * p.dvp;
-        to[4] = src[0];
-        to[6] = src[8];
-        to[5] = src[p.dvp];
-        to[7] = src[p.dvp + 8];
+        to[2] = *reinterpret_cast<const float2*>(src);
+        to[3] = *reinterpret_cast<const float2*>(src + p.dvp);
     };
-    const auto tiles = [](const float (&from)[8], float (&x)[4], float (&y)[4]) {
+    const auto tiles = [](const float2 (&from)[4], float (&x)[4], float (&y)[4]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = from[i];
-            y[i] = from[4 + i];
+        for (int i = 0; i < 2; ++i) {
+            x[i] = from[i].x;
+            x[2 + i] = from[i].y;
+            y[i] = from[2 + i].x;
+            y[2 + i] = from[2 + i].y;
         }
     };
     const float *s = p.states + at * p.dkp * p.dvp, *d = p.d + at * kChunk * p.dvp;
@@ -606,8 +593,8 @@ __global__ void __launch_bounds__(kOutThreads, 2) delta_output_kernel(const Args
 #pragma unroll
             for (int n = 0; n < 8; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    sh.o[(8 * n + 2 * t + (i & 1)) * LDO + 16 * warp + g + 8 * (i >> 1)] = from_f<T>(p.scale * acc[n][i]);
+                for (int i = 0; i < 2; ++i)
+                    put_pair(sh.o + (8 * n + 2 * t + i) * LDO + 16 * warp + 2 * g, p.scale * acc[n][i], p.scale * acc[n][2 + i]);
         }
         __syncthreads();
         const int width = min(kOutCols, (int)p.dv - pass);

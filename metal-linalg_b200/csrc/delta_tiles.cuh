@@ -465,6 +465,27 @@ __device__ __forceinline__ float exp_of(double x) { return exp_of((float)x, (flo
 // e^{G_i - G_j}. The difference of the leading parts is rounded once, 2^-24 of it: e^-x x 2^-24 is at most 2^-25 of e^0.
 __device__ __forceinline__ float decay_of(const Gates& g, int i, int j) { return exp_of(g.sum[i] - g.sum[j], g.rest[i] - g.rest[j]); }
 
+// A chain's 16 value columns as rows of its A operands: fragment rows g and g + 8 are columns 2g and 2g + 1, so that a lane
+// reads and writes pairs.
+template <typename T> __device__ __forceinline__ float2 pair_at(const T* p) {
+    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float2*>(p);
+    else {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+        if constexpr (__is_same(T, __half)) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+        else                                return make_float2(low_f(w), high_f(w));
+    }
+}
+template <typename T> __device__ __forceinline__ void put_pair(T* p, float x, float y) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p) = make_float2(x, y);
+    else if constexpr (__is_same(T, __half)) *reinterpret_cast<__half2*>(p) = __floats2half2_rn(x, y);
+    else *reinterpret_cast<uint32_t*>(p) = pack_bf16(x, y);
+}
+// A tile's two token (or key) rows 2t and 2t + 1, `ld` apart.
+__device__ __forceinline__ void put_tile(float* p, size_t ld, const float (&x)[4]) {
+    *reinterpret_cast<float2*>(p) = make_float2(x[0], x[2]);
+    *reinterpret_cast<float2*>(p + ld) = make_float2(x[1], x[3]);
+}
+
 // Of a chain's 8 token tiles, the i-th that warp `part` of its KS computes: 0 and 7 together, 1 and 6 ..., so that the
 // triangle's work is even.
 template <int KS>
