@@ -13,6 +13,7 @@
 //
 // S and D come from the forward's preparation and sequential pass, run again: keeping them from the forward would hold
 // 112 KB a chunk and head for the time between (the inputs are 48 KB in bfloat16).
+#include "common.cuh"
 #include "delta.h"
 #include "delta_tiles.cuh"
 #include "runtime.h"
@@ -38,6 +39,7 @@ struct DoShared {
 
 template <typename T, int DKP>
 __global__ void __launch_bounds__(kDoThreads) delta_do_kernel(const Args p) {
+    dependency_wait_only();
     extern __shared__ __align__(16) char raw[];
     using Sp = typename Split<T>::type;
     DoShared<T, DKP>& sh = *reinterpret_cast<DoShared<T, DKP>*>(raw);
@@ -119,6 +121,7 @@ struct ReverseShared {
 
 template <typename T, int DKP, int KS>
 __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Args p) {
+    dependency_wait_only();
     using Sh = ReverseShared<T, DKP, KS>;
     using Sp = typename Split<T>::type;
     using Tile = typename Split<T>::tile;
@@ -395,6 +398,7 @@ __device__ __forceinline__ void slice_a(SplitTf32& a, const T* tile, int m0) {
 }
 template <typename T, int DKP>
 __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) {
+    dependency_wait_only();
     extern __shared__ __align__(16) char raw[];
     using Sh = GradShared<T, DKP>;
     using Sp = typename Split<T>::type;
@@ -437,12 +441,12 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) 
             }
         }
     };
-    if (ch.rows == 0) {             // a ragged batch's blocks behind its chunks: tokens behind the last sequence get zeros
+    if (ch.rows == 0) {             // a ragged batch's blocks behind its chunks: tokens of no sequence get zeros
         const uint32_t used = p.first[p.sequences], spare = gridDim.x - used;
-        const int end = p.first[p.sequences + 1];
-        for (long long r0 = end + (long long)(c - used) * kChunk; r0 < (long long)p.tokens; r0 += (long long)spare * kChunk)
-            for (int r = warp; r < kChunk && r0 + r < (long long)p.tokens; r += kGradThreads / 32) {
-                const size_t token = r0 + r;
+        const Unused none(p);
+        for (long long r0 = (long long)(c - used) * kChunk; r0 < none.count; r0 += (long long)spare * kChunk)
+            for (int r = warp; r < kChunk && r0 + r < none.count; r += kGradThreads / 32) {
+                const size_t token = none.token(r0 + r);
                 for (int i = 2 * lane; i < (int)p.dk; i += 64) put_qk(token, i, 0.0f, 0.0f, 0.0f, 0.0f);
                 for (int i = lane; i < (int)p.dv; i += 32) dv[(token * p.value_heads + hv) * p.dv + i] = from_f<T>(0.0f);
                 if (lane == 0) p.dg[token * p.value_heads + hv] = p.dbeta[token * p.value_heads + hv] = 0.0f;
@@ -708,6 +712,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) 
 // The gradients of shared heads: the sums over the value heads that read them, in their order.
 template <typename T, int DKP>
 __global__ void __launch_bounds__(256) delta_fold_kernel(const Args p) {
+    dependency_wait_only();
     const size_t rows = (size_t)p.batch * p.tokens * p.heads;
     const uint32_t up = p.value_heads / p.heads;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < rows * p.dk; i += (size_t)gridDim.x * 256) {
@@ -728,7 +733,7 @@ void reverse_as(const Args& a, cudaStream_t stream) {
     using Sh = ReverseShared<T, DKP, KS>;
     opt_in<delta_reverse_kernel<T, DKP, KS>>(sizeof(Sh));
     const dim3 grid((a.dvp / 16 + Sh::kGroups - 1) / Sh::kGroups, a.value_heads, a.seqs);
-    delta_reverse_kernel<T, DKP, KS><<<grid, kReverseThreads, sizeof(Sh), stream>>>(a);
+    launch_dependent(delta_reverse_kernel<T, DKP, KS>, grid, kReverseThreads, sizeof(Sh), stream, a);
     cuda_check(cudaGetLastError(), "delta rule states backward");
 }
 
@@ -736,7 +741,7 @@ template <typename T, int DKP>
 void backward_as(const Args& a, cudaStream_t stream, int sm_count) {
     if (a.chunks) {
         opt_in<delta_do_kernel<T, DKP>>(sizeof(DoShared<T, DKP>));
-        delta_do_kernel<T, DKP><<<dim3(a.chunks, a.value_heads), kDoThreads, sizeof(DoShared<T, DKP>), stream>>>(a);
+        launch_dependent(delta_do_kernel<T, DKP>, dim3(a.chunks, a.value_heads), kDoThreads, sizeof(DoShared<T, DKP>), stream, a);
         cuda_check(cudaGetLastError(), "delta rule P^T dO");
     }
     // Four warps to a chain while there is at most one chain a multiprocessor, two up to two chains (or where sequences of
@@ -748,12 +753,13 @@ void backward_as(const Args& a, cudaStream_t stream, int sm_count) {
     else reverse_as<T, DKP, 1>(a, stream);
     if (a.chunks) {
         opt_in<delta_grad_kernel<T, DKP>>(sizeof(GradShared<T, DKP>));
-        delta_grad_kernel<T, DKP><<<dim3(a.chunks + (a.sequences ? 1 : 0), a.value_heads), kGradThreads, sizeof(GradShared<T, DKP>), stream>>>(a);
+        launch_dependent(delta_grad_kernel<T, DKP>, dim3(a.chunks + (a.sequences ? 1 : 0), a.value_heads), kGradThreads, sizeof(GradShared<T, DKP>),
+                         stream, a);
         cuda_check(cudaGetLastError(), "delta rule gradients");
         if (a.value_heads != a.heads) {
             const size_t count = (size_t)a.batch * a.tokens * a.heads * a.dk;
             const unsigned blocks = (unsigned)(count / 256 + 1 < (size_t)sm_count * 8 ? count / 256 + 1 : (size_t)sm_count * 8);
-            delta_fold_kernel<T, DKP><<<blocks, 256, 0, stream>>>(a);
+            launch_dependent(delta_fold_kernel<T, DKP>, blocks, 256, 0, stream, a);
             cuda_check(cudaGetLastError(), "delta rule shared heads");
         }
     }
@@ -761,10 +767,11 @@ void backward_as(const Args& a, cudaStream_t stream, int sm_count) {
 
 } // namespace
 
-void launch_backward(const Args& a, cudaStream_t stream, int sm_count) {
+void launch_backward(const Args& a, cudaStream_t stream, int device) {
+    const int sms = sm_count(device);
     launch_prepare(a, stream, true);
-    launch_states(a, stream, sm_count);
-    DELTA_DISPATCH(backward_as, a, stream, sm_count);
+    launch_states(a, stream, sms);
+    DELTA_DISPATCH(backward_as, a, stream, sms);
 }
 
 } // namespace delta

@@ -9,6 +9,7 @@
 // four blocks a head of 128 columns, so that one request alone still spreads over the multiprocessors. Slots, inputs and
 // states are asked for together, ahead of the search for rows of the same slot: 128 rows of 32 heads of 128 x 128 take 100 us
 // (5.4 TB/s), 143 with the search first; one row of 8 heads 3.4 us.
+#include "common.cuh"
 #include "delta.h"
 #include "delta_tiles.cuh"
 #include "runtime.h"
@@ -30,6 +31,7 @@ __device__ __forceinline__ long long slot_of(const StepArgs& a, uint32_t row) {
 
 template <typename T>
 __global__ void __launch_bounds__(kStepThreads, 7) delta_step_kernel(const StepArgs a) {
+    dependency_wait_only();
     __shared__ float qs[128], ks[128];
     __shared__ float sums[4][2][kStepCols + 4];     // a warp's sums of s_k and s_q, and of k . q behind them
     __shared__ int same[4];                         // a warp's rows of the same slot: 1 there are earlier ones, 2 later ones
@@ -176,9 +178,9 @@ __global__ void __launch_bounds__(kStepThreads, 7) delta_step_kernel(const StepA
 void launch_step(const StepArgs& a, cudaStream_t stream) {
     const dim3 grid((a.dv + kStepCols - 1) / kStepCols, a.value_heads, a.batch);
     switch (a.dtype) {
-        case METAL_LINALG_BFLOAT16: delta_step_kernel<bf16><<<grid, kStepThreads, 0, stream>>>(a); break;
-        case METAL_LINALG_FLOAT16: delta_step_kernel<__half><<<grid, kStepThreads, 0, stream>>>(a); break;
-        default: delta_step_kernel<float><<<grid, kStepThreads, 0, stream>>>(a); break;
+        case METAL_LINALG_BFLOAT16: launch_dependent(delta_step_kernel<bf16>, grid, kStepThreads, 0, stream, a); break;
+        case METAL_LINALG_FLOAT16: launch_dependent(delta_step_kernel<__half>, grid, kStepThreads, 0, stream, a); break;
+        default: launch_dependent(delta_step_kernel<float>, grid, kStepThreads, 0, stream, a); break;
     }
     cuda_check(cudaGetLastError(), "delta rule step");
 }

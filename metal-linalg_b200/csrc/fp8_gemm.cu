@@ -217,6 +217,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_slot;
+    dependency_wait_only();         // nothing above reads or writes memory that another kernel may hold
     if (a.split > 1) {          // the other blocks are there before anything is sent to them (arrival now, the wait before the first use)
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     }
@@ -525,12 +526,21 @@ void gemm_as(cudaStream_t stream, const CUtensorMap& mp, const CUtensorMap& mq, 
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = S::kShared;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = a.split;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    unsigned count = 0;
+    if (a.split > 1) {
+        attr[count].id = cudaLaunchAttributeClusterDimension;
+        attr[count].val.clusterDim.x = a.split;
+        attr[count].val.clusterDim.y = attr[count].val.clusterDim.z = 1;
+        ++count;
+    }
+    if (dependent_launches_enabled()) {         // as launch_dependent: the kernel's set-up beside the end of the one before it
+        attr[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[count].val.programmaticStreamSerializationAllowed = 1;
+        ++count;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = a.split > 1 ? 1 : 0;
+    cfg.numAttrs = count;
     cuda_check(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<BN, kByColumn>, mp, mq, a), "fp8 product launch");
 }
 

@@ -8,6 +8,7 @@
 //   tiles    the same in 128 x 128: 512 threads hold the tile in registers
 //   turned   x contiguous along rows (a transposed matrix): a 128 x 128 tile through shared memory as it lies, read back a
 //            quarter of a row of the result a thread, either block shape
+#include "common.cuh"
 #include "fp8.h"
 #include "runtime.h"
 
@@ -150,6 +151,7 @@ template <typename T> struct Eight {
 // kUnits blocks of 128 for every 16 lanes, all fetched before the first is used.
 template <typename T, bool kE5m2, int kUnits>
 __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const QuantizeArgs a) {
+    dependency_wait_only();
     const uint32_t blocks = (a.cols + kB - 1) / kB, z = blockIdx.y;
     const uint32_t first = blockIdx.x * (kRowThreads / 16 * kUnits) + (threadIdx.x >> 4);
     const uint32_t in = (threadIdx.x & 15) * 8;
@@ -201,6 +203,7 @@ __device__ __forceinline__ float block_max(float top, float* shared) {
 
 template <typename T, bool kE5m2>
 __global__ void __launch_bounds__(kTileThreads, sizeof(T) == 2 ? 4 : 2) quantize_tiles_kernel(const QuantizeArgs a) {
+    dependency_wait_only();
     constexpr int kRows = kTileThreads / 16, kHeld = kB / kRows;
     __shared__ float tops[kTileThreads / 32];
     const uint32_t blocks = (a.cols + kB - 1) / kB, z = blockIdx.y;
@@ -236,6 +239,7 @@ __global__ void __launch_bounds__(kTileThreads, sizeof(T) == 2 ? 4 : 2) quantize
 // row r, neighbouring lanes neighbouring rows.
 template <typename T, bool kE5m2>
 __global__ void __launch_bounds__(kThreads, 2) quantize_turned_kernel(const QuantizeArgs a) {
+    dependency_wait_only();
     extern __shared__ __align__(16) char raw[];
     T* tile = reinterpret_cast<T*>(raw);
     __shared__ float tops[kThreads];
@@ -314,16 +318,16 @@ void quantize_as(const QuantizeArgs& a, cudaStream_t stream) {
                        "quantize shared memory");
             once.mark(device);
         }
-        quantize_turned_kernel<T, kE5m2><<<dim3((unsigned)tiles, a.batch), kThreads, bytes, stream>>>(a);
+        launch_dependent(quantize_turned_kernel<T, kE5m2>, dim3((unsigned)tiles, a.batch), kThreads, bytes, stream, a);
     } else if (a.block_rows == 1) {
         // four blocks of 128 a thread where that still leaves every multiprocessor two thread blocks
         const uint64_t units = a.rows * blocks, each = kRowThreads / 16;
         if (units * a.batch >= 4 * each * 2 * (uint64_t)sm_count(current_device()))
-            quantize_rows_kernel<T, kE5m2, 4><<<dim3((unsigned)((units + 4 * each - 1) / (4 * each)), a.batch), kRowThreads, 0, stream>>>(a);
+            launch_dependent(quantize_rows_kernel<T, kE5m2, 4>, dim3((unsigned)((units + 4 * each - 1) / (4 * each)), a.batch), kRowThreads, 0, stream, a);
         else
-            quantize_rows_kernel<T, kE5m2, 1><<<dim3((unsigned)((units + each - 1) / each), a.batch), kRowThreads, 0, stream>>>(a);
+            launch_dependent(quantize_rows_kernel<T, kE5m2, 1>, dim3((unsigned)((units + each - 1) / each), a.batch), kRowThreads, 0, stream, a);
     } else {
-        quantize_tiles_kernel<T, kE5m2><<<dim3((unsigned)tiles, a.batch), kTileThreads, 0, stream>>>(a);
+        launch_dependent(quantize_tiles_kernel<T, kE5m2>, dim3((unsigned)tiles, a.batch), kTileThreads, 0, stream, a);
     }
     cuda_check(cudaGetLastError(), "quantize launch");
 }

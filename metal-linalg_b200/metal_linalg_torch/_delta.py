@@ -226,8 +226,8 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, cu_seq
     long as the last dimensions of q, k and v are contiguous; others are copied.
 
     Each batch row is a sequence. With ``cu_seqlens`` (int32 or int64, on the GPU, N + 1 values from 0 on, none falling) B is
-    1 and sequence ``i`` is the tokens ``cu_seqlens[i] .. cu_seqlens[i + 1] - 1``; a sequence may be empty, and tokens behind
-    the last one give zeros. ``initial_state`` [B or N, HV, Dk, Dv] (float32; default zero) is where each starts;
+    1 and sequence ``i`` is the tokens ``cu_seqlens[i] .. cu_seqlens[i + 1] - 1``; a sequence may be empty, and tokens of no
+    sequence give zeros. ``initial_state`` [B or N, HV, Dk, Dv] (float32; default zero) is where each starts;
     ``final_state`` has its shape. ``o`` has v's shape and type.
 
     Differentiable once in q, k, v, g, beta and initial_state, through both results.
@@ -311,4 +311,5 @@ def gated_delta_step(q, k, v, g, beta, state, *, slots=None, scale=None):
     g, beta = _float(g), _float(beta)
     if torch.compiler.is_compiling() or q.device.type == "meta":
         return torch.ops.metal_linalg.gated_delta_step(q, k, v, g, beta, state, slots, scale)
+    torch.autograd.graph.increment_version(state)       # a graph that saved the pool for its backward pass finds it changed
     return _step(q, k, v, g, beta, state, slots, scale)

@@ -685,3 +685,90 @@ def test_tensors_of_another_gpu_than_the_current_one():
     want_o, want_s = recurrence(*args)
     near(o, want_o, tolerance(torch.bfloat16))
     near(s, want_s, F32)
+
+
+# ---------------------------------------------------------------------------
+# Long sequences, whose parts overlap on two streams; tokens of no sequence; pools that graphs have saved
+# ---------------------------------------------------------------------------
+
+LONG = [
+    # B, T, H, HV, Dk, Dv, bounds
+    (1, 64 * 200 + 17, 1, 2, 64, 32, None), (2, 64 * 128, 1, 1, 128, 16, None), (1, 64 * 127 + 63, 2, 2, 16, 48, None),
+    (1, 64 * 200, 1, 2, 64, 32, (0, 64 * 200)), (1, 64 * 200, 1, 1, 32, 24, (5, 64 * 130 + 5)), (1, 64 * 300, 1, 1, 32, 16, (0, 100)),
+    (1, 64 * 192, 1, 1, 64, 64, (64, 64 * 129)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", LONG, ids=str)
+def test_long_sequences_in_parts_are_the_whole(shape):
+    """Captured calls run whole, eager ones in parts: the same products in the same order, bit for bit. And the float64
+    recurrence's, from a few tokens before the end on (a sequence in two calls)."""
+    b, t, h, hv, dk, dv, bounds = shape
+    q, k, v, g, beta, s0 = inputs(b, t, h, hv, dk, dv, torch.bfloat16, seed=t)
+    cu = None if bounds is None else torch.tensor(bounds, dtype=torch.int32, device="cuda")
+    call = lambda: mlt.gated_delta_rule(q, k, v, g, beta, initial_state=s0, cu_seqlens=cu)  # noqa: E731
+    o, s = call()
+    again = call()
+    assert torch.equal(o, again[0]) and torch.equal(s, again[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        whole = call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, whole[0]) and torch.equal(s, whole[1])
+    first, last = (0, t) if bounds is None else bounds
+    cut = max(first, last - 50)
+    part = lambda a, z: [x[:, a:z] for x in (q, k, v, g, beta)]  # noqa: E731
+    _, middle = mlt.gated_delta_rule(*part(first, cut), initial_state=s0)
+    want_o, want_s = recurrence(*part(cut, last), middle)
+    near(o[:, cut:last], want_o, tolerance(torch.bfloat16))
+    near(s, want_s, F32)
+
+
+@pytest.mark.gpu
+def test_long_sequences_on_many_streams_and_threads():
+    import threading
+    args = inputs(1, 64 * 150, 1, 2, 64, 32, torch.bfloat16)
+    want = mlt.gated_delta_rule(*args[:5], initial_state=args[5])
+    torch.cuda.synchronize()
+    got, failed = {}, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(4):
+                    got[i] = mlt.gated_delta_rule(*args[:5], initial_state=args[5])
+        except Exception as e:      # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [x.start() for x in threads]
+    [x.join() for x in threads]
+    torch.cuda.synchronize()
+    assert not failed and all(torch.equal(a, b) for r in got.values() for a, b in zip(r, want))
+
+
+@pytest.mark.gpu
+def test_tokens_before_the_first_sequence():
+    q, k, v, g, beta, s0 = inputs(1, 300, 1, 2, 32, 48, torch.float32, n=2)
+    cu = torch.tensor([70, 130, 210], device="cuda")
+    torch.full((1, 300, 2, 48), float("nan"), device="cuda")       # what the allocator hands out next
+    leaves = [x.requires_grad_() for x in (q, k, v, g, beta)]
+    o, s = mlt.gated_delta_rule(*leaves, initial_state=s0, cu_seqlens=cu)
+    grads = torch.autograd.grad((o, s), leaves, (torch.ones_like(o), torch.ones_like(s)))
+    inside = [x.detach()[:, 70:210] for x in leaves]
+    other, _ = mlt.gated_delta_rule(*inside, initial_state=s0, cu_seqlens=cu - 70)
+    assert torch.equal(o[:, 70:210], other)
+    for x in (o, *grads):
+        assert not x[:, :70].any() and not x[:, 210:].any() and x.isfinite().all()
+
+
+@pytest.mark.gpu
+def test_a_step_tells_the_graph_that_saved_its_pool():
+    q, k, v, g, beta, pool = inputs(2, 1, 1, 1, 16, 16, torch.float32)
+    o, _ = mlt.gated_delta_rule(q.requires_grad_(), k, v, g, beta, initial_state=pool)
+    with torch.no_grad():
+        mlt.gated_delta_step(q, k, v, g, beta, pool)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
