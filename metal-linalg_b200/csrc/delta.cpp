@@ -99,7 +99,6 @@ Args args_of(const metal_linalg_delta& p) {
     a.row_chunks = (p.tokens + kChunk - 1) / kChunk;
     // ragged: sum ceil(len / 64) <= total / 64 + sequences
     a.chunks = p.sequences ? p.tokens / kChunk + p.sequences : p.batch * a.row_chunks;
-    a.part1 = p.sequences ? a.chunks : a.row_chunks;
     return a;
 }
 
@@ -175,7 +174,7 @@ void gated_delta_rule(const metal_linalg_delta& p, void* o, float* final_state, 
     a.o = o;
     a.final_state = final_state;
     mlb::DeviceGuard guard(where.device);
-    mlb::delta::launch_forward(a, mlb::thread_stream(), where.device);
+    mlb::delta::launch_forward(a, mlb::thread_stream(), mlb::sm_count(where.device));
 }
 
 void gated_delta_rule_backward(const metal_linalg_delta& p, const void* d_o, const int64_t* d_o_stride,
@@ -206,7 +205,7 @@ void gated_delta_rule_backward(const metal_linalg_delta& p, const void* d_o, con
     a.d_final = d_final_state;
     a.dq = dq; a.dk_out = dk; a.dv_out = dv; a.dg = dg; a.dbeta = dbeta; a.d_initial = d_initial_state;
     mlb::DeviceGuard guard(where.device);
-    mlb::delta::launch_backward(a, mlb::thread_stream(), where.device);
+    mlb::delta::launch_backward(a, mlb::thread_stream(), mlb::sm_count(where.device));
 }
 
 void gated_delta_step(const metal_linalg_delta& p, void* o, float* pool, int64_t pool_stride, uint32_t pool_size,

@@ -53,7 +53,6 @@ struct Args {
     uint32_t  seqs;              // batch, or sequences
     uint32_t  row_chunks;        // chunks of a batch row (sequences == 0)
     uint32_t  chunks;            // all of them; an upper bound for a ragged batch
-    uint32_t  part0, part1;      // the chunks of a sequence that a launch of the preparation, the states or the outputs takes
     // workspace
     int*      table;             // ragged: {first token, tokens, sequence, 0} a chunk
     int*      first;             // ragged: [sequences + 3] first chunk of a sequence; then the number of chunks, the tokens
@@ -85,10 +84,10 @@ struct StepArgs {
     void*    o;
 };
 
-void launch_forward(const Args& a, cudaStream_t stream, int device);        // delta_forward.cu
+void launch_forward(const Args& a, cudaStream_t stream, int sm_count);      // delta_forward.cu
 void launch_prepare(const Args& a, cudaStream_t stream, bool backward);     // index, prep
 void launch_states(const Args& a, cudaStream_t stream, int sm_count);
-void launch_backward(const Args& a, cudaStream_t stream, int device);       // delta_backward.cu
+void launch_backward(const Args& a, cudaStream_t stream, int sm_count);     // delta_backward.cu
 void launch_step(const StepArgs& a, cudaStream_t stream);                   // delta_step.cu
 
 } // namespace delta

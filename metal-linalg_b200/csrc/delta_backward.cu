@@ -734,7 +734,6 @@ void reverse_as(const Args& a, cudaStream_t stream) {
     opt_in<delta_reverse_kernel<T, DKP, KS>>(sizeof(Sh));
     const dim3 grid((a.dvp / 16 + Sh::kGroups - 1) / Sh::kGroups, a.value_heads, a.seqs);
     launch_dependent(delta_reverse_kernel<T, DKP, KS>, grid, kReverseThreads, sizeof(Sh), stream, a);
-    cuda_check(cudaGetLastError(), "delta rule states backward");
 }
 
 template <typename T, int DKP>
@@ -742,36 +741,34 @@ void backward_as(const Args& a, cudaStream_t stream, int sm_count) {
     if (a.chunks) {
         opt_in<delta_do_kernel<T, DKP>>(sizeof(DoShared<T, DKP>));
         launch_dependent(delta_do_kernel<T, DKP>, dim3(a.chunks, a.value_heads), kDoThreads, sizeof(DoShared<T, DKP>), stream, a);
-        cuda_check(cudaGetLastError(), "delta rule P^T dO");
     }
     // Four warps to a chain while there is at most one chain a multiprocessor, two up to two chains (or where sequences of
-    // uneven lengths leave the longest ones running alone), one beyond. 64 chunks of 128 x 128: 128 chains 242 (KS 4) 272 (2) 490 us
-    // (1); 256 chains 318, 272, 491; 512 chains 622, 540, 493; 1408 chains of eleven ragged sequences 287, 258, 312.
+    // uneven lengths leave the longest ones running alone), one beyond, but for float16, whose one-warp chain spills. 64
+    // chunks of 128 x 128 in bfloat16: 128 chains 239 (four) 252 (two) 463 us (one); 256 chains 303, 253, 463; 512 chains 605,
+    // 504, 467; 1408 chains of eleven ragged sequences 307, 240, 297. 32 chunks in float32: 128 chains 166, 273, 482; 512 chains
+    // 654, 546, 488; in float16: 512 chains 335, 316, 341.
     const uint64_t chains = (uint64_t)(a.dvp / 16) * a.value_heads * a.seqs;
     if (chains <= (uint64_t)sm_count) reverse_as<T, DKP, 4>(a, stream);
-    else if (chains <= 2 * (uint64_t)sm_count || a.sequences) reverse_as<T, DKP, 2>(a, stream);
-    else reverse_as<T, DKP, 1>(a, stream);
+    else if (chains <= 2 * (uint64_t)sm_count || a.sequences || __is_same(T, __half)) reverse_as<T, DKP, 2>(a, stream);
+    else if constexpr (!__is_same(T, __half)) reverse_as<T, DKP, 1>(a, stream);
     if (a.chunks) {
         opt_in<delta_grad_kernel<T, DKP>>(sizeof(GradShared<T, DKP>));
         launch_dependent(delta_grad_kernel<T, DKP>, dim3(a.chunks + (a.sequences ? 1 : 0), a.value_heads), kGradThreads, sizeof(GradShared<T, DKP>),
                          stream, a);
-        cuda_check(cudaGetLastError(), "delta rule gradients");
         if (a.value_heads != a.heads) {
             const size_t count = (size_t)a.batch * a.tokens * a.heads * a.dk;
             const unsigned blocks = (unsigned)(count / 256 + 1 < (size_t)sm_count * 8 ? count / 256 + 1 : (size_t)sm_count * 8);
             launch_dependent(delta_fold_kernel<T, DKP>, blocks, 256, 0, stream, a);
-            cuda_check(cudaGetLastError(), "delta rule shared heads");
         }
     }
 }
 
 } // namespace
 
-void launch_backward(const Args& a, cudaStream_t stream, int device) {
-    const int sms = sm_count(device);
+void launch_backward(const Args& a, cudaStream_t stream, int sm_count) {
     launch_prepare(a, stream, true);
-    launch_states(a, stream, sms);
-    DELTA_DISPATCH(backward_as, a, stream, sms);
+    launch_states(a, stream, sm_count);
+    DELTA_DISPATCH(backward_as, a, stream, sm_count);
 }
 
 } // namespace delta

@@ -5,8 +5,6 @@
 #include "delta_tiles.cuh"
 #include "runtime.h"
 
-#include <mutex>
-
 namespace mlb {
 namespace delta {
 
@@ -100,7 +98,7 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const Args p, 
     extern __shared__ __align__(16) char raw[];
     PrepShared<T, DKP>& sh = *reinterpret_cast<PrepShared<T, DKP>*>(raw);
     constexpr int LD = DKP + 8;
-    const uint32_t c = chunk_of_block(p, blockIdx.x), hv = blockIdx.y, h = hv / (p.value_heads / p.heads);
+    const uint32_t c = blockIdx.x, hv = blockIdx.y, h = hv / (p.value_heads / p.heads);
     const size_t at = (size_t)c * p.value_heads + hv;
     const Chunk ch = chunk_at(p, c);
     if (ch.rows == 0) return;
@@ -279,12 +277,6 @@ __global__ void __launch_bounds__(kStateThreads, sizeof(T) == 2 ? 2 : 1) delta_s
         c0 = seq * p.row_chunks;
         c1 = c0 + p.row_chunks;
     }
-    // this launch's part: it starts from the state that the one before it left in place of its first chunk's
-    const bool starts = p.part0 == 0;
-    const uint32_t last = c1;
-    c1 = min(c1, c0 + p.part1);
-    c0 = min(c0 + p.part0, c1);
-    if (!starts && c0 == c1) return;
     if (warp >= 4) {            // the fetching warps: a chunk ahead, complete at the barrier that opens it
         const int tid = threadIdx.x - 128;
         const auto fetch = [&](uint32_t c, int which) {
@@ -318,19 +310,8 @@ __global__ void __launch_bounds__(kStateThreads, sizeof(T) == 2 ? 2 : 1) delta_s
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            s[n][i] = starts && p.initial_state && row(n, i) < (int)p.dk && col(i) < (int)p.dv
+            s[n][i] = p.initial_state && row(n, i) < (int)p.dk && col(i) < (int)p.dv
                           ? p.initial_state[state0 + (size_t)row(n, i) * p.dv + col(i)] : 0.0f;
-    const auto state_of = [&](uint32_t c) {         // where the state at chunk c's start lies, this lane's first values
-        return p.states + ((size_t)c * p.value_heads + hv) * p.dkp * p.dvp + (size_t)(k_base + 2 * t) * p.dvp + dv0 + 2 * g;
-    };
-    if (!starts && live) {
-        const float* from = state_of(c0);
-#pragma unroll
-        for (int n = 0; n < NT; ++n, from += 8 * p.dvp) {
-            const float2 x = *reinterpret_cast<const float2*>(from), y = *reinterpret_cast<const float2*>(from + p.dvp);
-            s[n][0] = x.x; s[n][1] = y.x; s[n][2] = x.y; s[n][3] = y.y;
-        }
-    }
 
     uint4* r_parts = sh.r + chain * 8 * kTileWords;
     uint4* d_parts = sh.part + chain * 8 * kTileWords;
@@ -342,7 +323,7 @@ __global__ void __launch_bounds__(kStateThreads, sizeof(T) == 2 ? 2 : 1) delta_s
 
         // the state at the chunk's start
         if (live) {
-            float* out = state_of(c);
+            float* out = p.states + at * p.dkp * p.dvp + (size_t)(k_base + 2 * t) * p.dvp + dv0 + 2 * g;
 #pragma unroll
             for (int n = 0; n < NT; ++n, out += 8 * p.dvp) put_tile(out, p.dvp, s[n]);
         }
@@ -477,13 +458,7 @@ __global__ void __launch_bounds__(kStateThreads, sizeof(T) == 2 ? 2 : 1) delta_s
             for (int i = 0; i < kOwn; ++i) put_tile(d_out + (size_t)(8 * own_tile<KS>(part, i)) * p.dvp, p.dvp, d[i]);
         }
     }
-    if (c1 < last) {
-        if (live) {
-            float* out = state_of(c1);
-#pragma unroll
-            for (int n = 0; n < NT; ++n, out += 8 * p.dvp) put_tile(out, p.dvp, s[n]);
-        }
-    } else if (p.final_state)
+    if (p.final_state)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -521,13 +496,12 @@ __global__ void __launch_bounds__(kOutThreads, 2) delta_output_kernel(const Args
     using Sp = typename Split<T>::type;
     Sh& sh = *reinterpret_cast<Sh*>(raw);
     constexpr int LD = DKP + 8, kHeld = DKP / 32, LDO = kOutCols + 8;
-    const uint32_t c = chunk_of_block(p, blockIdx.x), hv = blockIdx.y, h = hv / (p.value_heads / p.heads);
+    const uint32_t c = blockIdx.x, hv = blockIdx.y, h = hv / (p.value_heads / p.heads);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     T* o = static_cast<T*>(p.o);
     const Chunk ch = chunk_at(p, c);
-    if (ch.rows == 0) {             // a ragged batch's blocks behind its chunks, in the last part: tokens of no sequence become zero
-        if (p.part1 != p.chunks) return;
-        const uint32_t used = max((uint32_t)p.first[p.sequences], p.part0), spare = p.part0 + gridDim.x - used;
+    if (ch.rows == 0) {             // a ragged batch's blocks behind its chunks: tokens of no sequence become zero
+        const uint32_t used = p.first[p.sequences], spare = gridDim.x - used;
         const Unused none(p);
         for (long long r0 = (long long)(c - used) * kChunk; r0 < none.count; r0 += (long long)spare * kChunk)
             for (int i = threadIdx.x; i < kChunk * (int)p.dv; i += kOutThreads) {
@@ -653,15 +627,11 @@ __global__ void __launch_bounds__(kOutThreads, 2) delta_output_kernel(const Args
 // Launches
 // ---------------------------------------------------------------------------
 
-// Chunks of a launch over a part of every sequence.
-unsigned blocks_of(const Args& a) { return (a.sequences ? 1 : a.batch) * (a.part1 - a.part0); }
-
 template <typename T, int DKP>
 void prepare_as(const Args& a, cudaStream_t stream, bool backward) {
     const size_t bytes = sizeof(PrepShared<T, DKP>);
     opt_in<delta_prep_kernel<T, DKP>>(bytes);
-    launch_dependent(delta_prep_kernel<T, DKP>, dim3(blocks_of(a), a.value_heads), kPrepThreads, bytes, stream, a, backward);
-    cuda_check(cudaGetLastError(), "delta rule preparation");
+    launch_dependent(delta_prep_kernel<T, DKP>, dim3(a.chunks, a.value_heads), kPrepThreads, bytes, stream, a, backward);
 }
 
 template <typename T, int DKP, int KS>
@@ -670,15 +640,15 @@ void states_as(const Args& a, cudaStream_t stream) {
     opt_in<delta_state_kernel<T, DKP, KS>>(sizeof(Sh));
     const dim3 grid((a.dvp / 16 + Sh::kGroups - 1) / Sh::kGroups, a.value_heads, a.seqs);
     launch_dependent(delta_state_kernel<T, DKP, KS>, grid, kStateThreads, sizeof(Sh), stream, a);
-    cuda_check(cudaGetLastError(), "delta rule states");
 }
 
 template <typename T, int DKP>
 void states_of(const Args& a, cudaStream_t stream, int sm_count) {
-    // Four warps to a chain while there are at most two chains a multiprocessor, two beyond. 64 chunks of 128 x 128: 128 chains
-    // 134 (four) 210 us (two); 256 chains 190, 212; 512 chains 372, 310. (One warp a chain: 367 us whatever their number up to 512.)
+    // Four warps to a chain while their blocks are all resident (two a multiprocessor, one in float32), two beyond. 64 chunks of 128 x 128 in bfloat16: 128
+    // chains 108 (four) 186 us (two); 256 chains 174, 188; 512 chains 344, 304. 32 chunks in float32: 128 chains 83, 138;
+    // 256 chains 163, 144; 512 chains 323, 271. (One warp a chain: 367 us in bfloat16 whatever their number up to 512.)
     const uint64_t chains = (uint64_t)(a.dvp / 16) * a.value_heads * a.seqs;
-    if (chains <= 2 * (uint64_t)sm_count) states_as<T, DKP, 4>(a, stream);
+    if (chains <= (sizeof(T) == 2 ? 2 : 1) * (uint64_t)sm_count) states_as<T, DKP, 4>(a, stream);
     else states_as<T, DKP, 2>(a, stream);
 }
 
@@ -687,95 +657,22 @@ void output_as(const Args& a, cudaStream_t stream) {
     const size_t bytes = sizeof(OutShared<T, DKP>);
     opt_in<delta_output_kernel<T, DKP>>(bytes);
     // one block more than there can be chunks: a ragged batch's tokens of no sequence have a block to clear them
-    const unsigned spare = a.sequences && a.part1 == a.chunks;
-    launch_dependent(delta_output_kernel<T, DKP>, dim3(blocks_of(a) + spare, a.value_heads), kOutThreads, bytes, stream, a);
-    cuda_check(cudaGetLastError(), "delta rule outputs");
-}
-
-// The stream beside the caller's on which a long sequence's sequential pass runs, and its events; one set a GPU, made at first
-// use and kept. Calls from several threads take turns at enqueueing on it.
-struct Beside {
-    std::mutex   mutex;
-    cudaStream_t stream = nullptr;
-    cudaEvent_t  prepared = nullptr, passed = nullptr;
-};
-Beside& beside_of(int device) {
-    static Beside all[64];
-    Beside& b = all[device & 63];
-    std::lock_guard<std::mutex> lock(b.mutex);
-    if (!b.stream) {
-        int least, most;
-        cuda_check(cudaDeviceGetStreamPriorityRange(&least, &most), "cudaDeviceGetStreamPriorityRange");
-        if (!b.prepared) cuda_check(cudaEventCreateWithFlags(&b.prepared, cudaEventDisableTiming), "cudaEventCreate");
-        if (!b.passed) cuda_check(cudaEventCreateWithFlags(&b.passed, cudaEventDisableTiming), "cudaEventCreate");
-        cuda_check(cudaStreamCreateWithPriority(&b.stream, cudaStreamNonBlocking, most), "cudaStreamCreate");
-    }
-    return b;
-}
-// A stream that is being captured keeps to itself: the one beside it would belong to that capture until its end.
-bool may_overlap(cudaStream_t stream) {
-    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) {
-        cudaGetLastError();
-        return false;
-    }
-    return status == cudaStreamCaptureStatusNone;
+    launch_dependent(delta_output_kernel<T, DKP>, dim3(a.chunks + (a.sequences ? 1 : 0), a.value_heads), kOutThreads, bytes, stream, a);
 }
 
 } // namespace
 
 void launch_prepare(const Args& a, cudaStream_t stream, bool backward) {
-    if (a.sequences && a.part0 == 0) {
-        launch_dependent(delta_index_kernel, 1, kIndexThreads, 0, stream, a);
-        cuda_check(cudaGetLastError(), "delta rule index");
-    }
+    if (a.sequences) launch_dependent(delta_index_kernel, 1, kIndexThreads, 0, stream, a);
     if (a.chunks) DELTA_DISPATCH(prepare_as, a, stream, backward);
 }
 
 void launch_states(const Args& a, cudaStream_t stream, int sm_count) { DELTA_DISPATCH(states_of, a, stream, sm_count); }
 
-// A part's chunks. The parts of a long sequence overlap: one's outputs and the next but one's preparation run beside the
-// sequential pass over the next, which leaves a multiprocessor most of its registers and shared memory. @@
-constexpr uint32_t kPart = 64;
-
-void launch_forward(const Args& whole, cudaStream_t stream, int device) {
-    const int sms = sm_count(device);
-    Args a = whole;
-    const uint32_t length = a.part1;
-    const uint64_t chains = (uint64_t)(a.dvp / 16) * a.value_heads * a.seqs;
-    if ((a.sequences > 1) || length < 2 * kPart || chains > (uint64_t)sms || !may_overlap(stream)) {
-        launch_prepare(a, stream, false);
-        launch_states(a, stream, sms);
-        if (a.chunks) DELTA_DISPATCH(output_as, a, stream);
-        return;
-    }
-    Beside& beside = beside_of(device);
-    std::lock_guard<std::mutex> lock(beside.mutex);         // one call's events at a time
-    const auto take = [&](uint32_t from) {
-        a.part0 = from;
-        a.part1 = length - from < 2 * kPart ? length : from + kPart;
-    };
-    const auto follow = [&](cudaStream_t later, cudaEvent_t event, cudaStream_t earlier) {
-        cuda_check(cudaEventRecord(event, earlier), "cudaEventRecord");
-        cuda_check(cudaStreamWaitEvent(later, event, 0), "cudaStreamWaitEvent");
-    };
-    take(0);
+void launch_forward(const Args& a, cudaStream_t stream, int sm_count) {
     launch_prepare(a, stream, false);
-    follow(beside.stream, beside.prepared, stream);
-    for (;;) {
-        launch_states(a, beside.stream, sms);
-        cuda_check(cudaEventRecord(beside.passed, beside.stream), "cudaEventRecord");
-        const Args now = a;
-        const bool more = a.part1 < length;
-        if (more) {
-            take(a.part1);
-            launch_prepare(a, stream, false);
-            follow(beside.stream, beside.prepared, stream);
-        }
-        cuda_check(cudaStreamWaitEvent(stream, beside.passed, 0), "cudaStreamWaitEvent");
-        DELTA_DISPATCH(output_as, now, stream);
-        if (!more) return;
-    }
+    launch_states(a, stream, sm_count);
+    if (a.chunks) DELTA_DISPATCH(output_as, a, stream);
 }
 
 } // namespace delta

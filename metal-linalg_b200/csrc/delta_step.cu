@@ -182,7 +182,6 @@ void launch_step(const StepArgs& a, cudaStream_t stream) {
         case METAL_LINALG_FLOAT16: launch_dependent(delta_step_kernel<__half>, grid, kStepThreads, 0, stream, a); break;
         default: launch_dependent(delta_step_kernel<float>, grid, kStepThreads, 0, stream, a); break;
     }
-    cuda_check(cudaGetLastError(), "delta rule step");
 }
 
 } // namespace delta

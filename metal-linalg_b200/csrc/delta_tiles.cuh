@@ -401,12 +401,6 @@ __device__ __forceinline__ Chunk chunk_at(const Args& a, uint32_t c) {
     return r;
 }
 
-// The chunk that block x of a launch over a part of every sequence takes (ragged batches: a part of all chunks).
-__device__ __forceinline__ uint32_t chunk_of_block(const Args& a, uint32_t x) {
-    if (a.sequences) return a.part0 + x;
-    const uint32_t width = a.part1 - a.part0, b = x / width;
-    return b * a.row_chunks + a.part0 + (x - b * width);
-}
 // A ragged batch's tokens of no sequence, token(i) of i < count: those before the first sequence, then those behind the last one.
 struct Unused {
     long long front, end, count;

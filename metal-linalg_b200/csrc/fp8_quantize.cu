@@ -329,7 +329,6 @@ void quantize_as(const QuantizeArgs& a, cudaStream_t stream) {
     } else {
         launch_dependent(quantize_tiles_kernel<T, kE5m2>, dim3((unsigned)tiles, a.batch), kTileThreads, 0, stream, a);
     }
-    cuda_check(cudaGetLastError(), "quantize launch");
 }
 
 } // namespace

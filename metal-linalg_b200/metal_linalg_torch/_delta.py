@@ -24,6 +24,8 @@ __all__ = ["gated_delta_rule", "gated_delta_step"]
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _FLOATING = frozenset((torch.float32, torch.bfloat16, torch.float16, torch.float64))
 _PLACES = frozenset(("cuda", "meta"))
+_INDICES = frozenset((torch.int32, torch.int64))
+_changed = torch.autograd.graph.increment_version
 _PROBLEM = struct.Struct("=9IfiI7Q15q")
 
 
@@ -110,7 +112,7 @@ def _workspace(problem, backward, device):
 def _sequences(name, q, cu_seqlens):
     if cu_seqlens is None:
         return q.shape[0]
-    if not isinstance(cu_seqlens, Tensor) or cu_seqlens.dtype not in (torch.int32, torch.int64):
+    if not isinstance(cu_seqlens, Tensor) or cu_seqlens.dtype not in _INDICES:
         _fail(name, "cu_seqlens must be an int32 or int64 tensor", TypeError)
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
         _fail(name, f"cu_seqlens must hold the N + 1 bounds of N >= 1 sequences, got shape {tuple(cu_seqlens.shape)}")
@@ -275,17 +277,8 @@ def _(q, k, v, g, beta, state, slots, scale):
     return torch.empty_like(v, memory_format=torch.contiguous_format)
 
 
-def gated_delta_step(q, k, v, g, beta, state, *, slots=None, scale=None):
-    """A few tokens of every sequence through the gated delta rule, for decoding; updates ``state`` in place and returns
-    ``o`` [B, T, HV, Dv].
-
-    The inputs are `gated_delta_rule`'s (T is 1, or the tokens of a draft). ``state`` is a pool [S, HV, Dk, Dv] of float32
-    states, each contiguous (a layer's part of a larger cache is fine). Row ``b`` uses slot ``slots[b]`` (int32 or int64, on
-    the GPU; default: slot ``b``). A row whose slot is not one of the pool's, -1 say, is padding: its outputs are zero and no
-    state changes. Rows that name the same slot run one after another, in their order. Not differentiable.
-    """
-    name = "gated_delta_step"
-    b, t, h, dk, hv, dv = _check(name, q, k, v, g, beta)
+def _explain_step(name, q, b, hv, dk, dv, state, slots):
+    """Refuses a pool or slots that cannot be used; returns where the pool's strides only look unusual (dimensions of one)."""
     if not isinstance(state, Tensor) or state.dtype != torch.float32:
         _fail(name, "state must be a float32 tensor", TypeError)
     if state.dim() != 4 or state.shape[1:] != (hv, dk, dv):
@@ -298,12 +291,34 @@ def gated_delta_step(q, k, v, g, beta, state, *, slots=None, scale=None):
     if state.shape[0] > 1 and s0 < hv * dk * dv:
         _fail(name, "the slots of state overlap")
     if slots is not None:
-        if not isinstance(slots, Tensor) or slots.dtype not in (torch.int32, torch.int64):
+        if not isinstance(slots, Tensor) or slots.dtype not in _INDICES:
             _fail(name, "slots must be an int32 or int64 tensor", TypeError)
         if slots.shape != (b,) or slots.device != q.device:
             _fail(name, f"expected slots [{b}] on {q.device}, got {tuple(slots.shape)} on {slots.device}")
     elif b > state.shape[0]:
         _fail(name, f"{b} rows and {state.shape[0]} slots: name them with slots")
+
+
+def gated_delta_step(q, k, v, g, beta, state, *, slots=None, scale=None):
+    """A few tokens of every sequence through the gated delta rule, for decoding; updates ``state`` in place and returns
+    ``o`` [B, T, HV, Dv].
+
+    The inputs are `gated_delta_rule`'s (T is 1, or the tokens of a draft). ``state`` is a pool [S, HV, Dk, Dv] of float32
+    states, each contiguous (a layer's part of a larger cache is fine). Row ``b`` uses slot ``slots[b]`` (int32 or int64, on
+    the GPU; default: slot ``b``). A row whose slot is not one of the pool's, -1 say, is padding: its outputs are zero and no
+    state changes. Rows that name the same slot run one after another, in their order. Not differentiable.
+    """
+    name = "gated_delta_step"
+    b, t, h, dk, hv, dv = _check(name, q, k, v, g, beta)
+    try:
+        shape, (s0, s1, s2, s3) = state.shape, state.stride()
+        fine = (state.dtype == torch.float32 and shape[1:] == (hv, dk, dv) and state.device == q.device
+                and s3 == 1 and s2 == dv and s1 == dk * dv and s0 >= hv * s1
+                and (b <= shape[0] if slots is None else slots.dtype in _INDICES and slots.shape == (b,) and slots.device == q.device))
+    except (AttributeError, ValueError):
+        fine = False
+    if not fine:
+        _explain_step(name, q, b, hv, dk, dv, state, slots)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
                                     beta.requires_grad or state.requires_grad):
         _fail(name, "not differentiable; use gated_delta_rule for training, or torch.no_grad()", RuntimeError)
@@ -311,5 +326,5 @@ def gated_delta_step(q, k, v, g, beta, state, *, slots=None, scale=None):
     g, beta = _float(g), _float(beta)
     if torch.compiler.is_compiling() or q.device.type == "meta":
         return torch.ops.metal_linalg.gated_delta_step(q, k, v, g, beta, state, slots, scale)
-    torch.autograd.graph.increment_version(state)       # a graph that saved the pool for its backward pass finds it changed
+    _changed(state)                 # a graph that saved the pool for its backward pass finds it changed
     return _step(q, k, v, g, beta, state, slots, scale)

@@ -120,6 +120,29 @@ def _block_rows(name, what, rows, scales_rows):
     _fail(name, f"{what}_scale must have {rows} or {-(-rows // 128)} rows, got {scales_rows}")
 
 
+def _check_product(name, a, a_scale, b, b_scale):
+    """Refuses operands that do not fit; returns the rows of their scales' blocks."""
+    for what, x in (("a", a), ("a_scale", a_scale), ("b", b), ("b_scale", b_scale)):
+        _on_gpu(name, what, x)
+    device = a.device
+    if a_scale.device != device or b.device != device or b_scale.device != device:
+        _fail(name, f"a, a_scale, b and b_scale must be on one device, got {device}, {a_scale.device}, {b.device} and {b_scale.device}")
+    if a.dtype not in _KINDS or b.dtype not in _KINDS:
+        _fail(name, f"a and b must be float8_e4m3fn or float8_e5m2, got {a.dtype} and {b.dtype}", TypeError)
+    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
+        _fail(name, f"the scales must be float32, got {a_scale.dtype} and {b_scale.dtype}", TypeError)
+    sizes, others = a.shape, b.shape
+    if len(sizes) < 2 or len(others) < 2 or sizes[-1] != others[-1] or (len(others) > 2 and others[:-2] != sizes[:-2]):
+        _fail(name, f"expected a [..., M, K] and b [..., N, K] or [N, K], got {tuple(sizes)} and {tuple(others)}")
+    blocks = -(-sizes[-1] // 128)
+    rows = []
+    for what, x, s in (("a", sizes, a_scale.shape), ("b", others, b_scale.shape)):
+        if len(s) != len(x) or s[:-2] != x[:-2] or s[-1] != blocks:
+            _fail(name, f"expected {what}_scale [..., rows, {blocks}] for {tuple(x)}, got {tuple(s)}")
+        rows.append(_block_rows(name, what, x[-2], s[-2]))
+    return rows
+
+
 def _operand(x, scale, block_rows, batched):
     """A metal_linalg_fp8_operand as bytes, and the tensors it points to. What the library cannot read in place (rows that
     are not a multiple of 16 bytes apart, say) is copied once."""
@@ -142,9 +165,7 @@ def _matmul(a, a_scale, b, b_scale, a_rows, b_rows, out_dtype):
     *lead, m, k = a.shape
     n = b.shape[-2]
     out = a.new_empty((*lead, m, n), dtype=out_dtype)
-    if not out.numel():
-        return out
-    if k == 0:
+    if not (m and n and k) or not out.numel():
         return out.zero_()
     batch = 1
     if lead:
@@ -181,25 +202,9 @@ def matmul_fp8(a, a_scale, b, b_scale, *, out_dtype=torch.bfloat16):
     copied. Not differentiable.
     """
     name = "matmul_fp8"
-    for what, x in (("a", a), ("a_scale", a_scale), ("b", b), ("b_scale", b_scale)):
-        _on_gpu(name, what, x)
-    device = a.device
-    if a_scale.device != device or b.device != device or b_scale.device != device:
-        _fail(name, f"a, a_scale, b and b_scale must be on one device, got {device}, {a_scale.device}, {b.device} and {b_scale.device}")
-    if a.dtype not in _KINDS or b.dtype not in _KINDS:
-        _fail(name, f"a and b must be float8_e4m3fn or float8_e5m2, got {a.dtype} and {b.dtype}", TypeError)
-    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
-        _fail(name, f"the scales must be float32, got {a_scale.dtype} and {b_scale.dtype}", TypeError)
+    a_rows, b_rows = _check_product(name, a, a_scale, b, b_scale)
     if out_dtype not in _DTYPES:
         _fail(name, f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}", TypeError)
-    if a.dim() < 2 or b.dim() < 2 or a.shape[-1] != b.shape[-1] or (b.dim() > 2 and b.shape[:-2] != a.shape[:-2]):
-        _fail(name, f"expected a [..., M, K] and b [..., N, K] or [N, K], got {tuple(a.shape)} and {tuple(b.shape)}")
-    blocks = -(-a.shape[-1] // 128)
-    for what, x, s in (("a", a, a_scale), ("b", b, b_scale)):
-        if s.dim() != x.dim() or s.shape[:-2] != x.shape[:-2] or s.shape[-1] != blocks:
-            _fail(name, f"expected {what}_scale [..., rows, {blocks}] for {tuple(x.shape)}, got {tuple(s.shape)}")
-    a_rows = _block_rows(name, "a", a.shape[-2], a_scale.shape[-2])
-    b_rows = _block_rows(name, "b", b.shape[-2], b_scale.shape[-2])
     if torch.is_grad_enabled() and (a.requires_grad or a_scale.requires_grad or b.requires_grad or b_scale.requires_grad):
         _fail(name, "not differentiable; use linear_fp8, or detach the operands", RuntimeError)
     if torch.compiler.is_compiling() or a.device.type == "meta":

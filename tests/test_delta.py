@@ -688,7 +688,7 @@ def test_tensors_of_another_gpu_than_the_current_one():
 
 
 # ---------------------------------------------------------------------------
-# Long sequences, whose parts overlap on two streams; tokens of no sequence; pools that graphs have saved
+# Long sequences, eager and captured; tokens of no sequence; pools that graphs have saved
 # ---------------------------------------------------------------------------
 
 LONG = [
@@ -701,9 +701,9 @@ LONG = [
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", LONG, ids=str)
-def test_long_sequences_in_parts_are_the_whole(shape):
-    """Captured calls run whole, eager ones in parts: the same products in the same order, bit for bit. And the float64
-    recurrence's, from a few tokens before the end on (a sequence in two calls)."""
+def test_long_sequences(shape):
+    """Again and captured: the same products in the same order, bit for bit. And the float64 recurrence's, from a few tokens
+    before the end on (a sequence in two calls)."""
     b, t, h, hv, dk, dv, bounds = shape
     q, k, v, g, beta, s0 = inputs(b, t, h, hv, dk, dv, torch.bfloat16, seed=t)
     cu = None if bounds is None else torch.tensor(bounds, dtype=torch.int32, device="cuda")
