@@ -151,9 +151,9 @@ typedef enum metal_linalg_dtype {
  *
  * Sequences: with `sequences` 0 every batch row is one. Otherwise batch is 1 and
  * sequence i is the tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (index_bytes 4:
- * int32, 8: int64; sequences + 1 values, the first 0, none falling). Tokens
- * behind the last sequence give outputs and gradients of zero. A sequence may be empty: its state
- * passes through.
+ * int32, 8: int64; sequences + 1 values, none falling). Tokens of no sequence,
+ * before the first or behind the last one, give outputs and gradients of zero. A
+ * sequence may be empty: its state passes through.
  *
  * All pointers are CUDA device pointers on one GPU: `device` names it, which the
  * caller vouches for, or is -1 and the call looks each pointer up (about 0.3 us a

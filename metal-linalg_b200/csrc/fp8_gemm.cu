@@ -14,6 +14,12 @@
 // eight blocks of a cluster share a tile's k and add their sums through distributed shared memory, each a part of the columns, always in
 // the same order: no atomics, no workspace.
 //
+// What bounds a large product is the hand-over of accumulators: a block of 128 x 256 x 128 takes the tensor core 512 clocks and the
+// two epilogue warps of a quarter 1250 to 1400 to read, scale and add 256 x 32 sums each and hand the accumulator back:
+// 8192 x 8192 x 4096 in 300 us, 1.83 PFLOP/s (341 us when it runs for seconds and the clocks fall); scales for every
+// row of both operands 20 % more. 4096 x 4096 x 2048 53 us; 1024 x 1024 x 4096 14; 16 rows x 4096 x 8192 11.4 us
+// (the weight's 33.6 MB at 2.9 TB/s: the ring's start and the cluster's exchange are half of it).
+//
 // Every wait on an mbarrier is bounded. One that runs out makes the block's outputs NaN, sets the status word, waits
 // (bounded) for the block's own loads and products and ends.
 #include "common.cuh"
@@ -171,7 +177,7 @@ struct Shape {
     static constexpr int kStageBytes = (kRowsTile + BN) * kBlockK;
     static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 4 : BN == 64 ? 7 : 8;
     static constexpr int kReduceBytes = BN <= 128 ? BN * kRowsTile * 4 : 0;     // partial sums from the cluster's other blocks
-    static constexpr int kScaleBytes = kEpilogueWarps * 2 * kCols * 4;
+    static constexpr int kScaleBytes = kEpilogueWarps / 4 * 2 * kCols * 4;
     static constexpr size_t kShared = (size_t)kStages * kStageBytes + kReduceBytes + kScaleBytes + 1024;
     static_assert(kShared + 512 <= 232448, "with the barriers, more than a block's shared memory");
 };
@@ -226,12 +232,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
         if constexpr (S::kUneven) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quarter = warp & 3, part = warp >> 2;
         const uint32_t row = 32 * quarter + lane;
-        float* my_scales = scales + warp * 2 * S::kCols;
+        float* part_scales = scales + part * 2 * S::kCols;      // of this part's columns, two blocks of k
         uint32_t i = 0;
         bool ok = true;
         for (uint32_t tile = first; tile < a.tiles; tile += step) {
             const float *sp, *sq;               // this block's first scales of the thread's row, of its columns
-            uint32_t q_scales = 0;              // by column: how many of this lane's columns exist
+            bool q_there = false;               // by column: the four warps of a part fetch a quarter of its columns each
             {
                 uint32_t z, p, q0;
                 a.place<BN>(tile, z, p, q0);
@@ -240,9 +246,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
                 sp = a.sp + (a.batched_p ? z * a.sp_batch : 0) + (uint64_t)(p >> a.p_shift) * a.kb + kb0;
                 sq = a.sq + (a.batched_q ? z * a.sq_batch : 0) + kb0;
                 if constexpr (kByColumn) {
-                    sq += (uint64_t)(q0 + lane) * a.kb;
-                    q_scales = q0 + lane < a.q ? (min(a.q - q0, (uint32_t)S::kCols) - lane + 31) / 32 : 0;
-                    if (lane >= S::kCols) q_scales = 0;
+                    const uint32_t column = q0 + quarter * (S::kCols / 4) + lane;
+                    sq += (uint64_t)column * a.kb;
+                    q_there = lane < S::kCols / 4 && column < a.q;
                 } else {
                     sq += (uint64_t)(min(q0, a.q - 1) >> 7) * a.kb;
                 }
@@ -251,36 +257,30 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
 #pragma unroll
             for (int j = 0; j < S::kCols / 2; ++j) sum[j] = 0;
             // the next block's scales are fetched while this one's product is awaited
-            float row_scale = 0.0f, col_scale[kByColumn ? (S::kCols + 31) / 32 : 1];
+            float row_scale = 0.0f, col_scale = 0.0f;
             const auto fetch = [&]() {
                 row_scale = __ldg(sp++);
-                if constexpr (kByColumn) {
-#pragma unroll
-                    for (uint32_t j = 0; j < (S::kCols + 31) / 32; ++j) col_scale[j] = j < q_scales ? __ldg(sq + (uint64_t)(32 * j) * a.kb) : 0.0f;
-                } else {
-                    col_scale[0] = __ldg(sq);
-                }
+                if (!kByColumn || q_there) col_scale = __ldg(sq);
                 ++sq;
             };
             if (kb0 < kb1) fetch();
 #pragma unroll 1
-            for (uint32_t kb = kb0; ok && kb < kb1; ++kb, ++i) {
+            for (uint32_t kb = kb0; kb < kb1; ++kb, ++i) {
                 const uint32_t acc = i % S::kAcc;
                 float scale = row_scale;
-                float* by_column = my_scales + (kb & 1) * S::kCols;
+                float* by_column = part_scales + (i & 1) * S::kCols;
                 if constexpr (kByColumn) {
-#pragma unroll
-                    for (int j = 0; j < (S::kCols + 31) / 32; ++j)
-                        if (32 * j + lane < S::kCols) by_column[32 * j + lane] = col_scale[j];
-                    __syncwarp();
+                    if (lane < S::kCols / 4) by_column[quarter * (S::kCols / 4) + lane] = col_scale;
+                    // every one of the four warps comes here for every block of k, a failed wait behind it or not
+                    asm volatile("bar.sync %0, 128;" :: "r"(1 + part) : "memory");
                 } else {
-                    scale *= col_scale[0];
+                    scale *= col_scale;
                 }
                 const Pair scale2 = pair_of(scale, scale);
                 if (kb + 1 < kb1) fetch();
-                ok = wait(smem_u32(&acc_full[acc]), (i / S::kAcc) & 1, failed);
+                ok = ok && wait(smem_u32(&acc_full[acc]), (i / S::kAcc) & 1, failed);
                 ok = __all_sync(0xffffffffu, ok);       // (one lane asking for its warp was 8 % slower)
-                if (!ok) break;
+                if (!ok) continue;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t at = tmem + acc * BN + part * S::kCols + ((32u * quarter) << 16);
                 // two loads in flight; the next two go out as their registers are used up

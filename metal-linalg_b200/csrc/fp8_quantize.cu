@@ -3,11 +3,12 @@
 //     scale = max(max|x| / M, 2^-126),   value = x / scale, a float32, rounded to the nearest (ties to even)
 //
 // The quotient is correctly rounded, so that the values are the definition's bit for bit. Every kernel reads x once: what
-// bounds them is memory.
-//   rows     x contiguous along columns, 1 x 128: 16 lanes a block, eight values a lane
-//   tiles    the same in 128 x 128: 512 threads hold the tile in registers
+// bounds them is memory, and for 16-bit inputs the instructions of the quotients about as much.
+//   rows     x contiguous along columns, 1 x 128: 16 lanes a block, eight values a lane. 4096 x 4096 in bfloat16 14 us,
+//            8192 x 8192 in float32 56 us (6.0 TB/s)
+//   tiles    the same in 128 x 128: 256 threads hold the tile as it lies in memory. 4096 x 8192 in bfloat16 23 us (4.4 TB/s)
 //   turned   x contiguous along rows (a transposed matrix): a 128 x 128 tile through shared memory as it lies, read back a
-//            quarter of a row of the result a thread, either block shape
+//            quarter of a row of the result a thread, either block shape. 2048 x 4096 in bfloat16 11 us
 #include "common.cuh"
 #include "fp8.h"
 #include "runtime.h"
