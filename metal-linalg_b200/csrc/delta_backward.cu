@@ -102,16 +102,16 @@ __global__ void __launch_bounds__(kDoThreads) delta_do_kernel(const Args p) {
 // ---------------------------------------------------------------------------
 //
 // The forward's chain with dS'^T in the accumulators: Y^T = dS'^T K^T, dD^T = e^{G_63 - G} Y^T + (scale P^T dO)^T,
-// dR^T = dD^T T, dS^T = e^{G_63} dS'^T + (scale e^G dO)^T Q - (beta e^G dR)^T K. Bound by the chain, as the forward's: 3.7 us a
-// chunk, of which the waits for the one stage that fits beside four warps' exchange are a third (with two warps a chain
-// there are two stages: 3.9 us for twice the chains). 64 chunks of 16 heads of 128 x 128 239 us.
+// dR^T = dD^T T, dS^T = e^{G_63} dS'^T + (scale e^G dO)^T Q - (beta e^G dR)^T K. Bound by the chain, as the forward's: 2.5 us a
+// chunk with four warps a chain (3.7 with one stage, where the fetch was waited for), 3.9 us for twice the chains with two.
+// 64 chunks of 16 heads of 128 x 128 164 us.
 constexpr int kReverseThreads = 192;      // two fetching warps, as the forward's
 
 template <typename T, int DKP, int KS>
 struct ReverseShared {
     static constexpr int kGroups = 4 / KS;
     static constexpr int kLdV = 16 * kGroups + 8;
-    static constexpr int kStages = sizeof(T) == 4 || KS == 4 ? 1 : 2;      // two of float32 are more than a multiprocessor holds
+    static constexpr int kStages = sizeof(T) == 4 && KS < 4 ? 1 : 2;       // two of float32 are more than a multiprocessor holds
     struct Stage {
         alignas(16) T     k[kChunk * (DKP + 8)];
         alignas(16) T     q[kChunk * (DKP + 8)];
@@ -717,23 +717,43 @@ __global__ void __launch_bounds__(kGradThreads) delta_grad_kernel(const Args p) 
     }
 }
 
-// The gradients of shared heads: the sums over the value heads that read them, in their order. Bound by memory: 8192 tokens of 8
-// heads of 128, two value heads each, 40 us (4.2 TB/s).
+// The gradients of shared heads: the sums over the value heads that read them, in their order. A warp takes a token and head.
+// Bound by memory: 8192 tokens of 8 heads of
+// 128, two value heads each, 25 us (6.7 TB/s of reads and writes, some of them the L2's).
 template <typename T, int DKP>
 __global__ void __launch_bounds__(256) delta_fold_kernel(const Args p) {
     dependency_wait_only();
     const size_t rows = (size_t)p.batch * p.tokens * p.heads;
-    const uint32_t up = p.value_heads / p.heads;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < rows * p.dk; i += (size_t)gridDim.x * 256) {
-        const size_t row = i / p.dk, column = i - row * p.dk;
-        const size_t from = row * up * p.dk + column;       // [token][head][its value heads][dk]
-        float q = 0.0f, k = 0.0f;
-        for (uint32_t j = 0; j < up; ++j) {
-            q += p.fold_q[from + (size_t)j * p.dk];
-            k += p.fold_k[from + (size_t)j * p.dk];
+    const uint32_t up = p.value_heads / p.heads, lane = threadIdx.x & 31;
+    const bool quads = p.dk % 4 == 0 && ((reinterpret_cast<size_t>(p.dq) | reinterpret_cast<size_t>(p.dk_out)) & 15) == 0;
+    for (size_t row = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += (size_t)gridDim.x * 8) {
+        const size_t from = row * up * p.dk, to = row * p.dk;       // [token][head][its value heads][dk]
+        if (quads) {
+            const uint32_t column = 4 * lane;
+            if (column >= p.dk) continue;
+            float q[4] = {}, k[4] = {};
+            for (uint32_t j = 0; j < up; ++j) {
+                const float4 x = *reinterpret_cast<const float4*>(p.fold_q + from + (size_t)j * p.dk + column);
+                const float4 y = *reinterpret_cast<const float4*>(p.fold_k + from + (size_t)j * p.dk + column);
+                q[0] += x.x; q[1] += x.y; q[2] += x.z; q[3] += x.w;
+                k[0] += y.x; k[1] += y.y; k[2] += y.z; k[3] += y.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                put_pair(static_cast<T*>(p.dq) + to + column + i, q[i], q[i + 1]);
+                put_pair(static_cast<T*>(p.dk_out) + to + column + i, k[i], k[i + 1]);
+            }
+        } else {
+            for (uint32_t column = lane; column < p.dk; column += 32) {
+                float q = 0.0f, k = 0.0f;
+                for (uint32_t j = 0; j < up; ++j) {
+                    q += p.fold_q[from + (size_t)j * p.dk + column];
+                    k += p.fold_k[from + (size_t)j * p.dk + column];
+                }
+                static_cast<T*>(p.dq)[to + column] = from_f<T>(q);
+                static_cast<T*>(p.dk_out)[to + column] = from_f<T>(k);
+            }
         }
-        static_cast<T*>(p.dq)[i] = from_f<T>(q);
-        static_cast<T*>(p.dk_out)[i] = from_f<T>(k);
     }
 }
 
@@ -751,11 +771,11 @@ void backward_as(const Args& a, cudaStream_t stream, int sm_count) {
         opt_in<delta_do_kernel<T, DKP>>(sizeof(DoShared<T, DKP>));
         launch_dependent(delta_do_kernel<T, DKP>, dim3(a.chunks, a.value_heads), kDoThreads, sizeof(DoShared<T, DKP>), stream, a);
     }
-    // Four warps to a chain while there is at most one chain a multiprocessor, two up to two chains (or where sequences of
-    // uneven lengths leave the longest ones running alone), one beyond, but for float16, whose one-warp chain spills. 64
-    // chunks of 128 x 128 in bfloat16: 128 chains 239 (four) 252 (two) 463 us (one); 256 chains 303, 253, 463; 512 chains 605,
-    // 504, 467; 1408 chains of eleven ragged sequences 307, 240, 297. 32 chunks in float32: 128 chains 166, 273, 482; 512 chains
-    // 654, 546, 488; in float16: 512 chains 335, 316, 341.
+    // Four warps to a chain while there is at most one chain a multiprocessor (their two stages fill it), two up to two chains
+    // (or where sequences of uneven lengths leave the longest ones running alone), one beyond, but for float16, whose
+    // one-warp chain spills. 64 chunks of 128 x 128 in bfloat16: 128 chains 164 (four) 252 (two) 463 us (one); 256 chains 253 (two)
+    // 463 (one); 512 chains 504, 467; 1408 chains of eleven ragged sequences 240, 297. 32 chunks in float32: 128 chains
+    // 129, 273, 482; 512 chains 546 (two) 488 (one); in float16: 316, 341.
     const uint64_t chains = (uint64_t)(a.dvp / 16) * a.value_heads * a.seqs;
     if (chains <= (uint64_t)sm_count) reverse_as<T, DKP, 4>(a, stream);
     else if (chains <= 2 * (uint64_t)sm_count || a.sequences || __is_same(T, __half)) reverse_as<T, DKP, 2>(a, stream);
@@ -765,9 +785,8 @@ void backward_as(const Args& a, cudaStream_t stream, int sm_count) {
         launch_dependent(delta_grad_kernel<T, DKP>, dim3(a.chunks + (a.sequences ? 1 : 0), a.value_heads), kGradThreads, sizeof(GradShared<T, DKP>),
                          stream, a);
         if (a.value_heads != a.heads) {
-            const size_t count = (size_t)a.batch * a.tokens * a.heads * a.dk;
-            const unsigned blocks = (unsigned)(count / 256 + 1 < (size_t)sm_count * 8 ? count / 256 + 1 : (size_t)sm_count * 8);
-            launch_dependent(delta_fold_kernel<T, DKP>, blocks, 256, 0, stream, a);
+            const size_t blocks = (size_t)a.batch * a.tokens * a.heads / 8 + 1, most = (size_t)sm_count * 32;
+            launch_dependent(delta_fold_kernel<T, DKP>, (unsigned)(blocks < most ? blocks : most), 256, 0, stream, a);
         }
     }
 }

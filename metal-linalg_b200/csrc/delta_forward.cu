@@ -14,8 +14,8 @@ namespace {
 // Ragged batches: chunk c's first token, length and sequence; every sequence's first chunk
 // ---------------------------------------------------------------------------
 //
-// One block: sums of the sequences' chunks, 256 sequences at a time, then a thread a sequence writes its chunks. 2.5 us for
-// eleven sequences: a launch and two memory round trips.
+// One block: sums of the sequences' chunks, 256 sequences at a time, then a thread a sequence writes its chunks. 4 us for
+// eleven sequences: a launch and a few memory round trips.
 
 constexpr int kIndexThreads = 256;
 
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const Args p, 
 // meanwhile (one took longer to issue its copies than the chain to use them). A chain is alone on its quarter of the
 // multiprocessor, so what a product needs besides the one before it is read ahead of the barrier that opens it.
 //
-// What bounds it is the chain: a chunk takes 1.7 us (X 970 clocks, R and its exchange 500, T R 470, S 590, the rest
+// What bounds it is the chain: a chunk takes 1.7 us (X 970 clocks, T R 470, S 590, the rest R, exchanges and
 // barriers), whatever the number of chains up to one a multiprocessor; 64 chunks of 16 heads of 128 x 128 108 us. Beside the
 // outputs of chunks already done, on a second stream, it slowed to 2.7 us a chunk and the whole gained nothing.
 constexpr int kStateThreads = 192;
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kStateThreads, sizeof(T) == 2 ? 2 : 1) delta_s
 // and D read from memory as A operands (each value once, split once), Q from shared memory, and P (20 tiles of 16 x 8 over
 // the warps) kept there as the B fragments that its accumulators are. What bounds it is memory's latency: half of a warp's
 // S is on its way while P is made, each further part while the one before it is multiplied. 64 chunks of 16 heads of
-// 128 x 128: 70 us (the tensor core busy 30 % of it, S, D, Q, K and O at 2.0 TB/s); 128 chunks 127.
+// 128 x 128: 70 us (the tensor core busy 30 % of it, S, D, Q, K and O at 1.9 TB/s); 128 chunks 127.
 constexpr int kOutThreads = 256;
 constexpr int kOutCols = 16 * (kOutThreads / 32);       // value columns at a time
 

@@ -14,11 +14,12 @@
 // eight blocks of a cluster share a tile's k and add their sums through distributed shared memory, each a part of the columns, always in
 // the same order: no atomics, no workspace.
 //
-// What bounds a large product is the hand-over of accumulators: a block of 128 x 256 x 128 takes the tensor core 512 clocks and the
-// two epilogue warps of a quarter 1250 to 1400 to read, scale and add 256 x 32 sums each and hand the accumulator back:
-// 8192 x 8192 x 4096 in 300 us, 1.83 PFLOP/s (341 us when it runs for seconds and the clocks fall); scales for every
-// row of both operands 20 % more. 4096 x 4096 x 2048 53 us; 1024 x 1024 x 4096 14; 16 rows x 4096 x 8192 11.4 us
-// (the weight's 33.6 MB at 2.9 TB/s: the ring's start and the cluster's exchange are half of it).
+// What bounds a large product is the hand-over of accumulators: a block of 128 x 256 x 128 takes the tensor core 512 clocks, and
+// the eight epilogue warps 1250 to 1400 to wait for it, read it, scale it, add it and hand it back, two accumulators
+// taking turns: 8192 x 8192 x 4096 in 304 us, 1.81 PFLOP/s (347 us when it runs for seconds and the clocks fall). With a scale
+// for every row of both operands a second multiplication and a load of scales for four sums make that 2300 clocks: 546 us
+// (tiles of 128 columns: 602). 4096 x 4096 x 2048 55 us; 1024 x 1024 x 4096 14; 16 rows x 4096 x 8192 11.4 us (the
+// weight's 33.6 MB at 3.0 TB/s: the ring's start and the cluster's exchange are half of it).
 //
 // Every wait on an mbarrier is bounded. One that runs out makes the block's outputs NaN, sets the status word, waits
 // (bounded) for the block's own loads and products and ends.
