@@ -108,6 +108,7 @@ uint64_t carve(Args& a, char* base, bool backward) {
     if (a.sequences) {
         a.table = w.take<int>(4ull * a.chunks);
         a.first = w.take<int>((uint64_t)a.sequences + 3);
+        a.order = w.take<int>(a.sequences);
     }
     a.gates = w.take<Gates>(heads);
     a.tri = w.take<float>(heads * kTriFloats);

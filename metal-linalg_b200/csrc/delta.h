@@ -57,6 +57,7 @@ struct Args {
     int*      table;             // ragged: {first token, tokens, sequence, 0} a chunk
     int*      first;             // ragged: [sequences + 3] first chunk of a sequence; then the number of chunks, the tokens
                                  // behind the last sequence's end and those before the first one's start
+    int*      order;             // ragged: [sequences] the sequences, long ones first
     Gates*    gates;             // [chunk][value head]
     float*    tri;               // [chunk][value head][kTriFloats]: T as B fragments, k along columns
     float*    tri_b;             // the same with k along rows (backward)

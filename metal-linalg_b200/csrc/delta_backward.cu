@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kReverseThreads) delta_reverse_kernel(const Ar
     Sh& sh = *reinterpret_cast<Sh*>(raw);
     constexpr int LD = DKP + 8, NT = DKP / 8 / KS, LDV = Sh::kLdV, kOwn = 8 / KS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t hv = blockIdx.y, seq = blockIdx.z, h = hv / (p.value_heads / p.heads);
+    const uint32_t hv = blockIdx.y, seq = p.sequences ? p.order[blockIdx.z] : blockIdx.z, h = hv / (p.value_heads / p.heads);
     const int dv_block = blockIdx.x * 16 * Sh::kGroups;
     uint32_t c0, c1;
     if (p.sequences) {

@@ -14,8 +14,10 @@ namespace {
 // Ragged batches: chunk c's first token, length and sequence; every sequence's first chunk
 // ---------------------------------------------------------------------------
 //
-// One block: sums of the sequences' chunks, 256 sequences at a time, then a thread a sequence writes its chunks. 4 us for
-// eleven sequences: a launch and a few memory round trips.
+// One block: sums of the sequences' chunks, 256 sequences at a time, then a thread a sequence writes its chunks. The
+// sequences are also put in an order for the sequential passes, whose blocks start in it: the long ones first, by classes a
+// quarter of an octave wide (any order gives the same results). 4 us for eleven sequences: a launch and a few memory
+// round trips.
 
 constexpr int kIndexThreads = 256;
 
@@ -30,11 +32,19 @@ __device__ __forceinline__ void bounds_at(const Args& a, uint32_t i, int& begin,
     end = (int)e;
 }
 
+constexpr int kClasses = 4 * 31 + 1;
+__device__ __forceinline__ int class_of(int chunks) {
+    if (chunks <= 0) return 0;
+    const int octave = 31 - __clz(chunks);
+    return 1 + 4 * octave + (int)((((uint64_t)chunks << 2) >> octave) & 3);
+}
+
 __global__ void __launch_bounds__(kIndexThreads) delta_index_kernel(const Args a) {
     dependency_wait();
-    __shared__ int sums[kIndexThreads];
+    __shared__ int sums[kIndexThreads], classes[kClasses];
     __shared__ int carry;
     if (threadIdx.x == 0) carry = 0;
+    if (threadIdx.x < kClasses) classes[threadIdx.x] = 0;
     __syncthreads();
     for (uint32_t s0 = 0; s0 < a.sequences; s0 += kIndexThreads) {
         const uint32_t s = s0 + threadIdx.x;
@@ -54,6 +64,7 @@ __global__ void __launch_bounds__(kIndexThreads) delta_index_kernel(const Args a
         const int last = min(carry + sums[threadIdx.x], (int)a.chunks);
         if (s < a.sequences) {
             a.first[s] = first;
+            atomicAdd(&classes[class_of(mine)], 1);
             for (int c = first; c < last; ++c) {
                 const int t = begin + (c - first) * kChunk;
                 reinterpret_cast<int4*>(a.table)[c] = make_int4(t, min(kChunk, end - t), (int)s, 0);
@@ -70,6 +81,18 @@ __global__ void __launch_bounds__(kIndexThreads) delta_index_kernel(const Args a
         a.first[a.sequences + 1] = end;             // tokens from here on belong to no sequence
         bounds_at(a, 0, begin, end);
         a.first[a.sequences + 2] = begin;           // nor do those before
+        int before = 0;                             // the sequences of higher classes
+        for (int i = kClasses - 1; i >= 0; --i) {
+            const int count = classes[i];
+            classes[i] = before;
+            before += count;
+        }
+    }
+    __syncthreads();
+    for (uint32_t s = threadIdx.x; s < a.sequences; s += kIndexThreads) {
+        int begin, end;
+        bounds_at(a, s, begin, end);
+        a.order[atomicAdd(&classes[class_of((end - begin + kChunk - 1) / kChunk)], 1)] = (int)s;
     }
 }
 
@@ -275,7 +298,7 @@ __global__ void __launch_bounds__(kStateThreads, sizeof(T) == 2 ? 2 : 1) delta_s
     Sh& sh = *reinterpret_cast<Sh*>(raw);
     constexpr int LD = DKP + 8, NT = DKP / 8 / KS, kOwn = 8 / KS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t hv = blockIdx.y, seq = blockIdx.z, h = hv / (p.value_heads / p.heads);
+    const uint32_t hv = blockIdx.y, seq = p.sequences ? p.order[blockIdx.z] : blockIdx.z, h = hv / (p.value_heads / p.heads);
     const int dv_block = blockIdx.x * 16 * Sh::kGroups;
     uint32_t c0, c1;
     if (p.sequences) {
