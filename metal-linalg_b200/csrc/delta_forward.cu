@@ -518,6 +518,10 @@ struct OutShared {
     };
     alignas(16) float2 p[kTriTiles * 32];
     alignas(16) Gates  gates;
+    // S, where two blocks a multiprocessor still have room for it; 64-bit reads of a fragment meet no bank twice
+    static constexpr bool kStaged = sizeof(T) == 2;
+    static constexpr int  kLdS = kOutCols + 4;
+    alignas(16) float  s[kStaged ? DKP * kLdS : 4];
 };
 
 template <typename T, int DKP>
@@ -527,7 +531,7 @@ __global__ void __launch_bounds__(kOutThreads, 2) delta_output_kernel(const Args
     using Sh = OutShared<T, DKP>;
     using Sp = typename Split<T>::type;
     Sh& sh = *reinterpret_cast<Sh*>(raw);
-    constexpr int LD = DKP + 8, kHeld = DKP / 32, LDO = kOutCols + 8;
+    constexpr int LD = DKP + 8, kHeld = Sh::kStaged ? 4 : DKP / 32, LDO = kOutCols + 8;
     const uint32_t c = blockIdx.x, hv = blockIdx.y, h = hv / (p.value_heads / p.heads);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     T* o = static_cast<T*>(p.o);
@@ -567,10 +571,20 @@ __global__ void __launch_bounds__(kOutThreads, 2) delta_output_kernel(const Args
         }
     };
     const float *s = p.states + at * p.dkp * p.dvp, *d = p.d + at * kChunk * p.dvp;
-    if (16 * warp < (int)p.dvp)
+    // staged: all of the warp's own columns of S to shared memory and of D to registers, else half of S's to registers
+    float* mine = sh.s + 16 * warp;
+    const auto ahead = [&](int dv0) {
+        if constexpr (Sh::kStaged) {
+            const int r = lane >> 2, q = (lane & 3) * 4;
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) fetch(s + 16 * warp, 16 * i, held[i]);
-    cp_wait<0>();
+            for (int i = 0; i < DKP; i += 8) cp_async16(mine + (i + r) * Sh::kLdS + q, s + (size_t)(i + r) * p.dvp + dv0 + q, true);
+        }
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) fetch((Sh::kStaged ? d : s) + dv0, 16 * i, held[i]);
+    };
+    if (16 * warp < (int)p.dvp) ahead(16 * warp);
+    cp_commit();
+    cp_wait<1>();
     __syncthreads();
     // P's tiles of 16 x 8 on and below the diagonal, two neighbours at a time: (0, 0), (1, 0), (1, 1), (2, 0) ...
     for (int pair = warp; pair < 10; pair += kOutThreads / 32) {
@@ -597,20 +611,36 @@ __global__ void __launch_bounds__(kOutThreads, 2) delta_output_kernel(const Args
     for (int pass = 0; pass < (int)p.dvp; pass += kOutCols) {
         const int dv0 = pass + 16 * warp;
         if (dv0 < (int)p.dvp) {
-            const float *sv = s + dv0, *dv = d + dv0;
-            if (pass)
-#pragma unroll
-                for (int i = 0; i < kHeld; ++i) fetch(sv, 16 * i, held[i]);
+            [[maybe_unused]] const float *sv = s + dv0, *dv = d + dv0;
+            if (pass) {
+                ahead(dv0);             // (every lane is past the barrier behind its last reads)
+                cp_commit();
+            }
             float acc[8][4] = {};
+            if constexpr (Sh::kStaged) {
+                cp_wait<0>();
+                __syncwarp();
 #pragma unroll
-            for (int kk = 0; kk < 2 * kHeld; ++kk) {
-                float x[4], y[4];
-                tiles(held[kk % kHeld], x, y);
-                if (kk < kHeld) fetch(sv, 16 * (kHeld + kk), held[kk]);
-                else            fetch(dv, 16 * (kk - kHeld), held[kk - kHeld]);
-                Sp a;
-                a.set(x, y);
-                mma_tile<T, 8, false>(acc, a, sh.q, LD, 0, 16 * kk);
+                for (int kk = 0; kk < DKP / 16; ++kk) {
+                    const float* at = mine + (16 * kk + 2 * t) * Sh::kLdS + 2 * g;
+                    const float2 f[4] = {pair_at(at), pair_at(at + Sh::kLdS), pair_at(at + 8 * Sh::kLdS), pair_at(at + 9 * Sh::kLdS)};
+                    float x[4], y[4];
+                    tiles(f, x, y);
+                    Sp a;
+                    a.set(x, y);
+                    mma_tile<T, 8, false>(acc, a, sh.q, LD, 0, 16 * kk);
+                }
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < 2 * kHeld; ++kk) {
+                    float x[4], y[4];
+                    tiles(held[kk % kHeld], x, y);
+                    if (kk < kHeld) fetch(sv, 16 * (kHeld + kk), held[kk]);
+                    else            fetch(dv, 16 * (kk - kHeld), held[kk - kHeld]);
+                    Sp a;
+                    a.set(x, y);
+                    mma_tile<T, 8, false>(acc, a, sh.q, LD, 0, 16 * kk);
+                }
             }
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
