@@ -28,8 +28,9 @@ namespace {
 // ---------------------------------------------------------------------------
 //
 // A block takes a chunk and a value head, a warp 16 tokens' rows of P^T, whose accumulators stay as the A operand of the second
-// product; dO in slices of 64 value columns. Bound by memory's latency (one stage, three or more blocks a
-// multiprocessor hide it): 64 chunks of 16 heads of 128 x 128 36 us, 128 of them 60.
+// product; dO in slices of 64 value columns, two of them asked for with Q and K. Bound by memory's latency, four blocks a
+// multiprocessor hide some of it: 64 chunks of 16 heads of 128 x 128 26 us (36 with a slice fetched when its turn came),
+// 128 of them 44.
 
 constexpr int kDoThreads = 128;
 
@@ -37,12 +38,12 @@ template <typename T, int DKP>
 struct DoShared {
     alignas(16) T     q[kChunk * (DKP + 8)];
     alignas(16) T     k[kChunk * (DKP + 8)];
-    alignas(16) T     d_o[kChunk * (64 + 8)];
+    alignas(16) T     d_o[2][kChunk * (64 + 8)];
     alignas(16) Gates gates;
 };
 
 template <typename T, int DKP>
-__global__ void __launch_bounds__(kDoThreads) delta_do_kernel(const Args p) {
+__global__ void __launch_bounds__(kDoThreads, sizeof(T) == 2 ? 4 : 2) delta_do_kernel(const Args p) {
     dependency_wait_only();
     extern __shared__ __align__(16) char raw[];
     using Sp = typename Split<T>::type;
@@ -57,7 +58,15 @@ __global__ void __launch_bounds__(kDoThreads) delta_do_kernel(const Args p) {
     load_rows<T, kDoThreads, DKP>(sh.k, LD, p.k, at3(p.k_stride, ch.batch, ch.token, h), p.k_stride[1], ch.rows, (int)p.dk, p.vec, threadIdx.x);
     load_floats<kDoThreads, sizeof(Gates) / 4>(reinterpret_cast<float*>(&sh.gates), reinterpret_cast<const float*>(p.gates + at), threadIdx.x);
     cp_commit();
-    cp_wait<0>();
+    const auto fetch = [&](int dv0, int which) {            // a slice of dO, if there is one; a group in any case
+        if (dv0 < (int)p.dvp)
+            load_rows<T, kDoThreads, 64>(sh.d_o[which], LDO, p.d_o, at3(p.do_stride, ch.batch, ch.token, hv) + dv0, p.do_stride[1], ch.rows,
+                                         (int)p.dv - dv0, p.vec, threadIdx.x);
+        cp_commit();
+    };
+    fetch(0, 0);
+    fetch(64, 1);
+    cp_wait<2>();
     __syncthreads();
     // P^T: warp w the rows (tokens j) 16 w .. 16 w + 15; its accumulators are the next product's A operand
     float pt[8][4] = {};
@@ -71,11 +80,8 @@ __global__ void __launch_bounds__(kDoThreads) delta_do_kernel(const Args p) {
             pt[n][i] = r >= j ? p.scale * pt[n][i] * decay_of(sh.gates, r, j) : 0.0f;
         }
     for (int dv0 = 0; dv0 < (int)p.dvp; dv0 += 64) {
-        __syncthreads();
-        load_rows<T, kDoThreads, 64>(sh.d_o, LDO, p.d_o, at3(p.do_stride, ch.batch, ch.token, hv) + dv0, p.do_stride[1], ch.rows,
-                                     (int)p.dv - dv0, p.vec, threadIdx.x);
-        cp_commit();
-        cp_wait<0>();
+        const int which = (dv0 >> 6) & 1;
+        cp_wait<1>();
         __syncthreads();
         float acc[8][4] = {};
 #pragma unroll
@@ -83,7 +89,7 @@ __global__ void __launch_bounds__(kDoThreads) delta_do_kernel(const Args p) {
             if (kk < warp) continue;                        // tokens before these: zero
             Sp a;
             a.set(pt[2 * kk], pt[2 * kk + 1]);
-            mma_tile<T, 8, true>(acc, a, sh.d_o, LDO, 0, 16 * kk);
+            mma_tile<T, 8, true>(acc, a, sh.d_o[which], LDO, 0, 16 * kk);
         }
         float* out = p.dr + at * kChunk * p.dvp;
 #pragma unroll
@@ -94,6 +100,8 @@ __global__ void __launch_bounds__(kDoThreads) delta_do_kernel(const Args p) {
                 *reinterpret_cast<float2*>(out + (size_t)(16 * warp + 8 + g) * p.dvp + column) = make_float2(acc[n][2], acc[n][3]);
             }
         }
+        if (dv0 + 128 < (int)p.dvp) __syncthreads();        // the buffer is free
+        fetch(dv0 + 128, which);
     }
 }
 

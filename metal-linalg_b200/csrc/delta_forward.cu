@@ -503,9 +503,10 @@ __global__ void __launch_bounds__(kStateThreads, sizeof(T) == 2 ? 2 : 1) delta_s
 //
 // A block takes a chunk and a value head; a warp 16 value columns of all 64 tokens: O^T = S^T (e^G Q)^T + D^T P^T, with S
 // and D read from memory as A operands (each value once, split once), Q from shared memory, and P (20 tiles of 16 x 8 over
-// the warps) kept there as the B fragments that its accumulators are. What bounds it is memory's latency: half of a warp's
-// S is on its way while P is made, each further part while the one before it is multiplied. 64 chunks of 16 heads of
-// 128 x 128: 70 us (the tensor core busy 30 % of it, S, D, Q, K and O at 1.9 TB/s); 128 chunks 127.
+// the warps) kept there as the B fragments that its accumulators are. What bounds it is memory's latency and then the tensor
+// core: with 16-bit inputs all of S is on its way to shared memory and all of D to registers while P is made, two blocks a
+// multiprocessor (float32: half of S in registers, each further part fetched while the one before it is multiplied). 64
+// chunks of 16 heads of 128 x 128: 59 us (S, D, Q, K and O at 2.3 TB/s; 70 with S by registers); 128 chunks 109.
 constexpr int kOutThreads = 256;
 constexpr int kOutCols = 16 * (kOutThreads / 32);       // value columns at a time
 
