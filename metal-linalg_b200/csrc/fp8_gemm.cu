@@ -17,8 +17,8 @@
 // What bounds a large product is the hand-over of accumulators: a block of 128 x 256 x 128 takes the tensor core 512 clocks, and
 // the eight epilogue warps 1250 to 1400 to wait for it, read it, scale it, add it and hand it back, two accumulators
 // taking turns: 8192 x 8192 x 4096 in 304 us, 1.81 PFLOP/s (347 us when it runs for seconds and the clocks fall). With a scale
-// for every row of both operands a second multiplication and a load of scales for four sums make that 2300 clocks: 546 us
-// (tiles of 128 columns: 602). 4096 x 4096 x 2048 55 us; 1024 x 1024 x 4096 14; 16 rows x 4096 x 8192 11.4 us (the
+// for every row of both operands a second multiplication and a load of scales for four sums make that 2200 clocks: 522 us
+// (tiles of 128 columns 10 % more). 4096 x 4096 x 2048 55 us; 1024 x 1024 x 4096 14; 16 rows x 4096 x 8192 11.4 us (the
 // weight's 33.6 MB at 3.0 TB/s: the ring's start and the cluster's exchange are half of it).
 //
 // Every wait on an mbarrier is bounded. One that runs out makes the block's outputs NaN, sets the status word, waits
@@ -285,12 +285,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t at = tmem + acc * BN + part * S::kCols + ((32u * quarter) << 16);
                 // two loads in flight; the next two go out as their registers are used up
-                constexpr int kPiece = S::kCols >= 32 ? 32 : 16, kFlight = S::kCols > kPiece ? 2 : 1;
+                // (by column in pieces of 16: the scales of two of them take the registers)
+                constexpr int kPiece = S::kCols >= 32 && !kByColumn ? 32 : 16, kFlight = S::kCols > kPiece ? 2 : 1;
                 uint32_t v[kFlight][kPiece];
 #pragma unroll
                 for (int f = 0; f < kFlight; ++f) TmemLoad<kPiece>::load(v[f], at + f * kPiece);
 #pragma unroll
                 for (int j = 0; j < S::kCols; j += kFlight * kPiece) {
+                    ulonglong2 c[kByColumn ? kFlight * kPiece / 4 : 1];     // on their way while the accumulator is
+                    if constexpr (kByColumn)
+#pragma unroll
+                        for (int e = 0; e < kFlight * kPiece / 4; ++e) c[e] = *reinterpret_cast<const ulonglong2*>(by_column + j + 4 * e);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (j + kFlight * kPiece >= S::kCols) {     // everything is read: the accumulator is free
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -304,9 +309,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
                             const int to = j + f * kPiece + e;
                             Pair by[2] = {scale2, scale2};
                             if constexpr (kByColumn) {
-                                const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(by_column + to);
-                                by[0] = times(scale2, c.x);
-                                by[1] = times(scale2, c.y);
+                                by[0] = times(scale2, c[(f * kPiece + e) / 4].x);
+                                by[1] = times(scale2, c[(f * kPiece + e) / 4].y);
                             }
                             add_scaled(sum[to / 2], v[f][e], v[f][e + 1], by[0]);
                             add_scaled(sum[to / 2 + 1], v[f][e + 2], v[f][e + 3], by[1]);
