@@ -772,3 +772,20 @@ def test_a_step_tells_the_graph_that_saved_its_pool():
         mlt.gated_delta_step(q, k, v, g, beta, pool)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         o.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n, length", [(300, 70), (7, 130), (1, 200)])
+def test_ragged_rows_of_one_length_are_a_batch(n, length):
+    """Whatever order the sequences start in: the batch's results, bit for bit, and its gradients (the backward pass may share
+    its chains between other numbers of warps)."""
+    q, k, v, g, beta, s0 = inputs(n, length, 1, 2, 32, 16, torch.bfloat16, seed=n)
+    grads_of = lambda o, s, leaves: torch.autograd.grad((o, s), leaves, (torch.ones_like(o), torch.ones_like(s)))  # noqa: E731
+    batch = [x.clone().requires_grad_() for x in (q, k, v, g, beta, s0)]
+    rows = [x.reshape(1, n * length, *x.shape[2:]).clone().requires_grad_() for x in (q, k, v, g, beta)] + [s0.clone().requires_grad_()]
+    cu = torch.arange(n + 1, device="cuda", dtype=torch.int32) * length
+    o, s = mlt.gated_delta_rule(*batch[:5], initial_state=batch[5])
+    ro, rs = mlt.gated_delta_rule(*rows[:5], initial_state=rows[5], cu_seqlens=cu)
+    assert torch.equal(o.reshape(ro.shape), ro) and torch.equal(s, rs)
+    for x, y in zip(grads_of(o, s, batch), grads_of(ro, rs, rows)):
+        near(y.reshape(x.shape), x, tolerance(torch.bfloat16, grad=True))
