@@ -29,7 +29,9 @@ __device__ __forceinline__ long long slot_of(const StepArgs& a, uint32_t row) {
     return a.slots64 ? static_cast<const long long*>(a.slots)[row] : (long long)static_cast<const int*>(a.slots)[row];
 }
 
-template <typename T>
+// kVec: a state's rows can be read in pieces of 16 bytes; a thread's four columns are neighbours. Else they lie eight apart, so
+// that neighbouring lanes read neighbouring values (128 rows of 32 heads of 128 x 127 112 us, 134 with neighbours).
+template <typename T, bool kVec>
 __global__ void __launch_bounds__(kStepThreads, 7) delta_step_kernel(const StepArgs a) {
     dependency_wait_only();
     __shared__ float qs[128], ks[128];
@@ -38,7 +40,8 @@ __global__ void __launch_bounds__(kStepThreads, 7) delta_step_kernel(const StepA
     const uint32_t hv = blockIdx.y, row = blockIdx.z, h = hv / (a.value_heads / a.heads);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int quad = threadIdx.x & 7, group = threadIdx.x >> 3;
-    const int col = blockIdx.x * kStepCols + 4 * quad;
+    constexpr int apart = kVec ? 1 : 8;
+    const int col = blockIdx.x * kStepCols + (kVec ? 4 * quad : quad);
     T* o = static_cast<T*>(a.o);
     const long long slot = slot_of(a, row);
     // a token's inputs need no slot: the first one's are on their way with it
@@ -52,7 +55,7 @@ __global__ void __launch_bounds__(kStepThreads, 7) delta_step_kernel(const StepA
         beta = a.beta[at3(a.beta_stride, r, t, hv)];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            v[i] = col + i < (int)a.dv ? to_f(static_cast<const T*>(a.v)[at3(a.v_stride, r, t, hv) + col + i]) : 0.0f;
+            v[i] = col + apart * i < (int)a.dv ? to_f(static_cast<const T*>(a.v)[at3(a.v_stride, r, t, hv) + col + apart * i]) : 0.0f;
     };
     fetch(row, 0);
     int found = 0;
@@ -65,7 +68,8 @@ __global__ void __launch_bounds__(kStepThreads, 7) delta_step_kernel(const StepA
             if (group == 0)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (col + i < (int)a.dv) o[(((size_t)row * a.tokens + t) * a.value_heads + hv) * a.dv + col + i] = from_f<T>(0.0f);
+                    if (col + apart * i < (int)a.dv)
+                        o[(((size_t)row * a.tokens + t) * a.value_heads + hv) * a.dv + col + apart * i] = from_f<T>(0.0f);
         return;
     }
     // the state: every load issued before the first value is needed
@@ -75,12 +79,12 @@ __global__ void __launch_bounds__(kStepThreads, 7) delta_step_kernel(const StepA
     for (int j = 0; j < kMaxRows; ++j) {
         const int r = group + kRowGroups * j;
         const float* src = pool + (size_t)r * a.dv + col;
-        if (a.vec && r < (int)a.dk && col < (int)a.dv) {
+        if (kVec && r < (int)a.dk && col < (int)a.dv) {
             const float4 f = *reinterpret_cast<const float4*>(src);
             s[j][0] = f.x; s[j][1] = f.y; s[j][2] = f.z; s[j][3] = f.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[j][i] = r < (int)a.dk && col + i < (int)a.dv ? src[i] : 0.0f;
+            for (int i = 0; i < 4; ++i) s[j][i] = r < (int)a.dk && col + apart * i < (int)a.dv ? src[apart * i] : 0.0f;
         }
     }
     // rows of one slot: the first of them runs them all, in order
@@ -147,8 +151,8 @@ __global__ void __launch_bounds__(kStepThreads, 7) delta_step_kernel(const StepA
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 d[i] = beta * fmaf(-decay, sk[i], v[i]);
-                if (group == 0 && col + i < (int)a.dv)
-                    o[(((size_t)r * a.tokens + t) * a.value_heads + hv) * a.dv + col + i] =
+                if (group == 0 && col + apart * i < (int)a.dv)
+                    o[(((size_t)r * a.tokens + t) * a.value_heads + hv) * a.dv + col + apart * i] =
                         from_f<T>(a.scale * fmaf(decay, sq[i], kq * d[i]));
             }
 #pragma unroll
@@ -163,12 +167,12 @@ __global__ void __launch_bounds__(kStepThreads, 7) delta_step_kernel(const StepA
     for (int j = 0; j < kMaxRows; ++j) {
         const int r = group + kRowGroups * j;
         float* dst = pool + (size_t)r * a.dv + col;
-        if (a.vec && r < (int)a.dk && col < (int)a.dv) {
+        if (kVec && r < (int)a.dk && col < (int)a.dv) {
             *reinterpret_cast<float4*>(dst) = make_float4(s[j][0], s[j][1], s[j][2], s[j][3]);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (r < (int)a.dk && col + i < (int)a.dv) dst[i] = s[j][i];
+                if (r < (int)a.dk && col + apart * i < (int)a.dv) dst[apart * i] = s[j][i];
         }
     }
 }
@@ -177,10 +181,11 @@ __global__ void __launch_bounds__(kStepThreads, 7) delta_step_kernel(const StepA
 
 void launch_step(const StepArgs& a, cudaStream_t stream) {
     const dim3 grid((a.dv + kStepCols - 1) / kStepCols, a.value_heads, a.batch);
+    const auto launch = [&](auto plain, auto vec) { launch_dependent(a.vec ? vec : plain, grid, kStepThreads, 0, stream, a); };
     switch (a.dtype) {
-        case METAL_LINALG_BFLOAT16: launch_dependent(delta_step_kernel<bf16>, grid, kStepThreads, 0, stream, a); break;
-        case METAL_LINALG_FLOAT16: launch_dependent(delta_step_kernel<__half>, grid, kStepThreads, 0, stream, a); break;
-        default: launch_dependent(delta_step_kernel<float>, grid, kStepThreads, 0, stream, a); break;
+        case METAL_LINALG_BFLOAT16: launch(delta_step_kernel<bf16, false>, delta_step_kernel<bf16, true>); break;
+        case METAL_LINALG_FLOAT16: launch(delta_step_kernel<__half, false>, delta_step_kernel<__half, true>); break;
+        default: launch(delta_step_kernel<float, false>, delta_step_kernel<float, true>); break;
     }
 }
 
