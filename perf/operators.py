@@ -23,17 +23,7 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 FP8_MAX = 448.0                       # of e4m3
 
 
-_loaded = None
-
-
 def _package():
-    global _loaded
-    if _loaded is None:                 # once, as a user's program imports it
-        _loaded = _load()
-    return _loaded
-
-
-def _load():
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "metal-linalg_b200")
     if path not in sys.path:
         sys.path.insert(0, path)
