@@ -92,19 +92,22 @@ __device__ __forceinline__ void divided(const float (&v)[N], float scale, uint32
                          (bytes_of<kE5m2>(__fdiv_rn(v[i + 2], scale), __fdiv_rn(v[i + 3], scale)) << 16);
         return;
     }
-    const float r = 1.0f / scale;
-    const Pair r2 = pair_of(r, r), minus = pair_of(-scale, -scale);
+    // the quotients' negatives, whose sign of zero is right: with x = -0 the remainder is +0, and added to q = -0 it would leave +0,
+    // while (+0)(-r) + (+0) is the +0 that stands for -(-0). (0.25 instructions a value for the signs, back in the packed bytes;
+    // no NaN comes here.)
+    const float r = -1.0f / scale;
+    const Pair r2 = pair_of(r, r), plus = pair_of(scale, scale);
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
         uint32_t half[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const Pair x = pair_of(v[i + 2 * j], v[i + 2 * j + 1]), q = mul2(x, r2), y = fma2(fma2(q, minus, x), r2, q);
+            const Pair x = pair_of(v[i + 2 * j], v[i + 2 * j + 1]), q = mul2(x, r2), y = fma2(fma2(q, plus, x), r2, q);
             float low, high;
             asm("mov.b64 {%0, %1}, %2;" : "=f"(low), "=f"(high) : "l"(y));
             half[j] = bytes_of<kE5m2>(low, high);
         }
-        out[i / 4] = half[0] | (half[1] << 16);
+        out[i / 4] = (half[0] | (half[1] << 16)) ^ 0x80808080u;
     }
 }
 

@@ -179,6 +179,26 @@ def test_quantize_strides():
             assert torch.equal(got[0].float(), want[0].float()) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [E4M3, E5M2])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("block", [1, 128])
+def test_quantize_bytes(block, transpose, dtype, kind):
+    """Byte for byte: zeros of both signs, and values of both signs that round to zero, among ordinary ones."""
+    torch.manual_seed(8)
+    x = torch.randn(260, 300, device="cuda")
+    x[::3, ::5] = 0.0
+    x[1::3, ::4] = -0.0
+    x[2::3, 1::7] = -1e-9
+    x[::7, 2::9] = 1e-9
+    x = x.to(dtype)
+    values, _ = mlt.quantize_fp8(x, block=(block, 128), transpose=transpose, dtype=kind)
+    want = wanted(x.mT if transpose else x, block, kind)[0].float().to(kind)
+    assert (want.view(torch.uint8) == 0x80).sum() > 3000
+    assert torch.equal(values.contiguous().view(torch.uint8).cpu(), want.view(torch.uint8))
+
+
 # ---------------------------------------------------------------------------
 # The product
 # ---------------------------------------------------------------------------
