@@ -43,6 +43,8 @@ def _padded(x, lead, rows, cols, dtype):
 
 def _quantize(x, block_rows, transpose, dtype):
     *lead, m, n = x.shape
+    if len(lead) > 1 and x.numel():
+        x = x.reshape(-1, m, n)                         # copies only what no strides can describe
     *outer, rows, cols = x.stride()
     if transpose:
         m, n, rows, cols = n, m, cols, rows
@@ -55,17 +57,12 @@ def _quantize(x, block_rows, transpose, dtype):
         cols = 1
     elif m == 1 and cols != 1:
         rows = 1
-    batch, across = 1, 0
-    if len(lead) == 1:
-        (batch,), (across,) = lead, outer
-    elif lead or (rows != 1 and cols != 1):
-        x = x.reshape(-1, *x.shape[-2:])                # copies only what no strides can describe
-        batch, across = x.shape[0], x.stride(0)
-        rows, cols = (x.stride(2), x.stride(1)) if transpose else (x.stride(1), x.stride(2))
-    if rows != 1 and cols != 1 and n > 1:
+    elif rows != 1 and cols != 1:
         x = x.contiguous()
-        across = x.stride(0) if x.dim() == 3 else 0
-        rows, cols = (1, m) if transpose else (n, 1)
+        *outer, rows, cols = x.stride()
+        if transpose:
+            rows, cols = cols, rows
+    batch, across = (x.shape[0], outer[0]) if outer else (1, 0)
     device = _lib.use_stream_of(x)
     _lib.check(_lib.lib.metal_linalg_quantize_fp8(x.data_ptr(), _DTYPES[x.dtype], batch, m, n, across, rows, cols, block_rows,
                                                   _KINDS[dtype], values.data_ptr(), -(-n // 16) * 16, scales.data_ptr(), device))

@@ -118,6 +118,44 @@ def test_c_entries_refuse_without_a_gpu():
         assert matmul() == _lib.RUNTIME_ERROR and quantize() == _lib.RUNTIME_ERROR
 
 
+def layouts(device):
+    """Matrices with a row or a column of one whose strides are both other than 1, in two to five dimensions."""
+    f = lambda *s: torch.arange(math.prod(s), dtype=torch.float32, device=device).reshape(s)  # noqa: E731
+    return [f(5, 6)[:, ::2][:, :1], f(5, 6)[::2, ::3][:1], f(4, 5, 6)[..., ::2][..., :1], f(4, 5, 6)[:, :1, ::2], f(2, 3, 5, 4, 2)[..., :1, 0],
+            f(2, 3, 5, 7)[..., ::8], f(2, 3, 1, 8)[..., ::2], f(2, 3, 5, 8)[:, :, :1, ::2], f(2, 3, 2, 5, 6)[..., ::2][..., :1],
+            f(3, 2, 4, 6).transpose(0, 1)[..., ::2][..., :1], f(3, 2, 4, 6).transpose(0, 1)[..., :1, ::3], f(2, 3, 4, 6)[..., ::2],
+            f(2, 3, 4, 6)[..., ::2, ::3], f(1, 1).expand(4, 7), f(2, 1, 1, 1).expand(2, 3, 4, 7), f(2, 1, 4, 1).expand(2, 3, 4, 7),
+            f(2, 3, 4, 1)[:, :, ::2], f(1, 2, 1, 1)]
+
+
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("which", range(18))
+def test_quantize_hands_on_strides_that_read_the_matrix(which, transpose, monkeypatch):
+    """What the C entry is given, read back with numpy: one stride is 1, and the values are x's."""
+    import types
+
+    import numpy as np
+    from metal_linalg_torch import _fp8
+    x = layouts("cpu")[which]
+    seen = []
+
+    def entry(at, dtype, batch, rows, cols, *rest):
+        import ctypes
+        across, down, along = rest[:3]
+        assert down == 1 or along == 1
+        reach = (batch - 1) * across + (rows - 1) * down + (cols - 1) * along + 1
+        flat = np.ctypeslib.as_array(ctypes.cast(at, ctypes.POINTER(ctypes.c_float)), (reach,))
+        seen.append(np.lib.stride_tricks.as_strided(flat, (batch, rows, cols), tuple(4 * s for s in (across, down, along))).copy())
+        return _lib.OK
+
+    monkeypatch.setattr(_lib, "lib", types.SimpleNamespace(metal_linalg_quantize_fp8=entry))
+    monkeypatch.setattr(_lib, "use_stream_of", lambda x: 0)
+    values, scales = _fp8._quantize(x, 1, transpose, E4M3)
+    want = x.mT if transpose else x
+    assert values.shape == want.shape and scales.shape == (*want.shape[:-1], -(-want.shape[-1] // 128))
+    assert np.array_equal(seen[0], want.reshape(-1, *want.shape[-2:]).numpy())
+
+
 # ---------------------------------------------------------------------------
 # The quantiser
 # ---------------------------------------------------------------------------
@@ -177,6 +215,17 @@ def test_quantize_strides():
             assert torch.equal(got[0].float(), want[0].float()) and torch.equal(got[1], want[1])
             got, want = mlt.quantize_fp8(x, block=(block, 128), transpose=True), mlt.quantize_fp8(x.mT.contiguous(), block=(block, 128))
             assert torch.equal(got[0].float(), want[0].float()) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("block", [1, 128])
+def test_quantize_rows_and_columns_of_one(block, transpose):
+    for x in layouts("cuda"):
+        values, scales = mlt.quantize_fp8(x, block=(block, 128), transpose=transpose)
+        v, s, _ = wanted(x.mT if transpose else x, block, E4M3)
+        same(scales, s, "scales")
+        same(values.float(), v, "values")
 
 
 @pytest.mark.gpu
