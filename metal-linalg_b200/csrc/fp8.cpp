@@ -14,6 +14,8 @@ namespace {
 
 [[noreturn]] void refuse(const char* who, const std::string& what) { throw std::invalid_argument(std::string(who) + " " + what); }
 
+constexpr uint64_t kMostMatrices = 65535;       // of a quantiser's launch: its grid's second dimension
+
 bool is_fp8(uint32_t kind) { return kind == METAL_LINALG_FLOAT8_E4M3 || kind == METAL_LINALG_FLOAT8_E5M2; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -63,7 +65,6 @@ void quantize_fp8(const void* x, uint32_t dtype, uint32_t batch, uint32_t rows, 
     if (cpu_only()) throw std::runtime_error(std::string(who) + " this thread is set CPU-only, and this build has no CPU path");
     if (batch == 0 || rows == 0 || cols == 0) return;
     if (col_stride != 1 && row_stride != 1) refuse(who, "one of row_stride and col_stride must be 1");
-    if (batch > 65535) refuse(who, "batch must be at most 65535");
     if (rows >= 1u << 30 || cols >= 1u << 30 || (uint64_t)rows * ((cols + 127) / 128) >= 1ull << 31)
         refuse(who, "rows and cols must be below 2^30, and the matrix below 2^38 elements");
     if (!aligned16(values) || values_stride % 16 || values_stride < cols)
@@ -75,16 +76,21 @@ void quantize_fp8(const void* x, uint32_t dtype, uint32_t batch, uint32_t rows, 
     const int64_t size = dtype == METAL_LINALG_FLOAT32 ? 4 : 2;
     const int64_t across = col_stride == 1 ? row_stride : col_stride;
     mlb::fp8::QuantizeArgs a{};
-    a.x = x; a.rows = rows; a.cols = cols; a.batch = batch;
+    a.rows = rows; a.cols = cols;
     a.batch_stride = batch_stride; a.row_stride = row_stride; a.col_stride = col_stride;
     a.block_rows = block_rows;
     a.vec = aligned16(x) && across * size % 16 == 0 && (batch == 1 || batch_stride * size % 16 == 0);
-    a.values = static_cast<uint8_t*>(values);
     a.values_stride = values_stride;
     a.values_batch = values_stride * rows;
-    a.scales = scales;
     mlb::DeviceGuard guard(where.device);
-    mlb::fp8::launch_quantize(a, dtype, kind == METAL_LINALG_FLOAT8_E5M2, mlb::thread_stream());
+    const uint64_t scales_batch = (uint64_t)((rows + block_rows - 1) / block_rows) * ((cols + 127) / 128);
+    for (uint64_t first = 0; first < batch; first += kMostMatrices) {       // a launch's
+        a.batch = (uint32_t)(batch - first < kMostMatrices ? batch - first : kMostMatrices);
+        a.x = static_cast<const char*>(x) + (int64_t)first * batch_stride * size;
+        a.values = static_cast<uint8_t*>(values) + first * a.values_batch;
+        a.scales = scales + first * scales_batch;
+        mlb::fp8::launch_quantize(a, dtype, kind == METAL_LINALG_FLOAT8_E5M2, mlb::thread_stream());
+    }
 }
 
 void matmul_fp8(const metal_linalg_fp8_operand& a, const metal_linalg_fp8_operand& b, uint32_t batch, uint32_t m, uint32_t n,

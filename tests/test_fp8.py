@@ -229,6 +229,25 @@ def test_quantize_rows_and_columns_of_one(block, transpose):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("block", [1, 128])
+def test_quantize_more_matrices_than_a_grid_has_rows(block, transpose):
+    """Each as if it were alone; the last ones, behind the 65535th, and those on either side of it."""
+    torch.manual_seed(block)
+    x = torch.randn(70000, 3, 20, device="cuda").bfloat16()
+    values, scales = mlt.quantize_fp8(x, block=(block, 128), transpose=transpose)
+    for part in (slice(0, 3), slice(65533, 65538), slice(69990, 70000)):
+        v, s = mlt.quantize_fp8(x[part], block=(block, 128), transpose=transpose)
+        assert torch.equal(values[part].float(), v.float()) and torch.equal(scales[part], s)
+    if not transpose:
+        v, s = mlt.quantize_fp8(x.reshape(-1, 20))          # a scale a row: the matrices' rows behind one another
+        assert block != 1 or (torch.equal(values.reshape(-1, 20).float(), v.float()) and torch.equal(scales.reshape(-1, 1), s))
+    a = mlt.matmul_fp8(values, scales, values[0], scales[0], out_dtype=torch.float32)
+    one = mlt.matmul_fp8(values[-1:], scales[-1:], values[0], scales[0], out_dtype=torch.float32)
+    assert torch.equal(a[-1:], one)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", [E4M3, E5M2])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("transpose", [False, True])
