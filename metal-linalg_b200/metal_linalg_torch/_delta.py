@@ -197,7 +197,7 @@ def _grads(ctx, d_o, d_last, run=None):
         return (None,) * 8
     if d_o is None:
         d_o = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
-    if run is None or not direct(d_o, d_last, q, k, v, g, beta, initial, cu):
+    if run is None or not direct("gated_delta_rule", d_o, d_last, q, k, v, g, beta, initial, cu):
         run = torch.ops.metal_linalg.gated_delta_rule_backward
     dq, dk, dv, dg, dbeta, d_initial = run(d_o, d_last, q, k, v, g, beta, ctx.scale, initial, cu)
     return dq, dk, dv, dg, dbeta, None, None if initial is None else d_initial, None
@@ -248,7 +248,7 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, cu_seq
             _fail(name, f"initial_state is on {initial_state.device}, q on {q.device}")
     scale = _scale(scale, dk)
     g, beta = _float(g), _float(beta)
-    if not direct(q, k, v, g, beta, initial_state, cu_seqlens):
+    if not direct(name, q, k, v, g, beta, initial_state, cu_seqlens):
         return torch.ops.metal_linalg.gated_delta_rule(q, k, v, g, beta, scale, initial_state, cu_seqlens)
     initial = None if initial_state is None else initial_state.contiguous()
     tensors = (q, k, v, g, beta) if initial is None else (q, k, v, g, beta, initial)
@@ -326,7 +326,7 @@ def gated_delta_step(q, k, v, g, beta, state, *, slots=None, scale=None):
         _fail(name, "not differentiable; use gated_delta_rule for training, or torch.no_grad()", RuntimeError)
     scale = _scale(scale, dk)
     g, beta = _float(g), _float(beta)
-    if not direct(q, k, v, g, beta, state, slots):
+    if not direct(name, q, k, v, g, beta, state, slots):
         return torch.ops.metal_linalg.gated_delta_step(q, k, v, g, beta, state, slots, scale)
     _changed(state)                 # a graph that saved the pool for its backward pass finds it changed
     return _step(q, k, v, g, beta, state, slots, scale)

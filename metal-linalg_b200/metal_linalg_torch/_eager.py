@@ -6,6 +6,7 @@ torch.compile and export, `make_fx` and fake tensors (dispatch modes, pre-dispat
 `torch.func`, tensor subclasses and meta tensors.
 """
 import torch
+import torch.autograd.forward_ad as _forward_ad
 from torch import Tensor
 
 _PLAIN = frozenset((Tensor, torch.nn.Parameter, type(None)))
@@ -17,9 +18,12 @@ _is_included = torch._C._dispatch_tls_is_dispatch_key_included
 _PRE_DISPATCH = torch._C.DispatchKey.PreDispatch
 
 
-def direct(*tensors):
-    """Whether a call may use the addresses of `tensors` (None allowed behind the first)."""
+def direct(name, *tensors):
+    """Whether operator `name` may use the addresses of `tensors` (None allowed behind the first). Refuses forward-mode
+    tangents, which no operator here carries on."""
     if _is_compiling():
         return False
+    if _forward_ad._current_level >= 0 and any(x is not None and _forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise RuntimeError(f"metal_linalg_torch.{name}: forward-mode derivatives are not supported")
     return (not _dispatch_modes() and not _is_tracing() and _transforms() is None and not _is_included(_PRE_DISPATCH)
             and _PLAIN.issuperset(map(type, tensors)) and not tensors[0].is_meta)

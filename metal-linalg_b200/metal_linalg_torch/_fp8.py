@@ -105,7 +105,7 @@ def quantize_fp8(x, *, block=(1, 128), transpose=False, dtype=torch.float8_e4m3f
         _fail(name, f"expected a tensor of shape [..., M, N], got shape {tuple(x.shape)}")
     if torch.is_grad_enabled() and x.requires_grad:
         _fail(name, "not differentiable; use linear_fp8, or detach x", RuntimeError)
-    if not direct(x):
+    if not direct(name, x):
         return torch.ops.metal_linalg.quantize_fp8(x, block[0], bool(transpose), dtype)
     return _quantize(x, block[0], transpose, dtype)
 
@@ -205,7 +205,7 @@ def matmul_fp8(a, a_scale, b, b_scale, *, out_dtype=torch.bfloat16):
         _fail(name, f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}", TypeError)
     if torch.is_grad_enabled() and (a.requires_grad or a_scale.requires_grad or b.requires_grad or b_scale.requires_grad):
         _fail(name, "not differentiable; use linear_fp8, or detach the operands", RuntimeError)
-    if not direct(a, a_scale, b, b_scale):
+    if not direct(name, a, a_scale, b, b_scale):
         return torch.ops.metal_linalg.matmul_fp8(a, a_scale, b, b_scale, a_rows, b_rows, out_dtype)
     return _matmul(a, a_scale, b, b_scale, a_rows, b_rows, out_dtype)
 
@@ -218,7 +218,7 @@ def _product(quantize, matmul, x, y, x_block, y_block, x_turned, y_turned, out_d
 
 def _linear_grads(ctx, dy, quantize=None, matmul=None):
     x, w = ctx.saved_tensors
-    if quantize is None or not direct(dy, x, w):
+    if quantize is None or not direct("linear_fp8", dy, x, w):
         quantize, matmul = torch.ops.metal_linalg.quantize_fp8, torch.ops.metal_linalg.matmul_fp8
     dx = dw = None
     dy = dy.to(x.dtype)
@@ -272,7 +272,7 @@ def linear_fp8(x, w):
     if w.device != x.device:
         _fail(name, f"w is on {w.device}, x on {x.device}")
     flat = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
-    if not direct(x, w):
+    if not direct(name, x, w):
         y = torch.ops.metal_linalg.linear_fp8(flat, w)
     elif torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         y = _Linear.apply(flat, w)

@@ -1,8 +1,9 @@
 """The sequence and 8-bit operators under whatever watches or replaces torch's operators: fake tensors, make_fx, torch.jit.trace,
-torch.func, checkpointing. A traced function holds the operators themselves and gives an eager
+torch.func, forward-mode derivatives, checkpointing. A traced function holds the operators themselves and gives an eager
 call's results, bit for bit."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 
@@ -87,6 +88,23 @@ def test_make_fx_of_fake_tensors(case, pre_dispatch):
     with FakeTensorMode():
         graph = make_fx(f, pre_dispatch=pre_dispatch)(*make("fake"))
     assert ops <= held(graph)
+
+
+def test_forward_mode_is_refused():
+    meta = lambda *s: torch.empty(*s, device="meta")  # noqa: E731
+    args = [meta(1, 5, 1, 8), meta(1, 5, 1, 8), meta(1, 5, 2, 8), meta(1, 5, 2), meta(1, 5, 2), meta(1, 2, 8, 8)]
+    for name, call, i in (("gated_delta_rule", rule, 0), ("gated_delta_rule", rule, 5), ("gated_delta_rule", rule, 3), ("gated_delta_step", step, 2),
+                          ("gated_delta_step", step, 5)):
+        with fw.dual_level():
+            call(*args)
+            with pytest.raises(RuntimeError, match=f"{name}: forward-mode"):
+                call(*(fw.make_dual(x, torch.empty_like(x)) if j == i else x for j, x in enumerate(args)))
+    x, w = meta(4, 16), meta(3, 16)
+    for call, name in ((mlt.linear_fp8, "linear_fp8"), (product, "quantize_fp8")):
+        with fw.dual_level(), pytest.raises(RuntimeError, match=f"{name}: forward-mode"):
+            call(x, fw.make_dual(w, torch.empty_like(w)))
+        with pytest.raises(RuntimeError, match=f"{name}: forward-mode"):
+            torch.func.jvp(lambda y: call(y, w), (x,), (torch.empty_like(x),))
 
 
 # ---------------------------------------------------------------------------
