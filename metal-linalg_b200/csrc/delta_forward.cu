@@ -43,6 +43,9 @@ __global__ void __launch_bounds__(kIndexThreads) delta_index_kernel(const Args a
     dependency_wait();
     __shared__ int sums[kIndexThreads], classes[kClasses];
     __shared__ int carry;
+    // Sequences that overlap (a falling cu_seqlens) can name more chunks than there is room for, or than an int counts: every
+    // sum stops at the room, and what lies behind it has no chunks. Bounds that do not fall never name more.
+    const int room = (int)a.chunks;
     if (threadIdx.x == 0) carry = 0;
     if (threadIdx.x < kClasses) classes[threadIdx.x] = 0;
     __syncthreads();
@@ -51,17 +54,16 @@ __global__ void __launch_bounds__(kIndexThreads) delta_index_kernel(const Args a
         int begin = 0, end = 0;
         if (s < a.sequences) bounds_at(a, s, begin, end);
         const int mine = (end - begin + kChunk - 1) / kChunk;
-        sums[threadIdx.x] = mine;
+        sums[threadIdx.x] = min(mine, room);
         __syncthreads();
         for (int o = 1; o < kIndexThreads; o *= 2) {
             const int v = threadIdx.x >= o ? sums[threadIdx.x - o] : 0;
             __syncthreads();
-            sums[threadIdx.x] += v;
+            sums[threadIdx.x] = min(sums[threadIdx.x] + v, room);
             __syncthreads();
         }
-        // sequences that overlap (a falling cu_seqlens) could name more chunks than there is room for: none behind it
-        const int first = min(carry + sums[threadIdx.x] - mine, (int)a.chunks);
-        const int last = min(carry + sums[threadIdx.x], (int)a.chunks);
+        const int first = min(carry + (threadIdx.x ? sums[threadIdx.x - 1] : 0), room);
+        const int last = min(carry + sums[threadIdx.x], room);
         if (s < a.sequences) {
             a.first[s] = first;
             atomicAdd(&classes[class_of(mine)], 1);
@@ -71,13 +73,13 @@ __global__ void __launch_bounds__(kIndexThreads) delta_index_kernel(const Args a
             }
         }
         __syncthreads();
-        if (threadIdx.x == 0) carry += sums[kIndexThreads - 1];
+        if (threadIdx.x == 0) carry = min(carry + sums[kIndexThreads - 1], room);
         __syncthreads();
     }
     if (threadIdx.x == 0) {
         int begin, end;
         bounds_at(a, a.sequences - 1, begin, end);
-        a.first[a.sequences] = min(carry, (int)a.chunks);
+        a.first[a.sequences] = carry;
         a.first[a.sequences + 1] = end;             // tokens from here on belong to no sequence
         bounds_at(a, 0, begin, end);
         a.first[a.sequences + 2] = begin;           // nor do those before

@@ -789,3 +789,77 @@ def test_ragged_rows_of_one_length_are_a_batch(n, length):
     assert torch.equal(o.reshape(ro.shape), ro) and torch.equal(s, rs)
     for x, y in zip(grads_of(o, s, batch), grads_of(ro, rs, rows)):
         near(y.reshape(x.shape), x, tolerance(torch.bfloat16, grad=True))
+
+
+# ---------------------------------------------------------------------------
+# Bounds that are the caller's mistake: everything that is written lies inside the call's own buffers
+# ---------------------------------------------------------------------------
+
+GUARD, MARK = 8192, 0xA5
+
+
+class Guarded:
+    """Buffers of one allocation, each between two stretches that hold a pattern."""
+
+    def __init__(self, **sizes):
+        self.at, end = {}, GUARD
+        for name, size in sizes.items():
+            self.at[name] = (end, size)
+            end += -(-size // 256) * 256 + GUARD
+        self.memory = torch.full((end,), MARK, dtype=torch.uint8, device="cuda")
+
+    def __getitem__(self, name):
+        return self.memory.data_ptr() + self.at[name][0]
+
+    def untouched(self):
+        outside = torch.ones(self.memory.numel(), dtype=torch.bool, device="cuda")
+        for start, size in self.at.values():
+            outside[start:start + size] = False
+        return bool((self.memory[outside] == MARK).all())
+
+
+def guarded_calls(args, cu, d_o, d_s):
+    """Both directions through the C entries, every output and the workspace between guards."""
+    import struct
+
+    from metal_linalg_torch import _delta
+    q, k, v, g, beta, s0 = args
+    p = _delta._problem(q, k, v, g, beta, 0.5, s0, cu, cu.element_size())
+    size = lambda *xs: [x.numel() * x.element_size() for x in xs]  # noqa: E731
+    need = [_lib.lib.metal_linalg_gated_delta_rule_workspace_bytes(p, back) for back in (0, 1)]
+    _lib.use_stream_of(q)
+    sizes = dict(zip(("o", "s"), size(v, s0)))
+    b = Guarded(**sizes, ws=need[0])
+    _lib.check(_lib.lib.metal_linalg_gated_delta_rule(p, b["o"], b["s"], b["ws"], need[0]))
+    torch.cuda.synchronize()
+    assert b.untouched()
+    b = Guarded(**dict(zip(("dq", "dk", "dv", "dg", "db", "ds"), size(*args))), ws=need[1])
+    _lib.check(_lib.lib.metal_linalg_gated_delta_rule_backward(p, d_o.data_ptr(), struct.pack("=3q", *d_o.stride()[:3]), d_s.data_ptr(),
+                                                               *(b[n] for n in ("dq", "dk", "dv", "dg", "db", "ds")), b["ws"], need[1]))
+    torch.cuda.synchronize()
+    assert b.untouched()
+
+
+BAD = [[0, 300, 0, 300], [50, 40, 30, 20], [-7, 100, 5000, 300], [0, 2 ** 31 - 1, 0, 2 ** 31 - 1], [300, 0, 300, 0], [-5, -4, -3, -2],
+       [2 ** 31 - 1] * 4, [-2 ** 31, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1], [300, 300, 300, 0], [0, 65, 64, 300]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("bounds", BAD, ids=str)
+def test_bad_bounds_write_nothing_outside(bounds, index):
+    args, _ = ragged([100, 100, 100], 1, 2, 32, 40, torch.float32)
+    cu = torch.tensor(bounds, dtype=index).cuda()
+    guarded_calls(args, cu, torch.randn_like(args[2]), torch.randn_like(args[5]))
+
+
+@pytest.mark.gpu
+def test_overlapping_sequences_of_more_chunks_than_an_int_counts():
+    """32768 times all of 2^22 tokens: 2^31 chunks by their bounds, of which there is room for 131071."""
+    t, n = 1 << 22, 65535
+    one = torch.zeros(1, 1, 1, 16, device="cuda", dtype=torch.bfloat16)
+    q = one.expand(1, t, 1, 16)
+    gate = torch.zeros(1, 1, 1, device="cuda").expand(1, t, 1)
+    s0 = torch.ones(n, 1, 16, 16, device="cuda")
+    cu = (torch.arange(n + 1) % 2 * t).to("cuda", torch.int32)
+    guarded_calls((q, q, q, gate, gate, s0), cu, q, s0)
