@@ -257,11 +257,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
             Pair sum[S::kCols / 2];
 #pragma unroll
             for (int j = 0; j < S::kCols / 2; ++j) sum[j] = 0;
-            // the next block's scales are fetched while this one's product is awaited
+            // the next block's scales are fetched while this one's product is awaited (by plain loads: the kernel before this one may
+            // still write them when this one starts, so they are not constant for its whole run)
             float row_scale = 0.0f, col_scale = 0.0f;
             const auto fetch = [&]() {
-                row_scale = __ldg(sp++);
-                if (!kByColumn || q_there) col_scale = __ldg(sq);
+                row_scale = *sp++;
+                if (!kByColumn || q_there) col_scale = *sq;
                 ++sq;
             };
             if (kb0 < kb1) fetch();

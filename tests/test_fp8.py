@@ -534,3 +534,29 @@ def test_compiled():
         return mlt.matmul_fp8(*mlt.quantize_fp8(a), *mlt.quantize_fp8(b, block=(128, 128)))
 
     assert torch.equal(torch.compile(product, backend="aot_eager", fullgraph=True)(x, w), product(x, w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [5, 200, 1100])
+def test_a_call_sees_what_the_one_before_it_wrote(rows):
+    """Kernels start ahead of the end of those before them: a chain of maps through the same few buffers, values, scales and
+    inputs written by one call and read by the next, is what the same chain gives with a wait behind every call."""
+    torch.manual_seed(rows)
+    w = [torch.randn(256, 256, device="cuda").bfloat16() / 16 for _ in range(3)]
+    first = torch.randn(rows, 256, device="cuda").bfloat16()
+
+    def chain(wait):
+        outs, x = [], first
+        for i in range(60):
+            a, sa = mlt.quantize_fp8(x)
+            wait()
+            b, sb = mlt.quantize_fp8(w[i % 3], block=(1 if i % 2 else 128, 128))
+            wait()
+            x = mlt.matmul_fp8(a, sa, b, sb)
+            wait()
+            outs.append(x.clone())
+        return outs
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(chain(lambda: None), want))
