@@ -285,9 +285,9 @@ metal_linalg_status metal_linalg_synchronize(void);
 metal_linalg_status metal_linalg_release_workspaces(uint64_t* bytes_freed);
 
 /* Testing aid, no counterpart in the reference: the next `count` matrices that
- * the grid-parallel blocked QR factors are treated as if one of its tensor-core
- * products had given up on a wait at once (NaN outputs, the error at the next
- * metal_linalg_synchronize). Nothing on the GPU is made to wait, fault or fail. */
+ * the grid-parallel blocked QR factors, or calls of metal_linalg_matmul_fp8, are
+ * treated as if one of their tensor-core products had given up on a wait at once
+ * (NaN outputs, the error at the next metal_linalg_synchronize). Nothing on the GPU is made to wait, fault or fail. */
 void metal_linalg_inject_wait_failures(int count);
 
 /* ---------------------------------------------------------------------------

@@ -45,8 +45,9 @@ namespace metal_linalg {
     // need the memory back after one large factorisation.
     size_t release_workspaces();
     // Testing aid (no GPU is made to wait or fail): the next `count` matrices
-    // of the grid-parallel blocked QR are treated as if a tensor-core product
-    // had given up on a wait: NaN outputs, and the error at synchronize().
+    // of the grid-parallel blocked QR, or 8-bit products, are treated as if a
+    // tensor-core product had given up on a wait: NaN outputs, and the error at
+    // synchronize().
     void  inject_wait_failures(int count);
 
     // -------------------------------------------------------------------------

@@ -58,6 +58,7 @@ struct GemmArgs {
     uint32_t c_dtype;
     uint32_t wide;                     // C's rows (ldq == 1) can be written in 16-byte pieces
     unsigned* status;
+    uint32_t give_up;                  // as if every wait had run out at once: no load or product is issued (inject_wait_failures)
 
     // Tile t's matrix, first row and first column: tiles of a column of C behind one another.
     template <int BN> __device__ __forceinline__ void place(uint32_t t, uint32_t& z, uint32_t& p0, uint32_t& q0) const {
@@ -204,7 +205,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
     const uint32_t kb0 = (uint32_t)((uint64_t)a.kb * rank / a.split), kb1 = (uint32_t)((uint64_t)a.kb * (rank + 1) / a.split);
 
     if (threadIdx.x == 0) {
-        failed_word = 0;
+        failed_word = (int)a.give_up;
         for (int i = 0; i < S::kStages; ++i) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(smem_u32(&full[i])));
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(smem_u32(&empty[i])));
@@ -235,7 +236,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
         const uint32_t row = 32 * quarter + lane;
         float* part_scales = scales + part * 2 * S::kCols;      // of this part's columns, two blocks of k
         uint32_t i = 0;
-        bool ok = true;
+        bool ok = !a.give_up;
         for (uint32_t tile = first; tile < a.tiles; tile += step) {
             const float *sp, *sq;               // this block's first scales of the thread's row, of its columns
             bool q_there = false;               // by column: the four warps of a part fetch a quarter of its columns each
@@ -378,7 +379,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
     if (warp == S::kEpilogueWarps) {            // loads
         if (elect_one()) {
             uint32_t i = 0;                     // blocks of k so far
-            bool ok = true;
+            bool ok = !a.give_up;
             const uint32_t full0 = smem_u32(&full[0]), empty0 = smem_u32(&empty[0]), ring = smem_u32(base);
             uint32_t tile = first, kb = kb0, z, p0, q0;
             if (tile < a.tiles) a.place<BN>(tile, z, p0, q0);
@@ -409,7 +410,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant
         __syncwarp();
     } else if (warp == S::kEpilogueWarps + 1) { // products
         if (elect_one()) {
-            bool ok = true;
+            bool ok = !a.give_up;
             const uint32_t full0 = smem_u32(&full[0]), empty0 = smem_u32(&empty[0]), acc_full0 = smem_u32(&acc_full[0]),
                            acc_empty0 = smem_u32(&acc_empty[0]);
             const uint64_t ring = tile_desc(smem_u32(base));
@@ -592,6 +593,7 @@ void launch_gemm(cudaStream_t stream, int device, const GemmOperand& oa, const G
     const uint32_t size = c_dtype == METAL_LINALG_FLOAT32 ? 4 : 2;
     a.wide = !turned && (uint64_t)n * size % 16 == 0 && (reinterpret_cast<uintptr_t>(c) & 15) == 0;
     a.status = status;
+    a.give_up = take_injected_wait_failure();
     const CUtensorMap mp = tile_map(p, batch, k, kRowsTile), mq = tile_map(q, batch, k, bn);
     const bool by_column = a.q_shift == 0;
     switch (bn) {

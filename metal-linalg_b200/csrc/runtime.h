@@ -121,9 +121,9 @@ void launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t s
     cuda_check(cudaLaunchKernelEx(&cfg, kernel, Params(args)...), "cudaLaunchKernelEx");
 }
 
-// Testing aid: the next `count` matrices that go through the blocked QR behave as if a tensor-core
-// product's bounded wait had run out at once (their products return without touching memory, their
-// outputs are NaN, the context's status word is set). Nothing on the GPU is made to wait or fail.
+// Testing aid: the next `count` matrices that go through the blocked QR, or products in 8-bit floating
+// point, behave as if a tensor-core product's bounded wait had run out at once (their products return
+// without touching memory, or issue nothing; their outputs are NaN, the context's status word is set). Nothing on the GPU is made to wait or fail.
 void inject_wait_failures(int count);
 bool take_injected_wait_failure();
 

@@ -560,3 +560,23 @@ def test_a_call_sees_what_the_one_before_it_wrote(rows):
     want = chain(torch.cuda.synchronize)
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(chain(lambda: None), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("blocks", [(1, 128), (1, 1)])
+@pytest.mark.parametrize("size", [(16, 300, 4096), (33, 200, 1024), (100, 128, 4096), (300, 200, 128), (2304, 2300, 300), (4000, 4000, 256)])
+def test_a_product_that_gives_up_surfaces(size, blocks):
+    """Products that share a tile's k (their clusters exchange NaN) and that do not, one tile a block and several. The failure is
+    made on the host: the kernel starts as if its waits had run out, issues no copy and no product. No GPU waits or faults."""
+    m, n, k = size
+    a, sa = operand(m, k, blocks[0], E4M3, 13)
+    b, sb = operand(n, k, blocks[1], E4M3, 14)
+    want = mlt.matmul_fp8(a, sa, b, sb)
+    _lib.synchronize()
+    _lib.lib.metal_linalg_inject_wait_failures(1)
+    assert mlt.matmul_fp8(a, sa, b, sb).isnan().all()
+    with pytest.raises(RuntimeError, match=r"gave up on a bounded wait \(a copy or a tensor-core product in 8-bit floating point\); the tiles"):
+        _lib.synchronize()
+    _lib.synchronize()                      # reported once
+    assert torch.equal(mlt.matmul_fp8(a, sa, b, sb), want)
+    _lib.synchronize()
