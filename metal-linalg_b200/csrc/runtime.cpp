@@ -183,16 +183,17 @@ void throw_if_a_kernel_gave_up() {
     for (int i = 0; i < n; ++i) {
         const unsigned word = all[i]->take_status();
         if (!word) continue;
-        if (word == kStatusProductWait)
-            throw std::runtime_error("a kernel on GPU " + std::to_string(all[i]->device) + " gave up on a bounded wait (a copy or a "
-                                     "tensor-core product in 8-bit floating point); the tiles of the output concerned are NaN");
-        std::string what = "a kernel on GPU " + std::to_string(all[i]->device) + " gave up on a bounded wait (";
-        if (word & kStatusTensorWait) what += "a tensor-core product of the blocked QR";
-        if ((word & kStatusTensorWait) && (word & kStatusStreamWait)) what += ", ";
-        if (word & kStatusStreamWait) what += "a bulk copy of the streaming small-matrix kernel";
-        what += "); the outputs of the matrices concerned are NaN; last QR enqueued there: batch " +
-                std::to_string(all[i]->last_shape[0]) + " of " + std::to_string(all[i]->last_shape[1]) + " x " +
-                std::to_string(all[i]->last_shape[2]);
+        std::string kinds, outcome;
+        const auto add = [](std::string& to, const char* separator, const std::string& what) { to += (to.empty() ? "" : separator) + what; };
+        if (word & kStatusTensorWait) add(kinds, ", ", "a tensor-core product of the blocked QR");
+        if (word & kStatusStreamWait) add(kinds, ", ", "a bulk copy of the streaming small-matrix kernel");
+        if (word & kStatusProductWait) add(kinds, ", ", "a copy or a tensor-core product in 8-bit floating point");
+        if (word & (kStatusTensorWait | kStatusStreamWait))
+            add(outcome, "; ", "the outputs of the matrices concerned are NaN; last QR enqueued there: batch " +
+                                   std::to_string(all[i]->last_shape[0]) + " of " + std::to_string(all[i]->last_shape[1]) + " x " +
+                                   std::to_string(all[i]->last_shape[2]));
+        if (word & kStatusProductWait) add(outcome, "; ", "the tiles concerned of the 8-bit product's output are NaN");
+        const std::string what = "a kernel on GPU " + std::to_string(all[i]->device) + " gave up on a bounded wait (" + kinds + "); " + outcome;
         throw std::runtime_error(what);
     }
 }

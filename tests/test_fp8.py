@@ -580,3 +580,25 @@ def test_a_product_that_gives_up_surfaces(size, blocks):
     _lib.synchronize()                      # reported once
     assert torch.equal(mlt.matmul_fp8(a, sa, b, sb), want)
     _lib.synchronize()
+
+
+@pytest.mark.gpu
+def test_failures_of_several_kinds_are_all_named():
+    import os
+    a, sa = operand(100, 256, 1, E4M3, 15)
+    x = torch.randn(600, 600, device="cuda")
+    mlt.matmul_fp8(a, sa, a, sa)
+    os.environ["QR_KERNEL"] = "blocked"
+    try:
+        mlt.qr(x)
+        _lib.synchronize()
+        _lib.lib.metal_linalg_inject_wait_failures(2)
+        assert mlt.qr(x)[1].isnan().all() and mlt.matmul_fp8(a, sa, a, sa).isnan().all()
+    finally:
+        os.environ.pop("QR_KERNEL")
+        _lib.lib.metal_linalg_inject_wait_failures(0)
+    with pytest.raises(RuntimeError) as failed:
+        _lib.synchronize()
+    for part in ("blocked QR", "8-bit floating point", "600 x 600", "tiles concerned"):
+        assert part in str(failed.value)
+    _lib.synchronize()
