@@ -863,3 +863,64 @@ def test_overlapping_sequences_of_more_chunks_than_an_int_counts():
     s0 = torch.ones(n, 1, 16, 16, device="cuda")
     cu = (torch.arange(n + 1) % 2 * t).to("cuda", torch.int32)
     guarded_calls((q, q, q, gate, gate, s0), cu, q, s0)
+
+
+# ---------------------------------------------------------------------------
+# Every way in which warps share a chain. Which one a call takes goes by its number of chains (16 value columns of a value head
+# and sequence): with one chain a multiprocessor (148) at most, four warps, forward in 16 bits up to two; then two; backward
+# one beyond two chains a multiprocessor, but for float16 and ragged batches.
+# ---------------------------------------------------------------------------
+
+def recurrence_and_gradients(args, d_o, d_s, cu=None):
+    """In float64, token by token, on the GPU (torch's own operations): a ragged batch's sequences by themselves."""
+    leaves = [x.detach().double().requires_grad_() for x in args]
+    q, k, v, g, beta, s0 = leaves
+    up = v.shape[2] // q.shape[2]
+    spans = [(slice(None), 0, q.shape[1])] if cu is None else [(slice(i, i + 1), a, b) for i, (a, b) in enumerate(zip(cu, cu[1:]))]
+    outs, states = [], []
+    for rows, a, b in spans:
+        s = s0[rows]
+        for t in range(a, b):
+            kt, qt = (x[:, t].repeat_interleave(up, 1)[..., None] for x in (k, q))
+            s = s * g[:, t].exp()[..., None, None]
+            s = s + kt * (beta[:, t, :, None] * (v[:, t] - (kt * s).sum(-2)))[..., None, :]
+            outs.append(q.shape[-1] ** -0.5 * (qt * s).sum(-2))
+        states.append(s)
+    o, s = torch.stack(outs, 1), torch.cat(states)
+    return o.detach(), s.detach(), torch.autograd.grad((o, s), leaves, (d_o.double(), d_s.double()))
+
+
+def check_all(args, dtype, cu=None):
+    leaves = [x.detach().requires_grad_() for x in args]
+    bounds = None if cu is None else torch.tensor(cu, device="cuda", dtype=torch.int32)
+    o, s = mlt.gated_delta_rule(*leaves[:5], initial_state=leaves[5], cu_seqlens=bounds)
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    d_o = torch.randn(o.shape, device="cuda", generator=gen).to(dtype)
+    d_s = 0.3 * torch.randn(s.shape, device="cuda", generator=gen)
+    got = torch.autograd.grad((o, s), leaves, (d_o, d_s), retain_graph=True)
+    want_o, want_s, want = recurrence_and_gradients(args, d_o, d_s, cu)
+    near(o, want_o.cpu(), tolerance(dtype), "o")
+    near(s, want_s.cpu(), F32, "state")
+    for name, x, y in zip(NAMES, got, want):
+        near(x, y.cpu(), tolerance(x.dtype, grad=True), name)
+    assert all(torch.equal(x, y) for x, y in zip(got, torch.autograd.grad((o, s), leaves, (d_o, d_s))))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("chains", [144, 160, 320])
+def test_chains_of_several_chunks(chains, dtype, dk):
+    """Forward by four warps (144; 16 bits: 160), by two (float32: 160; 320); backward by four, two, one (float16: two)."""
+    hv = chains // 16
+    check_all(inputs(2, 215, hv // 2 if hv % 2 == 0 else hv, hv, dk, 128, dtype, seed=chains), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dk", [60, 128])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens", [[130, 0, 215, 64], [3, 130, 64, 0, 70, 215, 129, 1, 66, 100]], ids=len)
+def test_ragged_chains_of_several_chunks(lens, dtype, dk):
+    """96 and 240 chains: four warps a chain, and two."""
+    args, cu = ragged(lens, 2, 4, dk, 96, dtype, seed=len(lens))
+    check_all(args, dtype, cu.tolist())
