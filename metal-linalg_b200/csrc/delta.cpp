@@ -106,7 +106,7 @@ uint64_t carve(Args& a, char* base, bool backward) {
     Carver w{base};
     const uint64_t heads = (uint64_t)a.chunks * a.value_heads;
     if (a.sequences) {
-        a.table = w.take<int>(4ull * a.chunks);
+        a.table = w.take<int>(2ull * a.chunks);
         a.first = w.take<int>((uint64_t)a.sequences + 3);
         a.order = w.take<int>(a.sequences);
     }

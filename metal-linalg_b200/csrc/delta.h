@@ -54,7 +54,7 @@ struct Args {
     uint32_t  row_chunks;        // chunks of a batch row (sequences == 0)
     uint32_t  chunks;            // all of them; an upper bound for a ragged batch
     // workspace
-    int*      table;             // ragged: {first token, tokens, sequence, 0} a chunk
+    int*      table;             // ragged: {first token, tokens} a chunk
     int*      first;             // ragged: [sequences + 3] first chunk of a sequence; then the number of chunks, the tokens
                                  // behind the last sequence's end and those before the first one's start
     int*      order;             // ragged: [sequences] the sequences, long ones first

@@ -12,7 +12,7 @@
 //     dg = the sums of dG from the chunk's end
 //
 // S and D come from the forward's preparation and sequential pass, run again: keeping them from the forward would hold
-// 112 KB a chunk and head for the time between (the inputs are 48 KB in bfloat16).
+// 109 kB a chunk and head for the time between (the inputs are 49 kB in bfloat16).
 #include "common.cuh"
 #include "delta.h"
 #include "delta_tiles.cuh"

@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kIndexThreads) delta_index_kernel(const Args a
             atomicAdd(&classes[class_of(mine)], 1);
             for (int c = first; c < last; ++c) {
                 const int t = begin + (c - first) * kChunk;
-                reinterpret_cast<int4*>(a.table)[c] = make_int4(t, min(kChunk, end - t), (int)s, 0);
+                reinterpret_cast<int2*>(a.table)[c] = make_int2(t, min(kChunk, end - t));
             }
         }
         __syncthreads();
@@ -106,7 +106,8 @@ __global__ void __launch_bounds__(kIndexThreads) delta_index_kernel(const Args a
 // block's time, against twice the blocks), A from it in place, its inverse by blocks of 16 (diagonal blocks by
 // substitution, a column a lane; T_ij = -T_ii sum_m A_im T_mj outward from the diagonal on the tensor cores, whose
 // transposed inner product is the outer one's operand as it stands) and T as fragments for the products that follow.
-// What bounds it is latency, so T takes the place of K in shared memory and five blocks or more fit a multiprocessor.
+// What bounds it is latency, so T takes the place of K in shared memory and five blocks or more fit a multiprocessor (four of
+// float32 at 128 key columns).
 // 64 chunks of 16 heads of 128 (bfloat16): 27 us; 128 of them 44.
 constexpr int kPrepThreads = 128;
 constexpr int kLdA = 72;            // row length of A and T in shared memory: 64-bit reads of a fragment meet no bank twice

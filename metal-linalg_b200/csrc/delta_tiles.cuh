@@ -386,17 +386,17 @@ __device__ __forceinline__ void mma_triangle(float (&acc)[N][4], const TileTf32&
 // ---------------------------------------------------------------------------
 
 struct Chunk {
-    int batch, token, rows, seq;     // rows 0: no such chunk
+    int batch, token, rows;          // rows 0: no such chunk
 };
 __device__ __forceinline__ Chunk chunk_at(const Args& a, uint32_t c) {
     Chunk r;
     if (a.sequences) {
-        if (c >= (uint32_t)a.first[a.sequences]) return {0, 0, 0, 0};
-        const int4 e = reinterpret_cast<const int4*>(a.table)[c];
-        r = {0, e.x, e.y, e.z};
+        if (c >= (uint32_t)a.first[a.sequences]) return {0, 0, 0};
+        const int2 e = reinterpret_cast<const int2*>(a.table)[c];
+        r = {0, e.x, e.y};
     } else {
         const uint32_t b = c / a.row_chunks, i = c - b * a.row_chunks;
-        r = {(int)b, (int)(i * kChunk), (int)min((uint32_t)kChunk, a.tokens - i * kChunk), (int)b};
+        r = {(int)b, (int)(i * kChunk), (int)min((uint32_t)kChunk, a.tokens - i * kChunk)};
     }
     return r;
 }
