@@ -924,3 +924,44 @@ def test_ragged_chains_of_several_chunks(lens, dtype, dk):
     """96 and 240 chains: four warps a chain, and two."""
     args, cu = ragged(lens, 2, 4, dk, 96, dtype, seed=len(lens))
     check_all(args, dtype, cu.tolist())
+
+
+@pytest.mark.gpu
+def test_what_no_sequence_holds_is_not_read():
+    """Tokens of no sequence, and the inputs of a step's padding rows, may hold anything."""
+    q, k, v, g, beta, s0 = inputs(1, 300, 1, 2, 32, 48, torch.float32, n=2)
+    cu = torch.tensor([70, 130, 210], device="cuda")
+    d_o, d_s = torch.randn_like(v), torch.randn_like(s0)
+
+    def run(*args, d_o):
+        leaves = [x.detach().clone().requires_grad_() for x in args]
+        o, s = mlt.gated_delta_rule(*leaves[:5], initial_state=leaves[5], cu_seqlens=cu)
+        return (o, s, *torch.autograd.grad((o, s), leaves, (d_o, d_s)))
+
+    want = run(q, k, v, g, beta, s0, d_o=d_o)
+    bad = [x.clone() for x in (q, k, v, g, beta, d_o)]
+    for i, x in enumerate(bad):
+        x[:, :70] = (math.nan, math.inf, -math.inf)[i % 3]
+        x[:, 210:] = (math.inf, math.nan)[i % 2]
+    assert all(torch.equal(x, y) for x, y in zip(run(*bad[:5], s0, d_o=bad[5]), want))
+    q, k, v, g, beta, s0 = inputs(3, 1, 1, 2, 32, 48, torch.float32)
+    slots = torch.tensor([1, -1, 0], device="cuda")
+    for x in (q, k, v, g, beta):
+        x[1] = math.nan
+    state = s0.clone()
+    o = mlt.gated_delta_step(q, k, v, g, beta, state, slots=slots)
+    assert not o[1].any() and state.isfinite().all() and o.isfinite().all() and torch.equal(state[2], s0[2])
+
+
+@pytest.mark.gpu
+def test_decoding_in_inference_mode():
+    args = inputs(2, 70, 1, 2, 32, 32, torch.bfloat16)
+    want_o, want_s = mlt.gated_delta_rule(*args[:5], initial_state=args[5])
+    last = [x[:, -1:] for x in args[:5]]
+    with torch.no_grad():
+        pool = want_s.clone()
+        want = mlt.gated_delta_step(*last, pool)
+    with torch.inference_mode():
+        o, state = mlt.gated_delta_rule(*args[:5], initial_state=args[5])
+        got = mlt.gated_delta_step(*last, state)
+    assert torch.equal(o, want_o) and torch.equal(got, want) and torch.equal(state, pool)

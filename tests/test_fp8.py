@@ -602,3 +602,42 @@ def test_failures_of_several_kinds_are_all_named():
     for part in ("blocked QR", "8-bit floating point", "600 x 600", "tiles concerned"):
         assert part in str(failed.value)
     _lib.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block", [1, 128])
+def test_quantize_past_32_bits(block):
+    """Matrices of more than 2^31 elements, straight and transposed: their last rows as if they were alone."""
+    x = torch.empty(70000, 33000, device="cuda", dtype=torch.bfloat16)
+    x[-300:] = torch.randn(300, 33000, device="cuda").bfloat16()
+    rows = 70000 % 128 + 128                    # whole blocks from the first row on
+    x[-rows:] = torch.randn(rows, 33000, device="cuda").bfloat16()
+    values, scales = mlt.quantize_fp8(x, block=(block, 128))
+    v, s = mlt.quantize_fp8(x[-rows:], block=(block, 128))
+    assert torch.equal(values[-rows:].view(torch.uint8), v.view(torch.uint8)) and torch.equal(scales[-s.shape[0]:], s)
+    del values, scales
+    values, scales = mlt.quantize_fp8(x, block=(block, 128), transpose=True)
+    v, s = mlt.quantize_fp8(x[-rows:], block=(block, 128), transpose=True)
+    assert torch.equal(values[:, -rows:].contiguous().view(torch.uint8), v.contiguous().view(torch.uint8))
+    assert torch.equal(scales[:, -s.shape[1]:], s)
+
+
+@pytest.mark.gpu
+def test_matmul_past_32_bits():
+    """A product of more than 2^31 elements, and operands of more than 2^31 bytes: their last rows as if they were alone (the
+    same tiles, so the same bits)."""
+    a, sa = operand(47104, 100, 1, E4M3, 16)
+    b, sb = operand(47104, 100, 128, E4M3, 17)
+    c = mlt.matmul_fp8(a, sa, b, sb)
+    check_product(c[-200:, -500:], spread(a, sa)[-200:], spread(b, sb)[-500:], 100)
+    check_product(c[:100, -500:], spread(a, sa)[:100], spread(b, sb)[-500:], 100)
+    del c
+    a = torch.zeros(270000, 8192, device="cuda", dtype=torch.uint8).view(E4M3)
+    one, s_one = operand(256, 8192, 1, E4M3, 18)
+    a[-256:] = one
+    sa = torch.ones(270000, 64, device="cuda")
+    sa[-256:] = s_one
+    b, sb = operand(64, 8192, 128, E4M3, 19)
+    c = mlt.matmul_fp8(a, sa, b, sb, out_dtype=torch.float32)
+    check_product(c[-256:], spread(one, s_one), spread(b, sb), 8192)
+    assert not c[:-256].any()
