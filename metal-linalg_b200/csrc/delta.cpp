@@ -34,7 +34,9 @@ void check_shape(const char* who, const metal_linalg_delta& p) {
 void check_sequences(const char* who, const metal_linalg_delta& p) {
     if (p.sequences && p.batch != 1) refuse(who, "batch must be 1 where cu_seqlens names the sequences");
     if ((p.sequences ? p.sequences : p.batch) > 65535) refuse(who, "at most 65535 sequences");
-    if ((uint64_t)p.batch * ((uint64_t)p.tokens + kChunk) / kChunk >= 1ull << 30) refuse(who, "too many tokens");
+    const uint64_t chunks = (uint64_t)p.batch * ((uint64_t)p.tokens + kChunk) / kChunk + p.sequences;
+    // (2^32 chunks and heads: a workspace of 400 TB and more, whose size so never passes 64 bits)
+    if (chunks >= 1ull << 30 || chunks * p.value_heads >= 1ull << 32) refuse(who, "too many tokens");
 }
 
 // Every pointer is on one GPU, which is returned.

@@ -161,6 +161,17 @@ def test_c_entries_refuse_without_a_gpu():
         assert lib.metal_linalg_gated_delta_rule(problem(), None, None, None, 0) == _lib.RUNTIME_ERROR
 
 
+def test_workspaces_of_more_than_64_bits_are_refused():
+    """A size that ran over would be one that a caller's workspace seems to have."""
+    from metal_linalg_torch._delta import _PROBLEM
+    size = lambda b, t, hv, seqs=0: _lib.lib.metal_linalg_gated_delta_rule_workspace_bytes(  # noqa: E731
+        _PROBLEM.pack(b, t, hv, hv, 128, 256, seqs, 0, 4, 1.0, -1, 0, *[0] * 7, *[0] * 15), 1)
+    for bad in ((65535, 1 << 19, 65535), (1, (1 << 30) - 1, 65535), (1, (1 << 30) - 1, 65535, 65535), (65535, 1 << 12, 2048)):
+        assert size(*bad) == 0 and "too many tokens" in _lib.last_error()
+    chunk = size(1, 128, 1) - size(1, 64, 1)
+    assert size(1, 1 << 24, 64) == chunk * (1 << 18) * 64 and size(65535, 64, 1) == chunk * 65535
+
+
 # ---------------------------------------------------------------------------
 # Values
 # ---------------------------------------------------------------------------
