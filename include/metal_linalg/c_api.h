@@ -147,7 +147,8 @@ typedef enum metal_linalg_dtype {
  * value_dim] have element type `dtype` (float32, bfloat16 or float16), g and
  * beta [batch, tokens, value_heads] are float32. The last dimension of q, k and
  * v is contiguous; *_stride are the elements between batches, tokens and heads.
- * key_dim <= 128, value_dim <= 256, value_heads a multiple of heads.
+ * key_dim <= 128, value_dim <= 256, value_heads a multiple of heads and at most
+ * 65535, tokens below 2^30, at most 65535 sequences (or batch rows).
  *
  * Sequences: with `sequences` 0 every batch row is one. Otherwise batch is 1 and
  * sequence i is the tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (index_bytes 4:

@@ -232,9 +232,9 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, cu_seq
     Each batch row is a sequence. With ``cu_seqlens`` (int32 or int64, on the GPU, N + 1 values from 0 on, none falling) B is
     1 and sequence ``i`` is the tokens ``cu_seqlens[i] .. cu_seqlens[i + 1] - 1``; a sequence may be empty, and tokens of no
     sequence give zeros. ``initial_state`` [B or N, HV, Dk, Dv] (float32; default zero) is where each starts;
-    ``final_state`` has its shape. ``o`` has v's shape and type.
+    ``final_state`` has its shape. ``o`` has v's shape and type. At most 65535 sequences, fewer than 2 ** 30 tokens each.
 
-    Differentiable once in q, k, v, g, beta and initial_state, through both results.
+    Differentiable once in q, k, v, g, beta and initial_state, through both results (not in forward mode).
     """
     name = "gated_delta_rule"
     b, t, h, dk, hv, dv = _check(name, q, k, v, g, beta)
@@ -308,7 +308,7 @@ def gated_delta_step(q, k, v, g, beta, state, *, slots=None, scale=None):
     The inputs are `gated_delta_rule`'s (T is 1, or the tokens of a draft). ``state`` is a pool [S, HV, Dk, Dv] of float32
     states, each contiguous (a layer's part of a larger cache is fine). Row ``b`` uses slot ``slots[b]`` (int32 or int64, on
     the GPU; default: slot ``b``). A row whose slot is not one of the pool's, -1 say, is padding: its outputs are zero and no
-    state changes. Rows that name the same slot run one after another, in their order. Not differentiable.
+    state changes. Rows that name the same slot run one after another, in their order. At most 65535 rows. Not differentiable.
     """
     name = "gated_delta_step"
     b, t, h, dk, hv, dv = _check(name, q, k, v, g, beta)

@@ -261,6 +261,7 @@ def linear_fp8(x, w):
     x is quantised with a scale for 128 values of a row, w with one for each 128 x 128. The gradients are the products of
     operands quantised along the dimension they are summed over: ``dx = dy @ w`` from dy's rows and w's 128 x 128
     blocks, ``dw = dy.mT @ x`` from both in blocks of 128 along the tokens. Quantisation itself counts as the identity.
+    Differentiable once, not in forward mode.
     """
     name = "linear_fp8"
     _on_gpu(name, "x", x)
