@@ -219,6 +219,7 @@ metal_linalg_status metal_linalg_gated_delta_step(const metal_linalg_delta* p, v
  * largest value (448 or 57344), value = x / scale, a float32 rounded to the nearest, ties to even.
  * scales [batch, ceil(rows / block_rows), ceil(cols / 128)]. A block with a NaN or an
  * infinity stands for NaN throughout. (A transposed matrix is given by its strides.)
+ * rows and cols are below 2^30, a matrix below 2^38 elements.
  * device: the GPU that every pointer is on, vouched for by the caller, or -1: the call
  * looks each pointer up (about 0.3 us a pointer) and refuses those that are not on one GPU. */
 metal_linalg_status metal_linalg_quantize_fp8(const void* x, metal_linalg_dtype dtype, uint32_t batch, uint32_t rows,
@@ -241,6 +242,7 @@ typedef struct metal_linalg_fp8_operand {
 
 /* c [batch, m, n] = a [batch, m, k] b [batch, n, k]^T (float32, bfloat16 or float16, contiguous):
  * products of 128 along k on the tensor cores, times both blocks' scales and summed in float32.
+ * m, n and k are below 2^30, c below 2^28 tiles of 128 x 16 to 128 x 256.
  * device: as for metal_linalg_quantize_fp8. */
 metal_linalg_status metal_linalg_matmul_fp8(const metal_linalg_fp8_operand* a, const metal_linalg_fp8_operand* b,
                                             uint32_t batch, uint32_t m, uint32_t n, uint32_t k, void* c,
